@@ -174,6 +174,109 @@ int wf_gemm_w8a8_act(const void* xq, const float* x_scale, const void* wq, const
                      void* y, int M, int N, int K, int64_t y_row_stride, int qtype, int scale_mode, int activation,
                      void* stream);
 
+/* --------------------------------------------------- paged K/V cache */
+
+/* A pool of K and V pages of one layer.  Page p holds `page_size` rows (token
+ * positions) of each of `heads` K/V heads, 128 elements a row; strides are
+ * {page, head, row} in elements and multiples of 16 bytes.  dtype
+ * WF_DTYPE_BF16: bf16 rows, scales NULL.  WF_DTYPE_E4M3 / WF_DTYPE_S8: one
+ * byte an element and an f32 scale per row, k_scale[page * k_scale_stride[0] +
+ * head * k_scale_stride[1] + row]; a row's value is code * scale. */
+typedef struct wf_kv_pages {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t n_pages;
+  int32_t page_size;
+  int32_t heads;
+  int32_t head_dim; /* 128 */
+  int32_t dtype;
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t k_scale_stride[2];
+  int64_t v_scale_stride[2];
+} wf_kv_pages;
+
+/* Sequences over such a pool, all on the device: position p of sequence b lies
+ * in page table[b * table_stride + p / page_size], row p % page_size.  Packed
+ * rows [cu[b], cu[b + 1]) are the newest of sequence b: row i of n sits at
+ * position lens[b] - n + i.  Rows of [0, rows) behind cu[seqs] belong to no
+ * sequence.  A page id outside the pool, or a position past max_pages, raises
+ * bit 9 of the status word; it is not written, and counts as absent (the
+ * attention) or zero (the read) when read. */
+typedef struct wf_kv_batch {
+  const int32_t* table; /* [seqs, max_pages] */
+  int64_t table_stride;
+  const int32_t* cu;   /* [seqs + 1], non-decreasing */
+  const int32_t* lens; /* [seqs], each at least its packed rows (earlier rows have no position: not written) */
+  int32_t seqs;
+  int32_t max_pages;
+  int64_t rows;
+} wf_kv_batch;
+
+/* Writes the packed rows k, v (bf16, strides {row, head}) to their positions.
+ * 8-bit pages: per row a = max(max|x|, 2^-100), scale = a / Q (Q = 448 e4m3,
+ * 127 s8), code nearest to x * Q / a with ties to even; a row with a NaN or an
+ * infinity gets scale NaN and codes 0.  Where two packed rows of one call land
+ * in one slot (a page listed twice) the later row is kept.  The per-token,
+ * per-head form of the codec that the reference applies to whole tensors
+ * (wave_rt/denoiser/exchange/common.py:143-150), at the page's own place
+ * instead of a transport buffer (paged.py:120-145). */
+int wf_paged_kv_write(const wf_kv_pages* pages, const wf_kv_batch* batch, const void* k, const void* v,
+                      const int64_t* k_stride, const int64_t* v_stride, void* stream);
+
+/* Reads the same positions back as bf16(code * scale) into packed rows (strides
+ * {row, head}); with lens the sequences' lengths and cu their prefix sums it
+ * reads whole sequences.  Rows behind cu[seqs] are left as they were. */
+int wf_paged_kv_read(const wf_kv_pages* pages, const wf_kv_batch* batch, void* k, void* v, const int64_t* k_stride,
+                     const int64_t* v_stride, void* stream);
+
+/* O = softmax(Q K^T * softmax_scale) V of the packed query rows q, o [rows, H,
+ * 128] bf16 (strides {row, head}) over the pages of their sequences; query head
+ * h reads K/V head h / (H / pages->heads).  A row at position p of a sequence of
+ * length len sees key k when k < hi and (k < sink or k >= hi - window), with
+ *   hi = min(len, (p / block + 1) * block), or len when block is 0;
+ * window 0 keeps every key below hi.  block 1 is causal; block = the chunk's
+ * tokens is the block-causal mask of a chunk over clean pages, and sink/window
+ * the anchor and working pages of wave_rt/denoiser/exchange/common.py:70-91,
+ * read where they lie instead of from an assembled buffer (paged.py:191-255).
+ * A row that sees nothing gives zeros.  lse (f32 [rows, H] dense, or NULL)
+ * receives the natural log of the sum of exponentials, -inf for such rows.
+ * Keys that no row of the call sees may hold anything, NaN included; a
+ * non-finite V row that some query sees can also reach other queries that do
+ * not.  max_new and max_len are upper bounds of the sequences' packed rows and
+ * lengths: they choose how the work is cut, never what is computed.
+ * workspace: wf_paged_attn_workspace bytes of device memory, 16-byte aligned,
+ * used by this call alone until it has run (NULL when that is 0). */
+int wf_paged_attn(const wf_kv_pages* pages, const wf_kv_batch* batch, const void* q, const int64_t* q_stride, void* o,
+                  const int64_t* o_stride, float* lse, int H, int block, int window, int sink, int64_t max_new,
+                  int64_t max_len, float softmax_scale, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace the same call needs (host arithmetic only), or -1. */
+int64_t wf_paged_attn_workspace(const wf_kv_pages* pages, const wf_kv_batch* batch, int H, int64_t max_new,
+                                int64_t max_len);
+
+/* Cross attention: O = softmax(Q K^T * softmax_scale) V of q, o [batch, Lq, H,
+ * 128] bf16 against states k, v [states, Lk, kv_heads, 128] bf16 (strides
+ * {batch, token, head} in elements, multiples of 8) of another length.  Query
+ * entry b reads states kv_index[b] (int32 on the device; NULL: b, or 0 when
+ * there is one).  Keys k < kv_lens[n] (NULL: all) with key_mask[n *
+ * mask_stride + k] != 0 (NULL: all) count; the others may hold anything.  A
+ * query left without keys gives zeros.  lse f32 [batch, Lq, H] dense or NULL.
+ * The text cross attention of naive_rt/rolling_forcing/wan/modules/model.py:
+ * 158-196, which the reference leaves on torch SDPA over the padded text
+ * (wave_rt/runtime/backend.py:215-219).  An index outside the states raises
+ * bit 9 of the status word and leaves its queries without keys. */
+int wf_cross_attn(const void* q, const void* k, const void* v, void* o, float* lse, int batch, int Lq, int states,
+                  int Lk, int H, int kv_heads, int D, const int64_t* q_stride, const int64_t* k_stride,
+                  const int64_t* v_stride, const int64_t* o_stride, const int32_t* kv_index, const int32_t* kv_lens,
+                  const uint8_t* key_mask, int64_t mask_stride, float softmax_scale, void* workspace,
+                  int64_t workspace_bytes, void* stream);
+
+/* Bytes of workspace the same call needs (host arithmetic only), or -1. */
+int64_t wf_cross_attn_workspace(int batch, int Lq, int states, int Lk, int H, int kv_heads);
+
 /* ------------------------------------------------------ context assembly */
 
 #define WF_SEG_COPY 0    /* bf16 rows copied */

@@ -50,6 +50,22 @@ class KvPublishDst(C.Structure):
                 ("scales_v", C.c_void_p)]
 
 
+class KvPagesDesc(C.Structure):
+    """wf_kv_pages (include/wfk.h)."""
+
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("n_pages", C.c_int64), ("page_size", C.c_int32), ("heads", C.c_int32), ("head_dim", C.c_int32),
+                ("dtype", C.c_int32), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3),
+                ("k_scale_stride", C.c_int64 * 2), ("v_scale_stride", C.c_int64 * 2)]
+
+
+class KvBatchDesc(C.Structure):
+    """wf_kv_batch (include/wfk.h)."""
+
+    _fields_ = [("table", C.c_void_p), ("table_stride", C.c_int64), ("cu", C.c_void_p), ("lens", C.c_void_p),
+                ("seqs", C.c_int32), ("max_pages", C.c_int32), ("rows", C.c_int64)]
+
+
 PUBLISH_MAX_STAGES, PUBLISH_MAX_DST = 8, 8
 
 # name -> (restype, argtypes)
@@ -85,6 +101,14 @@ _SIGS = {
     "wf_qk_norm_rope_publish": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _i64, _i64, _f32,
                                        C.POINTER(KvPublishDst), C.POINTER(C.c_int32), _i32, _vp]),
     "wf_rms_norm": (_i32, [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _f32, _vp]),
+    "wf_paged_kv_write": (_i32, [C.POINTER(KvPagesDesc), C.POINTER(KvBatchDesc), _vp, _vp, _pi64, _pi64, _vp]),
+    "wf_paged_kv_read": (_i32, [C.POINTER(KvPagesDesc), C.POINTER(KvBatchDesc), _vp, _vp, _pi64, _pi64, _vp]),
+    "wf_paged_attn": (_i32, [C.POINTER(KvPagesDesc), C.POINTER(KvBatchDesc), _vp, _pi64, _vp, _pi64, _vp, _i32, _i32,
+                             _i32, _i32, _i64, _i64, _f32, _vp, _i64, _vp]),
+    "wf_paged_attn_workspace": (_i64, [C.POINTER(KvPagesDesc), C.POINTER(KvBatchDesc), _i32, _i64, _i64]),
+    "wf_cross_attn": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _pi64, _pi64, _pi64,
+                             _pi64, _vp, _vp, _vp, _i64, _f32, _vp, _i64, _vp]),
+    "wf_cross_attn_workspace": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32]),
     "wf_ipc_export": (_i32, [_vp, C.POINTER(C.c_uint8), C.POINTER(_u64)]),
     "wf_ipc_open": (_i32, [C.POINTER(C.c_uint8), C.POINTER(_vp)]),
     "wf_ipc_close": (_i32, [_vp]),

@@ -17,6 +17,7 @@ enum StatusCode : uint32_t {
   ST_FLAG_TIMEOUT = 1u << 6,
   ST_DRAIN_TIMEOUT = 1u << 7,
   ST_ATTN_CONVERT = 1u << 8,
+  ST_PAGE_ID = 1u << 9,  // a page id outside the pool, or a length past the page table
 };
 
 static __device__ unsigned int g_status;  // one word per translation unit

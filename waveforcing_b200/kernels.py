@@ -516,3 +516,219 @@ def rms_norm(x: torch.Tensor, w: torch.Tensor, eps: float) -> torch.Tensor:
     L.check(L.lib().wf_rms_norm(x.data_ptr(), x.stride(0), w.data_ptr(), out.data_ptr(), out.stride(0), rows, dim,
                                 eps, _stream()), "wf_rms_norm")
     return out
+
+
+# ------------------------------------------------- paged K/V cache, cross attention
+def _strides(t: torch.Tensor, n: int) -> tuple:
+    """The first n strides; a dim of one element, whose stride torch leaves open, gets 16."""
+    return tuple(st if sz > 1 else 16 for st, sz in zip(t.stride()[:n], t.shape))
+
+
+_PAGE_DTYPES = {torch.bfloat16: L.WF_DTYPE_BF16, torch.uint8: L.WF_DTYPE_E4M3, torch.int8: L.WF_DTYPE_S8}
+
+
+class KVPages:
+    """K and V pages of one layer: ``k``, ``v`` [pages, kv_heads, page_size, 128]
+    as bf16 rows, e4m3 codes (uint8) or signed 8-bit codes (int8), the 8-bit
+    forms with f32 ``k_scale``, ``v_scale`` [pages, kv_heads, page_size] (a row's
+    value is code * scale).  Strides are free (multiples of 16 bytes, the 128
+    elements of a row and the scales of a page contiguous), so pages stored
+    token-major are passed as a transposed view."""
+
+    __slots__ = ("k", "v", "k_scale", "v_scale", "kv_dtype")
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None,
+                 v_scale: torch.Tensor | None = None) -> None:
+        _check(k.dtype in _PAGE_DTYPES and v.dtype == k.dtype, "KVPages: k and v must both be bf16, uint8 (e4m3) or int8")
+        _check(k.dim() == 4 and v.shape == k.shape and v.device == k.device and k.stride(3) == v.stride(3) == 1,
+               "KVPages: k and v must be [pages, kv_heads, page_size, 128] with contiguous rows, on one device")
+        self.kv_dtype = _PAGE_DTYPES[k.dtype]
+        if self.kv_dtype == L.WF_DTYPE_BF16:
+            _check(k_scale is None and v_scale is None, "KVPages: bf16 pages take no scales")
+        else:
+            for s in (k_scale, v_scale):
+                _check(s is not None and s.dtype == torch.float32 and s.shape == k.shape[:3] and s.device == k.device
+                       and (s.stride(2) == 1 or s.shape[2] == 1),
+                       "KVPages: 8-bit pages need f32 scales [pages, kv_heads, page_size], contiguous in a page")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+
+    @classmethod
+    def empty(cls, pages: int, kv_heads: int, page_size: int, dtype: torch.dtype = torch.bfloat16,
+              device="cuda") -> "KVPages":
+        """A zeroed pool of pages."""
+        k, v = (torch.zeros((pages, kv_heads, page_size, 128), dtype=dtype, device=device) for _ in range(2))
+        if dtype == torch.bfloat16:
+            return cls(k, v)
+        return cls(k, v, *(torch.zeros((pages, kv_heads, page_size), device=device) for _ in range(2)))
+
+    def _desc(self) -> L.KvPagesDesc:
+        k, v, ks, vs = self.k, self.v, self.k_scale, self.v_scale
+        P, G, ps, D = k.shape
+        if ks is None:
+            return L.KvPagesDesc(k.data_ptr(), v.data_ptr(), None, None, P, ps, G, D, self.kv_dtype, _strides(k, 3),
+                                 _strides(v, 3))
+        return L.KvPagesDesc(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), P, ps, G, D, self.kv_dtype,
+                             _strides(k, 3), _strides(v, 3), _strides(ks, 2), _strides(vs, 2))
+
+
+def _no_grad(what: str, *ts: torch.Tensor) -> None:
+    _check(not (torch.is_grad_enabled() and any(t.requires_grad for t in ts)),
+           f"{what}: no gradient is computed; call it under torch.no_grad()")
+
+
+def _on(dev: torch.device, fn, *args) -> int:
+    """fn(*args, stream) on ``dev``'s current stream, with ``dev`` the current device."""
+    LAUNCHES[0] += 1
+    if dev.index == torch.cuda.current_device():
+        return fn(*args, torch.cuda.current_stream().cuda_stream)
+    with torch.cuda.device(dev):
+        return fn(*args, torch.cuda.current_stream().cuda_stream)
+
+
+def _batch_desc(what: str, table: torch.Tensor, cu: torch.Tensor, lens: torch.Tensor, rows: int, dev) -> L.KvBatchDesc:
+    B = lens.shape[0]
+    _check(table.dtype == cu.dtype == lens.dtype == torch.int32 and lens.dim() == cu.dim() == 1 and table.dim() == 2
+           and table.shape[0] == B and table.shape[1] >= 1 and cu.shape[0] == B + 1 and lens.is_contiguous()
+           and cu.is_contiguous() and (table.stride(1) == 1 or table.shape[1] == 1),
+           f"{what}: page_table [B, max_pages], cu_new [B + 1] and seq_lens [B] must be int32 with contiguous rows")
+    _check(table.device == cu.device == lens.device == dev, f"{what}: all tensors must be on one device")
+    return L.KvBatchDesc(table.data_ptr(), table.stride(0), cu.data_ptr(), lens.data_ptr(), B, table.shape[1], rows)
+
+
+def _packed(what: str, t: torch.Tensor, heads: int) -> None:
+    _check(t.dim() == 3 and t.shape[1] == heads and t.shape[2] == 128 and t.dtype == torch.bfloat16
+           and t.stride(2) == 1, f"{what}: packed rows must be bf16 [rows, {heads}, 128] with a contiguous last dim")
+
+
+def paged_kv_write(pages: KVPages, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, cu_new: torch.Tensor,
+                   seq_lens: torch.Tensor) -> None:
+    """Write the packed new rows k, v bf16 [rows, kv_heads, 128] of a batch into
+    their pages, quantised with a scale per token and head where the pages are
+    8-bit.  Rows [cu_new[b], cu_new[b + 1]) are the last of sequence b's
+    seq_lens[b] positions, and position p lies in page page_table[b, p //
+    page_size].  All three are int32 on the device, so one captured call serves
+    every step.  A slot that two rows land in keeps the later row."""
+    _packed("paged_kv_write", k, pages.k.shape[1])
+    _packed("paged_kv_write", v, pages.k.shape[1])
+    _check(k.shape == v.shape, "paged_kv_write: k and v must have the same number of rows")
+    _no_grad("paged_kv_write", k, v)
+    dev = pages.k.device
+    _check(k.device == v.device == dev, "paged_kv_write: all tensors must be on one device")
+    batch = _batch_desc("paged_kv_write", page_table, cu_new, seq_lens, k.shape[0], dev)
+    _need_cuda(k)
+    L.check(_on(dev, L.lib().wf_paged_kv_write, pages._desc(), batch, k.data_ptr(), v.data_ptr(),
+                L.i64_array(_strides(k, 2)), L.i64_array(_strides(v, 2))), "wf_paged_kv_write")
+
+
+def paged_kv_read(pages: KVPages, page_table: torch.Tensor, cu_new: torch.Tensor, seq_lens: torch.Tensor,
+                  rows: int | None = None, out_k: torch.Tensor | None = None, out_v: torch.Tensor | None = None):
+    """The inverse of paged_kv_write: positions seq_lens[b] - n_b .. of each
+    sequence, n_b = cu_new[b + 1] - cu_new[b], as packed bf16 rows [rows,
+    kv_heads, 128] (whole sequences when cu_new is the prefix sum of seq_lens).
+    ``rows`` (or the outputs' size) is the packed total; rows behind cu_new[-1]
+    are not written."""
+    G = pages.k.shape[1]
+    dev = pages.k.device
+    _check((out_k is None) == (out_v is None), "paged_kv_read: give both outputs or neither")
+    if out_k is None:
+        _check(rows is not None and rows >= 0, "paged_kv_read: rows is needed without outputs")
+        out_k, out_v = (torch.empty((rows, G, 128), dtype=torch.bfloat16, device=dev) for _ in range(2))
+    _packed("paged_kv_read", out_k, G)
+    _packed("paged_kv_read", out_v, G)
+    _check(out_k.shape == out_v.shape and (rows is None or rows == out_k.shape[0]) and out_k.device == dev
+           and out_v.device == dev, "paged_kv_read: outputs must both hold `rows` rows on the pages' device")
+    batch = _batch_desc("paged_kv_read", page_table, cu_new, seq_lens, out_k.shape[0], dev)
+    _need_cuda(out_k)
+    L.check(_on(dev, L.lib().wf_paged_kv_read, pages._desc(), batch, out_k.data_ptr(), out_v.data_ptr(),
+                L.i64_array(_strides(out_k, 2)), L.i64_array(_strides(out_v, 2))), "wf_paged_kv_read")
+    return out_k, out_v
+
+
+def paged_attention(q: torch.Tensor, pages: KVPages, page_table: torch.Tensor, cu_new: torch.Tensor,
+                    seq_lens: torch.Tensor, *, max_new: int | None = None, max_len: int | None = None, block: int = 0,
+                    window: int = 0, sink: int = 0, softmax_scale: float | None = None,
+                    out: torch.Tensor | None = None, return_lse: bool = False):
+    """Attention of packed new rows q bf16 [rows, H, 128] over their sequences'
+    pages (already holding the rows' own K/V, paged_kv_write); the batch is
+    described as there.  H is a multiple of the pages' K/V heads.
+
+    A row at position p sees keys below hi = min(len, (p // block + 1) * block)
+    (block 0: the whole sequence; 1: causal; a chunk's tokens: block-causal);
+    with window > 0 only the last ``window`` of those and the first ``sink``.
+    Rows that see nothing are zero.  ``max_new`` / ``max_len`` bound a
+    sequence's new rows and length where the caller knows them; they steer the
+    split of the work only.  Rows behind cu_new[-1] are not written.  With
+    ``return_lse`` also the f32 log-sum-exp [rows, H]."""
+    _check(q.dim() == 3, "paged_attention: q must be packed rows [rows, H, 128]")
+    rows, H = q.shape[:2]
+    _packed("paged_attention", q, H)
+    _no_grad("paged_attention", q)
+    dev = q.device
+    G, ps = pages.k.shape[1:3]
+    _check(pages.k.device == dev, "paged_attention: all tensors must be on one device")
+    _check(H % G == 0, "paged_attention: query heads must be a multiple of the K/V heads")
+    batch = _batch_desc("paged_attention", page_table, cu_new, seq_lens, rows, dev)
+    if out is None:
+        out = torch.empty((rows, H, 128), dtype=torch.bfloat16, device=dev)
+    _packed("paged_attention", out, H)
+    _check(out.shape == q.shape and out.device == dev, "paged_attention: out must match q")
+    _need_cuda(q)
+    lse = torch.empty((rows, H), dtype=torch.float32, device=dev) if return_lse else None
+    max_new = rows if max_new is None else int(max_new)
+    max_len = page_table.shape[1] * ps if max_len is None else int(max_len)
+    desc = pages._desc()
+    lib = L.lib()
+    need = lib.wf_paged_attn_workspace(desc, batch, H, max_new, max_len)
+    ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need > 0 else None
+    scale = 1.0 / math.sqrt(128) if softmax_scale is None else float(softmax_scale)
+    L.check(_on(dev, lib.wf_paged_attn, desc, batch, q.data_ptr(), L.i64_array(_strides(q, 2)), out.data_ptr(),
+                L.i64_array(_strides(out, 2)), lse.data_ptr() if lse is not None else None, H, block, window, sink,
+                max_new, max_len, scale, ws.data_ptr() if ws is not None else None, need), "wf_paged_attn")
+    return (out, lse) if return_lse else out
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_lens: torch.Tensor | None = None,
+                    key_mask: torch.Tensor | None = None, kv_index: torch.Tensor | None = None,
+                    softmax_scale: float | None = None, out: torch.Tensor | None = None, return_lse: bool = False):
+    """Attention of q bf16 [B, Lq, H, 128] to an encoder's states k, v [N, Lk,
+    kv_heads, 128] of another length.  Entry b attends to states kv_index[b]
+    (int32 [B]; without it N is B, or 1 for states that all share), there to
+    the keys below kv_lens[n] (int32 [N]) that key_mask [N, Lk] (bool) keeps;
+    what the other keys hold does not matter.  Queries left without keys give
+    zeros.  With ``return_lse`` also the f32 log-sum-exp [B, Lq, H]."""
+    _check(q.dim() == 4 and k.dim() == 4 and v.shape == k.shape
+           and q.dtype == k.dtype == v.dtype == torch.bfloat16 and q.shape[3] == k.shape[3]
+           and q.stride(3) == k.stride(3) == v.stride(3) == 1,
+           "cross_attention: q [B, Lq, H, 128] and k, v [N, Lk, kv_heads, 128] must be bf16 with contiguous last dims")
+    B, Lq, H, D = q.shape
+    N, Lk, G, _ = k.shape
+    dev = q.device
+    _check(N >= 1 and Lk >= 1 and G >= 1 and H % G == 0,
+           "cross_attention: query heads must be a multiple of the K/V heads, states not empty")
+    _check(kv_index is not None or N in (1, B), "cross_attention: N states for B entries need kv_index")
+    for t, n in ((kv_index, B), (kv_lens, N)):
+        _check(t is None or (t.dtype == torch.int32 and t.shape == (n,) and t.is_contiguous() and t.device == dev),
+               "cross_attention: kv_index [B] and kv_lens [N] must be contiguous int32 on q's device")
+    _check(key_mask is None or (key_mask.dtype == torch.bool and key_mask.shape == (N, Lk) and key_mask.device == dev
+                                and (key_mask.stride(1) == 1 or Lk == 1)),
+           "cross_attention: key_mask must be bool [N, Lk] with contiguous rows on q's device")
+    _no_grad("cross_attention", q, k, v)
+    if out is None:
+        out = torch.empty((B, Lq, H, D), dtype=torch.bfloat16, device=dev)
+    _check(out.shape == q.shape and out.dtype == torch.bfloat16 and out.stride(3) == 1 and out.device == dev
+           and k.device == dev and v.device == dev, "cross_attention: out must match q, all tensors on one device")
+    _need_cuda(q)
+    lse = torch.empty((B, Lq, H), dtype=torch.float32, device=dev) if return_lse else None
+    lib = L.lib()
+    need = lib.wf_cross_attn_workspace(B, Lq, N, Lk, H, G)
+    ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need > 0 else None
+    scale = 1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale)
+    L.check(_on(dev, lib.wf_cross_attn, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                lse.data_ptr() if lse is not None else None, B, Lq, N, Lk, H, G, D, L.i64_array(_strides(q, 3)),
+                L.i64_array(_strides(k, 3)), L.i64_array(_strides(v, 3)), L.i64_array(_strides(out, 3)),
+                kv_index.data_ptr() if kv_index is not None else None,
+                kv_lens.data_ptr() if kv_lens is not None else None,
+                key_mask.data_ptr() if key_mask is not None else None,
+                key_mask.stride(0) if key_mask is not None else 0, scale,
+                ws.data_ptr() if ws is not None else None, need), "wf_cross_attn")
+    return (out, lse) if return_lse else out
