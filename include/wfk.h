@@ -254,8 +254,8 @@ int wf_paged_attn(const wf_kv_pages* pages, const wf_kv_batch* batch, const void
                   int64_t max_len, float softmax_scale, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Bytes of workspace the same call needs (host arithmetic only), or -1. */
-int64_t wf_paged_attn_workspace(const wf_kv_pages* pages, const wf_kv_batch* batch, int H, int64_t max_new,
-                                int64_t max_len);
+int64_t wf_paged_attn_workspace(const wf_kv_pages* pages, const wf_kv_batch* batch, int H, int window, int sink,
+                                int64_t max_new, int64_t max_len);
 
 /* Cross attention: O = softmax(Q K^T * softmax_scale) V of q, o [batch, Lq, H,
  * 128] bf16 against states k, v [states, Lk, kv_heads, 128] bf16 (strides

@@ -1,0 +1,249 @@
+"""Model check of the synchronisation of waveforcing_b200/csrc/paged_tile.cu (CPU).
+
+The kernel's roles (TMA producer, MMA issue, marks, two softmax warpgroups,
+code expansion) meet on mbarriers by parity.  The model transcribes every
+wait, arrival, load, MMA and commit with the kernel's phase formulas and runs
+the roles under random interleavings: copies land in any order, the tensor
+pipe runs in issue order.  Items have one or two sub-tiles and any number of
+key tiles, none included.  Every run must end, and every access must find the
+tile it expects: ring slots, Q, the marks, S, P (which overwrites S) and O.
+"""
+import random
+
+import pytest
+
+from tests.test_attn_protocol import Bar
+
+META = 4
+
+
+class Sim:
+    wrong = None
+
+    def __init__(self, items, kv8, seed):
+        self.items, self.kv8, self.rnd = items, kv8, random.Random(seed)  # items: (sub-tiles, key tiles)
+        self.NS = 4 if kv8 else 5
+        B = {}
+        for s in range(self.NS):
+            B[f"raw{s}"], B[f"full{s}"], B[f"empty{s}"] = Bar(1), Bar(2 if kv8 else 1), Bar(1)
+        for u in range(2):
+            for n in ("q_full", "q_empty", "s", "p", "o_full"):
+                B[f"{n}{u}"] = Bar(1)
+        self.b = B
+        self.slot = [None] * self.NS     # what a ring slot holds: (kind, item, tile, state)
+        self.users = [0] * self.NS       # MMAs issued that will read it
+        self.q = [None, None]
+        self.qusers = [0, 0]
+        self.marks = [None] * META
+        self.S, self.O = [None, None], [None, None]  # S: ("S", i, j) or ("P", i, j); O: (i, tiles summed)
+        self.tma, self.pipe = [], []
+
+    def wait(self, name, n):
+        while not self.b[name].done(n & 1):
+            yield
+
+    def producer(self):
+        n, qn = 0, [0, 0]
+        for i, (nsub, nt) in enumerate(self.items):
+            if nt == 0:
+                continue
+            for u in range(nsub):
+                if qn[u] > 0:
+                    yield from self.wait(f"q_empty{u}", qn[u] - 1)
+                assert self.qusers[u] == 0
+                self.b[f"q_full{u}"].arrive(1)
+                self.tma.append(("q", u, i, f"q_full{u}"))
+                qn[u] += 1
+            for j in range(nt):
+                for kind in "KV":
+                    s = n % self.NS
+                    if n >= self.NS:
+                        yield from self.wait(f"empty{s}", n // self.NS - 1)
+                    assert self.users[s] == 0, "slot overwritten before it was read"
+                    self.slot[s] = None
+                    self.b[f"raw{s}"].arrive(1)
+                    self.tma.append(("slot", s, (kind, i, j), f"raw{s}"))
+                    n += 1
+                    yield
+
+    def qk(self, u, n, i, j):
+        s = n % self.NS
+        assert self.slot[s] == ("K", i, j, "ready"), (self.slot[s], i, j)
+        assert self.q[u] == i
+        self.users[s] += 1
+        self.qusers[u] += 1
+        self.pipe.append(("qk", u, s, i, j))
+        self.pipe.append(("commit", f"s{u}"))
+
+    def mma(self):
+        n, items, pn = 0, [0, 0], [0, 0]
+        for i, (nsub, nt) in enumerate(self.items):
+            if nt == 0:
+                continue
+            yield from self.wait(f"full{n % self.NS}", n // self.NS)
+            for u in range(nsub):
+                yield from self.wait(f"q_full{u}", items[u])
+                self.qk(u, n, i, 0)
+                if nt == 1:
+                    self.pipe.append(("commit", f"q_empty{u}"))
+                yield
+            self.pipe.append(("commit", f"empty{n % self.NS}"))
+            n += 1
+            for j in range(nt):
+                sv, sk, more = n, n + 1, j + 1 < nt
+                yield from self.wait(f"full{sv % self.NS}", sv // self.NS)
+                for u in range(nsub):
+                    if self.wrong == "p":
+                        yield from self.wait(f"p{u}", pn[u] + 1)
+                    else:
+                        yield from self.wait(f"p{u}", pn[u])
+                    pn[u] += 1
+                    s = sv % self.NS
+                    assert self.slot[s] == ("V", i, j, "ready")
+                    self.users[s] += 1
+                    self.pipe.append(("pv", u, s, i, j))
+                    if u == nsub - 1:
+                        self.pipe.append(("commit", f"empty{s}"))
+                    if not more:
+                        self.pipe.append(("commit", f"o_full{u}"))
+                    yield
+                    if more:
+                        if u == 0:
+                            yield from self.wait(f"full{sk % self.NS}", sk // self.NS)
+                        self.qk(u, sk, i, j + 1)
+                        if j + 2 == nt:
+                            self.pipe.append(("commit", f"q_empty{u}"))
+                        if u == nsub - 1:
+                            self.pipe.append(("commit", f"empty{sk % self.NS}"))
+                        yield
+                n += 2 if more else 1
+            for u in range(nsub):
+                items[u] += 1
+
+    def ready(self, s, what):
+        """A stage before the tensor pipe is done with the slot; the last one makes it ready."""
+        kind, i, j, state = self.slot[s]
+        assert (kind, i, j) == what
+        self.slot[s] = (kind, i, j, "ready" if state == "half" or not self.kv8 else "half")
+        self.b[f"full{s}"].arrive()
+
+    def mark(self):
+        n = tiles = 0
+        for i, (_, nt) in enumerate(self.items):
+            for j in range(nt):
+                for kind in "KV":
+                    s = n % self.NS
+                    yield from self.wait(f"raw{s}", n // self.NS)
+                    if kind == "K":
+                        self.marks[tiles % (1 if self.wrong == "meta" else META)] = (i, j)
+                    self.ready(s, (kind, i, j))
+                    n += 1
+                    yield
+                tiles += 1
+
+    def expand(self):
+        n = 0
+        for i, (_, nt) in enumerate(self.items):
+            for j in range(nt):
+                for kind in "KV":
+                    s = n % self.NS
+                    yield from self.wait(f"raw{s}", n // self.NS)
+                    yield
+                    self.ready(s, (kind, i, j))
+                    n += 1
+                    yield
+
+    def softmax(self, u):
+        sn = items = tiles = 0
+        for i, (nsub, nt) in enumerate(self.items):
+            if u >= nsub:
+                tiles += nt
+                continue
+            for j in range(nt):
+                yield from self.wait(f"s{u}", sn)
+                assert self.S[u] == ("S", i, j), (self.S[u], i, j)
+                for _ in range(3):  # the marks are read until P is complete
+                    assert self.marks[tiles % (1 if self.wrong == "meta" else META)] == (i, j), "marks overwritten"
+                    yield
+                if j > 0:
+                    assert self.O[u] == (i, j), "O rescaled while a PV is pending"
+                yield
+                assert self.S[u] == ("S", i, j)
+                self.S[u] = ("P", i, j)
+                self.b[f"p{u}"].arrive()
+                sn, tiles = sn + 1, tiles + 1
+                yield
+            if nt:
+                yield from self.wait(f"o_full{u}", items)
+                items += 1
+                for _ in range(2):
+                    assert self.O[u] == (i, nt), (self.O[u], i, nt)
+                    yield
+
+    def step_tma(self):
+        kind, at, what, bar = self.tma.pop(self.rnd.randrange(len(self.tma)))
+        if kind == "q":
+            self.q[at] = what
+        else:
+            self.slot[at] = what + ("raw",)
+        self.b[bar].complete_tx(1)
+
+    def step_pipe(self):
+        op = self.pipe.pop(0)
+        if op[0] == "commit":
+            self.b[op[1]].arrive()
+            return
+        _, u, s, i, j = op
+        self.users[s] -= 1
+        if op[0] == "qk":
+            assert self.S[u] is None or self.S[u][0] == "done", ("S overwritten", self.S[u])
+            self.S[u] = ("S", i, j)
+            self.qusers[u] -= 1
+        else:
+            assert self.S[u] == ("P", i, j), (self.S[u], i, j)
+            self.S[u] = ("done", i, j)
+            if j > 0:
+                assert self.O[u] == (i, j)
+            self.O[u] = (i, j + 1)
+
+    def run(self):
+        roles = [self.producer(), self.mma(), self.mark(), self.softmax(0), self.softmax(1)]
+        if self.kv8:
+            roles.append(self.expand())
+        idle = 0
+        while roles or self.pipe or self.tma:
+            k = self.rnd.randrange(len(roles) + 2)
+            before = (len(self.tma), len(self.pipe), len(roles), tuple(b.phase * 1000 + b.pend for b in self.b.values()))
+            if k < len(roles):
+                try:
+                    next(roles[k])
+                except StopIteration:
+                    roles.pop(k)
+            elif k == len(roles) and self.tma:
+                self.step_tma()
+            elif k == len(roles) + 1 and self.pipe:
+                self.step_pipe()
+            after = (len(self.tma), len(self.pipe), len(roles), tuple(b.phase * 1000 + b.pend for b in self.b.values()))
+            idle = idle + 1 if before == after else 0
+            assert idle < 5000, "deadlock"
+
+
+def random_items(rnd):
+    return [(rnd.choice([1, 2, 2]), rnd.choice([0, 1, 1, 2, 3, 5])) for _ in range(rnd.randrange(1, 7))]
+
+
+@pytest.mark.parametrize("kv8", [False, True])
+def test_protocol(kv8):
+    for seed in range(150):
+        Sim(random_items(random.Random(seed)), kv8, seed).run()
+
+
+@pytest.mark.parametrize("wrong", ["p", "meta"])
+def test_protocol_errors_are_caught(wrong):
+    class Bad(Sim):
+        pass
+
+    Bad.wrong = wrong
+    with pytest.raises(AssertionError):
+        for seed in range(200):
+            Bad([(2, 4), (2, 3), (1, 2), (2, 1), (2, 3)], False, seed).run()

@@ -140,7 +140,7 @@ def calls(p, b):
 def test_abi_refuses_bad_pages(change, code):
     for call in calls(desc(**change), batch()):
         assert call() == code and L.last_error()
-    assert L.lib().wf_paged_attn_workspace(desc(**change), batch(), 4, 8, 64) == -1
+    assert L.lib().wf_paged_attn_workspace(desc(**change), batch(), 4, 0, 0, 8, 64) == -1
 
 
 @pytest.mark.parametrize("change,code", BAD_BATCH, ids=str)

@@ -105,7 +105,7 @@ _SIGS = {
     "wf_paged_kv_read": (_i32, [C.POINTER(KvPagesDesc), C.POINTER(KvBatchDesc), _vp, _vp, _pi64, _pi64, _vp]),
     "wf_paged_attn": (_i32, [C.POINTER(KvPagesDesc), C.POINTER(KvBatchDesc), _vp, _pi64, _vp, _pi64, _vp, _i32, _i32,
                              _i32, _i32, _i64, _i64, _f32, _vp, _i64, _vp]),
-    "wf_paged_attn_workspace": (_i64, [C.POINTER(KvPagesDesc), C.POINTER(KvBatchDesc), _i32, _i64, _i64]),
+    "wf_paged_attn_workspace": (_i64, [C.POINTER(KvPagesDesc), C.POINTER(KvBatchDesc), _i32, _i32, _i32, _i64, _i64]),
     "wf_cross_attn": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _pi64, _pi64, _pi64,
                              _pi64, _vp, _vp, _vp, _i64, _f32, _vp, _i64, _vp]),
     "wf_cross_attn_workspace": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32]),

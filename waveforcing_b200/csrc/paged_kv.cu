@@ -270,7 +270,7 @@ int check_pages(const char* who, const wf_kv_pages* p) {
 int check_batch(const char* who, const wf_kv_batch* b, int page_size) {
   if (!b || b->seqs < 0 || b->seqs > (1 << 24) || b->max_pages < 1 || b->rows < 0 || b->rows > INT_MAX - 1024)
     return fail(WF_ERR_INVALID_ARG, "%s: bad batch sizes", who);
-  if ((int64_t)b->max_pages * page_size > INT_MAX - 1024)
+  if ((int64_t)b->max_pages * page_size > INT_MAX - 4096)
     return fail(WF_ERR_INVALID_ARG, "%s: %d pages of %d rows pass 2^31 positions", who, b->max_pages, page_size);
   if (b->seqs > 0 && (!b->table || !b->cu || !b->lens || b->table_stride < 0))
     return fail(WF_ERR_INVALID_ARG, "%s: null page table, offsets or lengths", who);

@@ -17,6 +17,11 @@ enum StatusCode : uint32_t {
   ST_FLAG_TIMEOUT = 1u << 6,
   ST_DRAIN_TIMEOUT = 1u << 7,
   ST_ATTN_CONVERT = 1u << 8,
+  ST_PAGED_PRODUCER = 1u << 10,
+  ST_PAGED_MMA = 1u << 11,
+  ST_PAGED_MARK = 1u << 12,
+  ST_PAGED_SOFTMAX = 1u << 13,
+  ST_PAGED_EXPAND = 1u << 14,
   ST_PAGE_ID = 1u << 9,  // a page id outside the pool, or a length past the page table
 };
 

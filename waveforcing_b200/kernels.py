@@ -678,7 +678,7 @@ def paged_attention(q: torch.Tensor, pages: KVPages, page_table: torch.Tensor, c
     max_len = page_table.shape[1] * ps if max_len is None else int(max_len)
     desc = pages._desc()
     lib = L.lib()
-    need = lib.wf_paged_attn_workspace(desc, batch, H, max_new, max_len)
+    need = lib.wf_paged_attn_workspace(desc, batch, H, window, sink, max_new, max_len)
     ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need > 0 else None
     scale = 1.0 / math.sqrt(128) if softmax_scale is None else float(softmax_scale)
     L.check(_on(dev, lib.wf_paged_attn, desc, batch, q.data_ptr(), L.i64_array(_strides(q, 2)), out.data_ptr(),
