@@ -30,13 +30,14 @@ constexpr int SLOT = 2 * HALF;    // a K or V tile, or a Q sub-tile: [d 0-63][d 
 constexpr int META = 4;           // tiles whose marks (and scales) are kept
 constexpr uint32_t COL_S = 0, COL_O = 256;
 
+constexpr int WORK_BYTES = 80;
 template <bool KV8>
 struct Cfg {
   static constexpr int NS = KV8 ? 4 : 5;  // ring slots
   static constexpr int THREADS = KV8 ? 512 : 384;
   static constexpr int NBARS = (3 * NS + 10 + 1 + 1) & ~1;  // even: what follows is 16-byte aligned
   static constexpr int META_BYTES = META * (16 + (KV8 ? 2 * BN * 4 : 0) + 4);
-  static constexpr int SMEM = 1024 + 2 * SLOT + NS * SLOT + NBARS * 8 + META_BYTES + 16;
+  static constexpr int SMEM = 1024 + 2 * SLOT + NS * SLOT + NBARS * 8 + META_BYTES + 16 + 8 * WORK_BYTES;
   static_assert(SMEM <= 232448, "shared memory of one CTA");
 };
 
@@ -85,7 +86,9 @@ struct Work {
   int t0, t1;        // this item's share of the tile list
 };
 
-// Tile rows of the launch over all sequences (one warp).
+static_assert(sizeof(Work) <= WORK_BYTES, "a softmax warp's item");
+
+// Query tiles of the launch over all sequences (one warp).
 __device__ __forceinline__ int count_tiles(const Keys& ky, const Queries& qr, const Tiling& tl, int lane) {
   if (ky.cross) return qr.seqs * ((qr.Lq + 2 * tl.tq - 1) / (2 * tl.tq));
   int n = 0;
@@ -390,13 +393,13 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
         return ok;
       };
       auto qk = [&](int u, uint32_t slot) {
-        if (lane == 0) {
-          const uint32_t aQ = smem_u32(sQ + u * SLOT), aK = smem_u32(ring + (slot % NS) * SLOT);
+        const uint64_t dQ = desc_sw128(smem_u32(sQ + u * SLOT), 16, 1024);
+        const uint64_t dK = desc_sw128(smem_u32(ring + (slot % NS) * SLOT), 16, 1024);
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * HALF + (kk & 3) * 32;
-            umma_f16_ss(tbase + COL_S + u * BN, desc_sw128(aQ + off, 16, 1024), desc_sw128(aK + off, 16, 1024),
-                        idesc_qk, kk > 0);
+            const uint32_t off = ((kk >> 2) * HALF + (kk & 3) * 32) >> 4;
+            umma_f16_ss(tbase + COL_S + u * BN, dQ + off, dK + off, idesc_qk, kk > 0);
           }
           umma_commit(&bar_s[u]);
         }
@@ -411,10 +414,10 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
           if (!wait(&q_full[u], items[u])) break;
           tc_fence_after();
           qk(u, slot_n);
-          if (lane == 0 && nt == 1) umma_commit(&q_empty[u]);
+          if (nt == 1 && elect_one()) umma_commit(&q_empty[u]);
         }
         if (!ok) break;
-        if (lane == 0) umma_commit(&empty[slot_n % NS]);
+        if (elect_one()) umma_commit(&empty[slot_n % NS]);
         ++slot_n;
         for (int j = 0; ok && j < nt; ++j) {
           const uint32_t sv = slot_n, sk = slot_n + 1;
@@ -425,12 +428,12 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
             ++pn[u];
             // P_u of an item's first tile also says that the last item's O_u has been read
             tc_fence_after();
-            if (lane == 0) {
-              const uint32_t aV = smem_u32(ring + (sv % NS) * SLOT);
+            const uint64_t dV = desc_sw128(smem_u32(ring + (sv % NS) * SLOT), HALF, 1024);
+            if (elect_one()) {
 #pragma unroll
               for (int kk = 0; kk < BN / 16; ++kk)
-                umma_f16_ts(tbase + COL_O + u * HD, tbase + COL_S + u * BN + kk * 8,
-                            desc_sw128(aV + kk * 2048, HALF, 1024), idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
+                umma_f16_ts(tbase + COL_O + u * HD, tbase + COL_S + u * BN + kk * 8, dV + kk * 128, idesc_pv,
+                            (j > 0 || kk > 0) ? 1u : 0u);
               if (u == last_u) umma_commit(&empty[sv % NS]);
               if (!more) umma_commit(&o_full[u]);
             }
@@ -439,7 +442,7 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
               if (u == 0 && !wait(&full[sk % NS], sk / NS)) break;
               tc_fence_after();
               qk(u, sk);
-              if (lane == 0) {
+              if (elect_one()) {
                 if (j + 2 == nt) umma_commit(&q_empty[u]);
                 if (u == last_u) umma_commit(&empty[sk % NS]);
               }
@@ -450,7 +453,7 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
         for (int u = 0; u < w.nsub; ++u) ++items[u];
       }
       // nothing of ours may still be running when TMEM is released
-      if (lane == 0) {
+      if (elect_one()) {
         umma_commit(bar_fin);
         drain(bar_fin, 0, 200000000ull);
       }
@@ -540,8 +543,16 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
     const uint32_t tS = tbase + lane_off + COL_S + u * BN, tO = tbase + lane_off + COL_O + u * HD;
     uint32_t sn = 0, items = 0, tiles = 0;  // S_u consumed, items with keys, tiles of the CTA
     bool ok = true;
-    Work w;
-    for (long long it = blockIdx.x; ok && find_work(w, ky, qr, tl, n_tiles, G, it, lane); it += gridDim.x) {
+    // The item lies in shared memory: the loop over its tiles has no registers to spare.
+    Work& w = *reinterpret_cast<Work*>(reinterpret_cast<uint8_t*>(tmem_slot) + 16 + (warp - 4) * WORK_BYTES);
+    for (long long it = blockIdx.x; ok; it += gridDim.x) {
+      {
+        Work next;
+        if (!find_work(next, ky, qr, tl, n_tiles, G, it, lane)) break;
+        __syncwarp();
+        if (lane == 0) w = next;
+        __syncwarp();
+      }
       const int nt = w.t1 - w.t0;
       if (u >= w.nsub) {
         tiles += max(nt, 0);
@@ -555,6 +566,9 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
         ok = warp_wait(&bar_s[u], sn, abort_flag, ST_PAGED_SOFTMAX);
         if (!ok) break;
         tc_fence_after();
+        const uint32_t m = tiles % META;
+        const uint4 lv = *reinterpret_cast<const uint4*>(live + m * 4);
+        const int k0 = first_key[m];
         float s[BN];
         {
           uint32_t r[64];
@@ -565,7 +579,6 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
 #pragma unroll
           for (int k = 0; k < 64; ++k) s[64 + k] = __uint_as_float(r[k]);
         }
-        const uint32_t m = tiles % META;
         if constexpr (KV8) {
           const float4* ks = reinterpret_cast<const float4*>(scales + m * 2 * BN);
 #pragma unroll
@@ -578,8 +591,6 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
         }
         // Which of the tile's keys this row sees.  128 live keys lie at
         // consecutive positions, whatever the page size.
-        const uint4 lv = *reinterpret_cast<const uint4*>(live + m * 4);
-        const int k0 = first_key[m];
         const bool whole = (lv.x & lv.y & lv.z & lv.w) == 0xFFFFFFFFu && k0 + BN <= se.hi &&
                            (k0 >= se.lo || k0 + BN <= se.sink);
         const bool masked = !__all_sync(0xffffffffu, whole);
@@ -783,7 +794,8 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Keys 
 static int64_t tiles_bound(const Shape& sh) {
   const int step = 2 * (BM / sh.group);
   if (sh.cross) return (int64_t)sh.seqs * ((sh.Lq + step - 1) / step);
-  return sh.rows / step + (sh.rows < sh.seqs ? sh.rows : sh.seqs);
+  const int64_t seqs = sh.rows < sh.seqs ? sh.rows : sh.seqs;
+  return (sh.rows + seqs * (step - 1)) / step;
 }
 static int64_t key_tiles(const Shape& sh) {
   const int rows = (sh.page_size + 7) & ~7;
