@@ -10,8 +10,14 @@ Tolerances, from the arithmetic:
       2^-8 |o| the output is rounded to bf16,
       5e-4 A   both exponentials' polynomial (7.5e-5, in p and in the sum), f32
                scores of at most 128 products, f32 sums;
-  * lse: 2e-4 for the polynomial in the sum, and f32 rounding of the value.
+    over 8-bit pages p and code * scale are rounded to f16, half a step of which
+    is 2^-11: 2^-11 A more for v, and for k each score moves by at most
+    d = 2^-11 sum_i |q_i k_i| / sqrt(128), so each p, and each sum of p, by a
+    factor within exp(+-d): exp(2 d) - 1 of A more;
+  * lse: 2e-4 for the polynomial in the sum, f32 rounding of the value, and d.
 """
+
+import math
 
 import pytest
 import torch
@@ -37,6 +43,18 @@ def healthy():
     from waveforcing_b200 import _lib
 
     assert _lib.status_take() == 0
+
+
+def most_move(q, k):
+    """d of the header: q [.., n, 128] against k [.., L, 128] of the same heads."""
+    return 2 ** -11 * SCALE * float((q.double().abs() @ k.nan_to_num(0.0).double().abs().transpose(-1, -2)).max())
+
+
+def score_move(pool, q):
+    if pool.dtype == BF:
+        return 0.0
+    k = pool.val[0].transpose(0, 1).flatten(1, 2)  # [heads, keys, 128]
+    return most_move(q.transpose(0, 1), k.repeat_interleave(q.shape[1] // k.shape[0], 0))
 
 
 class Pool:
@@ -83,15 +101,21 @@ class Pool:
         return cu, (t(self.table), t(cu), t(self.lens))
 
 
-def close(out, lse, ref, ref_lse, mag, what=""):
+def tolerance(ref, mag, d=0.0):
+    extra = 2 ** -11 + math.expm1(2 * d) if d else 0.0
+    return (2 ** -8 + 5e-4 + extra) * mag + 2 ** -8 * ref.abs() + 1e-30
+
+
+def close(out, lse, ref, ref_lse, mag, d=0.0):
+    """``d``: the most that a score moves by its key's rounding to f16, 0 for bf16 keys."""
     o, l = out.double().cpu(), lse.double().cpu()
-    tol = (2 ** -8 + 5e-4) * mag + 2 ** -8 * ref.abs() + 1e-30
+    tol = tolerance(ref, mag, d)
     bad = ~((o - ref).abs() <= tol)
-    assert not bad.any(), (what, int(bad.sum()), float(((o - ref).abs() / tol).nan_to_num(9e9).max()))
+    assert not bad.any(), (int(bad.sum()), float(((o - ref).abs() / tol).nan_to_num(9e9).max()))
     none = torch.isinf(ref_lse)
-    assert torch.equal(torch.isinf(l), none), what
+    assert torch.equal(torch.isinf(l), none)
     err = (l - ref_lse)[~none].abs()
-    assert (err <= 2e-4 + 1e-6 * ref_lse[~none].abs()).all(), (what, float(err.max()))
+    assert (err <= 2e-4 + d + 1e-6 * ref_lse[~none].abs()).all(), float(err.max())
 
 
 def check_attention(pool, new, H, block=0, window=0, sink=0, q_scale=1.0, seed=0, hints=(None, None), tail=0, q=None):
@@ -106,7 +130,7 @@ def check_attention(pool, new, H, block=0, window=0, sink=0, q_scale=1.0, seed=0
     ref, ref_lse, written = O.paged_attention(q[:cu[-1]], *pool.val, pool.table, cu, pool.lens, block, window, sink, SCALE)
     mag, _, _ = O.paged_attention(q[:cu[-1]], pool.val[0], pool.val[1].abs(), pool.table, cu, pool.lens, block, window,
                                   sink, SCALE)
-    close(got[:cu[-1]], lse[:cu[-1]], ref, ref_lse, mag)
+    close(got[:cu[-1]], lse[:cu[-1]], ref, ref_lse, mag, score_move(pool, q))
     assert (got[cu[-1]:] == 7.0).all()  # rows behind the last sequence are left as they were
     return got
 
@@ -209,7 +233,7 @@ def test_attention_replays_with_new_lengths():
         torch.cuda.synchronize()
         ref, _, _ = O.paged_attention(q.cpu(), *pool.val, pool.table, cu, lens, 1, 0, 0, SCALE)
         mag, _, _ = O.paged_attention(q.cpu(), pool.val[0], pool.val[1].abs(), pool.table, cu, lens, 1, 0, 0, SCALE)
-        assert ((out.double().cpu() - ref).abs() <= (2 ** -8 + 5e-4) * mag + 2 ** -8 * ref.abs()).all()
+        assert ((out.double().cpu() - ref).abs() <= tolerance(ref, mag, score_move(pool, q.cpu()))).all()
     healthy()
 
 
@@ -388,13 +412,13 @@ def test_write_then_attend_then_cross_as_a_layer_does():
                 ref, _ = O.softmax_rows(*args, vv[:, h // 2], keep, SCALE)
                 mag, _ = O.softmax_rows(*args, vv[:, h // 2].abs(), keep, SCALE)
                 err = (o[cu[b]:cu[b + 1], h].double().cpu() - ref).abs()
-                assert (err <= (2 ** -8 + 5e-4) * mag + 2 ** -8 * ref.abs()).all()
+                assert (err <= tolerance(ref, mag, most_move(*args))).all()
         if new[0] == new[1]:
             x = o.view(2, 1, H, 128)
             c = K().cross_attention(x, text.to(DEV), text.to(DEV), kv_lens=t(tl))
             ref, _ = O.cross_attention(x.cpu(), text, text, tl, None, None, SCALE)
             mag, _ = O.cross_attention(x.cpu(), text, text.abs(), tl, None, None, SCALE)
-            assert ((c.double().cpu() - ref).abs() <= (2 ** -8 + 5e-4) * mag + 2 ** -8 * ref.abs()).all()
+            assert ((c.double().cpu() - ref).abs() <= tolerance(ref, mag)).all()
     healthy()
 
 

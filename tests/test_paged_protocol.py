@@ -14,7 +14,7 @@ import pytest
 
 from tests.test_attn_protocol import Bar
 
-META = 4
+META = 3
 
 
 class Sim:
@@ -25,9 +25,11 @@ class Sim:
         self.NS = 4 if kv8 else 5
         B = {}
         for s in range(self.NS):
-            B[f"raw{s}"], B[f"full{s}"], B[f"empty{s}"] = Bar(1), Bar(2 if kv8 else 1), Bar(1)
+            B[f"raw{s}"], B[f"full{s}"], B[f"empty{s}"] = Bar(1), Bar(1), Bar(1)
+        for m in range(META):
+            B[f"marked{m}"] = Bar(1)
         for u in range(2):
-            for n in ("q_full", "q_empty", "s", "p", "o_full"):
+            for n in ("q_raw", "q_full", "q_empty", "s", "p0", "p1", "o_full"):
                 B[f"{n}{u}"] = Bar(1)
         self.b = B
         self.slot = [None] * self.NS     # what a ring slot holds: (kind, item, tile, state)
@@ -35,6 +37,7 @@ class Sim:
         self.q = [None, None]
         self.qusers = [0, 0]
         self.marks = [None] * META
+        self.qpow = [[None, None], [None, None]]
         self.S, self.O = [None, None], [None, None]  # S: ("S", i, j) or ("P", i, j); O: (i, tiles summed)
         self.tma, self.pipe = [], []
 
@@ -51,8 +54,9 @@ class Sim:
                 if qn[u] > 0:
                     yield from self.wait(f"q_empty{u}", qn[u] - 1)
                 assert self.qusers[u] == 0
-                self.b[f"q_full{u}"].arrive(1)
-                self.tma.append(("q", u, i, f"q_full{u}"))
+                bar = f"q_raw{u}" if self.kv8 else f"q_full{u}"
+                self.b[bar].arrive(1)
+                self.tma.append(("q", u, i, bar))
                 qn[u] += 1
             for j in range(nt):
                 for kind in "KV":
@@ -93,15 +97,15 @@ class Sim:
                 sv, sk, more = n, n + 1, j + 1 < nt
                 yield from self.wait(f"full{sv % self.NS}", sv // self.NS)
                 for u in range(nsub):
-                    if self.wrong == "p":
-                        yield from self.wait(f"p{u}", pn[u] + 1)
-                    else:
-                        yield from self.wait(f"p{u}", pn[u])
-                    pn[u] += 1
                     s = sv % self.NS
-                    assert self.slot[s] == ("V", i, j, "ready")
-                    self.users[s] += 1
-                    self.pipe.append(("pv", u, s, i, j))
+                    for half in range(2):
+                        if not (self.wrong == "p" and half):
+                            yield from self.wait(f"p{half}{u}", pn[u])
+                        assert self.slot[s] == ("V", i, j, "ready")
+                        self.users[s] += 1
+                        self.pipe.append(("pv", u, s, i, j, half))
+                        yield
+                    pn[u] += 1
                     if u == nsub - 1:
                         self.pipe.append(("commit", f"empty{s}"))
                     if not more:
@@ -121,37 +125,53 @@ class Sim:
                 items[u] += 1
 
     def ready(self, s, what):
-        """A stage before the tensor pipe is done with the slot; the last one makes it ready."""
-        kind, i, j, state = self.slot[s]
-        assert (kind, i, j) == what
-        self.slot[s] = (kind, i, j, "ready" if state == "half" or not self.kv8 else "half")
+        assert self.slot[s] == what + ("raw",)
+        self.slot[s] = what + ("ready",)
         self.b[f"full{s}"].arrive()
 
     def mark(self):
         n = tiles = 0
         for i, (_, nt) in enumerate(self.items):
             for j in range(nt):
+                s = n % self.NS
+                yield from self.wait(f"raw{s}", n // self.NS)
+                self.marks[tiles % (1 if self.wrong == "meta" else META)] = (i, j)
+                if self.kv8:
+                    self.b[f"marked{tiles % META}"].arrive()
+                    n += 2
+                else:
+                    self.ready(s, ("K", i, j))
+                    s = (n + 1) % self.NS
+                    yield from self.wait(f"raw{s}", (n + 1) // self.NS)
+                    self.ready(s, ("V", i, j))
+                    n += 2
+                yield
+                tiles += 1
+
+    def expand(self):
+        n, tiles, qn = 0, 0, [0, 0]
+        for i, (nsub, nt) in enumerate(self.items):
+            if nt == 0:
+                continue
+            for u in range(nsub):
+                yield from self.wait(f"q_raw{u}", qn[u])
+                assert self.q[u] == i
+                self.qpow[u][qn[u] % (1 if self.wrong == "qpow" else 2)] = i
+                qn[u] += 1
+                self.b[f"q_full{u}"].arrive()
+                yield
+            for j in range(nt):
+                m = tiles % META
+                yield from self.wait(f"marked{m}", tiles // META)
                 for kind in "KV":
                     s = n % self.NS
                     yield from self.wait(f"raw{s}", n // self.NS)
-                    if kind == "K":
-                        self.marks[tiles % (1 if self.wrong == "meta" else META)] = (i, j)
+                    yield
+                    assert self.marks[m] == (i, j), "scales overwritten"
                     self.ready(s, (kind, i, j))
                     n += 1
                     yield
                 tiles += 1
-
-    def expand(self):
-        n = 0
-        for i, (_, nt) in enumerate(self.items):
-            for j in range(nt):
-                for kind in "KV":
-                    s = n % self.NS
-                    yield from self.wait(f"raw{s}", n // self.NS)
-                    yield
-                    self.ready(s, (kind, i, j))
-                    n += 1
-                    yield
 
     def softmax(self, u):
         sn = items = tiles = 0
@@ -165,12 +185,15 @@ class Sim:
                 for _ in range(3):  # the marks are read until P is complete
                     assert self.marks[tiles % (1 if self.wrong == "meta" else META)] == (i, j), "marks overwritten"
                     yield
+                if self.kv8 and j == 0:
+                    assert self.qpow[u][items % (1 if self.wrong == "qpow" else 2)] == i
                 if j > 0:
                     assert self.O[u] == (i, j), "O rescaled while a PV is pending"
-                yield
-                assert self.S[u] == ("S", i, j)
-                self.S[u] = ("P", i, j)
-                self.b[f"p{u}"].arrive()
+                for half in range(2):
+                    yield
+                    assert self.S[u] == (("P0", i, j) if half else ("S", i, j)) or half and self.S[u] == ("P0 read", i, j)
+                    self.S[u] = (f"P{half}" + (" after" if self.S[u][0] == "P0 read" else ""), i, j)
+                    self.b[f"p{half}{u}"].arrive()
                 sn, tiles = sn + 1, tiles + 1
                 yield
             if nt:
@@ -193,18 +216,24 @@ class Sim:
         if op[0] == "commit":
             self.b[op[1]].arrive()
             return
-        _, u, s, i, j = op
+        u, s, i, j = op[1:5]
         self.users[s] -= 1
         if op[0] == "qk":
             assert self.S[u] is None or self.S[u][0] == "done", ("S overwritten", self.S[u])
             self.S[u] = ("S", i, j)
             self.qusers[u] -= 1
         else:
-            assert self.S[u] == ("P", i, j), (self.S[u], i, j)
-            self.S[u] = ("done", i, j)
-            if j > 0:
-                assert self.O[u] == (i, j)
-            self.O[u] = (i, j + 1)
+            half = op[5]
+            assert self.S[u][1:] == (i, j) and self.S[u][0] in (("P1", "P1 after") if half else ("P0", "P1")), self.S[u]
+            if half:
+                assert self.O[u] == (i, j, "half")
+                self.S[u], self.O[u] = ("done", i, j), (i, j + 1)
+            else:
+                if j > 0:
+                    assert self.O[u] == (i, j)
+                self.O[u] = (i, j, "half")
+                if self.S[u][0] == "P0":
+                    self.S[u] = ("P0 read", i, j)
 
     def run(self):
         roles = [self.producer(), self.mma(), self.mark(), self.softmax(0), self.softmax(1)]
@@ -238,7 +267,7 @@ def test_protocol(kv8):
         Sim(random_items(random.Random(seed)), kv8, seed).run()
 
 
-@pytest.mark.parametrize("wrong", ["p", "meta"])
+@pytest.mark.parametrize("wrong", ["p", "meta", "qpow"])
 def test_protocol_errors_are_caught(wrong):
     class Bad(Sim):
         pass
@@ -246,4 +275,4 @@ def test_protocol_errors_are_caught(wrong):
     Bad.wrong = wrong
     with pytest.raises(AssertionError):
         for seed in range(200):
-            Bad([(2, 4), (2, 3), (1, 2), (2, 1), (2, 3)], False, seed).run()
+            Bad([(2, 4), (2, 1), (1, 1), (2, 1), (2, 3)], wrong == "qpow", seed).run()

@@ -93,13 +93,9 @@ __device__ __forceinline__ Sees sees(const Queries& qr, const Span& s, int i) {
   return v;
 }
 
-// Page of the keys [j * page_size, ...) of sequence b, -1 when its id is bad.
-__device__ __forceinline__ int page_of(const Keys& ky, const Span& s, int b, int j) {
-  if (ky.cross) return s.state;
-  const int id = __ldg(ky.table + b * ky.table_stride + j);
-  if (id >= 0 && id < ky.n_pages) return id;
-  status_raise(ST_PAGE_ID);
-  return -1;
+// Page of the keys [j * page_size, ...) of sequence b, unchecked.
+__device__ __forceinline__ int page_id(const Keys& ky, const Span& s, int b, int j) {
+  return ky.cross ? s.state : __ldg(ky.table + b * ky.table_stride + j);
 }
 
 // What the host knows of a call: the rows and lengths' upper bounds, from which

@@ -8,13 +8,24 @@
 //   warp 2       marks the live keys of each tile, zeroes the V rows of the
 //                others (their P is 0, but 0 * NaN is not), fetches scales
 //   warps 4-11   softmax; warpgroup u owns sub-tile u, a thread a row
-//   warps 12-15  (8-bit pages) expand codes to bf16
+//   warps 12-15  (8-bit pages) expand codes to f16
 // TMEM columns: S_0 [0,128) S_1 [128,256) O_0 [256,384) O_1 [384,512); P_u
-// (bf16) overwrites the first half of S_u, which its warpgroup holds in
+// (16 bits) overwrites the first half of S_u, which its warpgroup holds in
 // registers by then.  The tensor pipe runs in issue order, PV_0(j) QK_0(j+1)
 // PV_1(j) QK_1(j+1) ..., so QK_u(j+1) overwrites P_u(j) only after PV_u(j) has
 // read it, and S_u(j+1) complete means that PV_u(j) is: O_u may be rescaled.
 // While one sub-tile's products run, the other's exponentials do.
+//
+// 8-bit pages: both contractions run on f16 operands, whose 11 bits hold
+// code * scale to 2^-11 where bf16 would round to 2^-8, with the range taken
+// care of by powers of two: Q rows are scaled to at most 1, each K tile by its
+// largest row scale, V by the largest so far (O is rescaled when that grows);
+// the powers return in the softmax scale and in the last factor of O.  A
+// scale per key applied to S and P instead costs two shared-memory reads of
+// 512 bytes a row and tile: 525 against 398 us without at 9472 x 16384 x 4
+// heads, where the rows' reads and the operands' share shared memory.
+#include <cuda_fp16.h>
+
 #include <cmath>
 
 #include "paged_attn.cuh"
@@ -27,7 +38,7 @@ constexpr int BM = 128;  // rows of a sub-tile
 constexpr int BN = 128;  // keys of a tile
 constexpr int HALF = 16384;       // 128 rows x 64 bf16
 constexpr int SLOT = 2 * HALF;    // a K or V tile, or a Q sub-tile: [d 0-63][d 64-127]
-constexpr int META = 4;           // tiles whose marks (and scales) are kept
+constexpr int META = 3;           // tiles whose marks (and scales) are kept
 constexpr uint32_t COL_S = 0, COL_O = 256;
 
 constexpr int WORK_BYTES = 80;
@@ -35,8 +46,8 @@ template <bool KV8>
 struct Cfg {
   static constexpr int NS = KV8 ? 4 : 5;  // ring slots
   static constexpr int THREADS = KV8 ? 512 : 384;
-  static constexpr int NBARS = (3 * NS + 10 + 1 + 1) & ~1;  // even: what follows is 16-byte aligned
-  static constexpr int META_BYTES = META * (16 + (KV8 ? 2 * BN * 4 : 0) + 4);
+  static constexpr int NBARS = (3 * NS + 14 + META + 1 + 1) & ~1;  // even: what follows is 16-byte aligned
+  static constexpr int META_BYTES = META * (16 + (KV8 ? 2 * BN * 4 : 0) + 16) + (KV8 ? 4 * BM * 4 : 0);
   static constexpr int SMEM = 1024 + 2 * SLOT + NS * SLOT + NBARS * 8 + META_BYTES + 16 + 8 * WORK_BYTES;
   static_assert(SMEM <= 232448, "shared memory of one CTA");
 };
@@ -81,7 +92,8 @@ struct Work {
   int b, hk, split;
   int i0, nsub;  // first token, sub-tiles with rows
   Span sp;
-  int hi, lo, sink;  // keys the item's rows see: [0, sink) and [lo, hi)
+  int hi, lo, sink;  // keys the item's rows see together: [0, sink) and [lo, hi)
+  int hi_min, lo_max, sink_min;  // and those that each of them sees
   int n_sink, t_lo;  // tiles of the sink range; first tile of the other
   int t0, t1;        // this item's share of the tile list
 };
@@ -146,6 +158,9 @@ __device__ __forceinline__ bool find_work(Work& w, const Keys& ky, const Queries
   w.hi = last.hi;
   w.lo = first.lo;
   w.sink = min(last.sink, w.hi);
+  w.hi_min = w.i0 + w.sp.pos0 < 0 ? 0 : first.hi;
+  w.lo_max = last.lo;
+  w.sink_min = first.sink;
   int n = 0;
   w.n_sink = w.t_lo = 0;
   if (w.hi > 0) {
@@ -160,11 +175,10 @@ __device__ __forceinline__ bool find_work(Work& w, const Keys& ky, const Queries
 }
 __device__ __forceinline__ int nth_tile(const Work& w, int i) { return i < w.n_sink ? i : i - w.n_sink + w.t_lo; }
 
-// Page j of the item's sequence if some row of the item sees one of its keys: its id, or -1.
-__device__ __forceinline__ int needed_page(const Keys& ky, const Work& w, const Tiling& tl, int j) {
+// Whether some row of the item sees a key of its sequence's page j.
+__device__ __forceinline__ bool needed(const Work& w, const Tiling& tl, int j) {
   const long long p0 = (long long)j * tl.ps;
-  if (!((p0 < w.hi && p0 + tl.ps > w.lo) || p0 < w.sink)) return -1;
-  return page_of(ky, w.sp, w.b, j);
+  return (p0 < w.hi && p0 + tl.ps > w.lo) || p0 < w.sink;
 }
 
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, uint32_t code) {
@@ -187,42 +201,48 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   return r;
 }
 
-// Two e4m3 codes in the high bytes of t's halves -> bf16x2, exactly: the
-// code's exponent and mantissa moved into bf16's fields are the value times
-// 2^-120 (subnormal codes become subnormal bf16 and stay exact).  The NaN
-// codes come out as +-480; a row that holds NaN has a NaN scale instead.
-__device__ __forceinline__ uint32_t e4m3x2_bf16x2(uint32_t t) {
-  const uint32_t u = (t & 0x80008000u) | ((t >> 4) & 0x07F007F0u);
+__device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// c * (hi + lo) for a pair of codes: the row's scale in 22 bits, so that its
+// rounding does not shift all of a key's products the same way.
+__device__ __forceinline__ uint32_t scaled_f16x2(uint32_t c, uint32_t hi, uint32_t lo) {
   uint32_t r;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(u), "r"(0x7B807B80u));
+  asm("{\n\t.reg .b32 t;\n\t"
+      "mul.rn.f16x2 t, %1, %3;\n\t"
+      "fma.rn.f16x2 %0, %1, %2, t;\n\t}"
+      : "=r"(r)
+      : "r"(c), "r"(hi), "r"(lo));
   return r;
 }
-// Two signed bytes in the low bytes of t's halves -> bf16x2, exactly: (128 +
-// low 7 bits) - (128, or 256 for a negative byte).
-__device__ __forceinline__ uint32_t s8x2_bf16x2(uint32_t t) {
-  const uint32_t a = (t & 0x007F007Fu) | 0x43004300u, b = (t & 0x00800080u) | 0x43004300u;
-  uint32_t r;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
+__device__ __forceinline__ uint32_t hi_lo_f16(float x) {  // x as the sum of two f16, the larger in the low half
+  const float hi = __half2float(__float2half_rn(x));
+  return f16x2(hi, x - hi);
 }
+// Four codes -> four f16 products with the row's scale.
 template <int DT>
-__device__ __forceinline__ void expand4(uint32_t w, uint32_t& lo, uint32_t& hi) {  // 4 codes -> 4 bf16
+__device__ __forceinline__ void expand4(uint32_t w, uint32_t s_hi, uint32_t s_lo, uint32_t& lo, uint32_t& hi) {
   if constexpr (DT == WF_DTYPE_E4M3) {
-    lo = e4m3x2_bf16x2(__byte_perm(w, 0, 0x1404));
-    hi = e4m3x2_bf16x2(__byte_perm(w, 0, 0x3424));
-  } else {
-    lo = s8x2_bf16x2(__byte_perm(w, 0, 0x4140));
-    hi = s8x2_bf16x2(__byte_perm(w, 0, 0x4342));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(lo) : "h"(static_cast<uint16_t>(w)));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hi) : "h"(static_cast<uint16_t>(w >> 16)));
+  } else {  // 1024 + (c + 128) by its bits, minus 1152: exact
+    const uint32_t x = w ^ 0x80808080u;
+    const uint32_t a = __byte_perm(x, 0x64646464u, 0x4140), b = __byte_perm(x, 0x64646464u, 0x4342);
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(a), "r"(0x64806480u));
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(b), "r"(0x64806480u));
   }
+  lo = scaled_f16x2(lo, s_hi, s_lo);
+  hi = scaled_f16x2(hi, s_hi, s_lo);
 }
 
 // Expands the 32 rows of one converter warp of a code tile (128 bytes a row,
-// swizzled, in the slot's upper half) in place to two halves of bf16 rows.  A
-// code row shares its line with the upper bf16 row: the eight lanes of a row
+// swizzled, in the slot's upper half) in place to two halves of f16 rows.  A
+// code row shares its line with the upper f16 row: the eight lanes of a row
 // read all of it before any of them writes.  Lanes 4-7 of a row write their
 // odd chunk first, so that a row's eight stores meet eight bank groups.
 template <int DT>
-__device__ __forceinline__ void expand_rows(uint8_t* slot, int row0, int lane) {
+__device__ __forceinline__ void expand_rows(uint8_t* slot, int row0, int lane, const uint32_t* scale) {
   const int c = lane & 7, hi = c >> 2;
 #pragma unroll 1
   for (int i = 0; i < 32; i += 8) {
@@ -230,10 +250,12 @@ __device__ __forceinline__ void expand_rows(uint8_t* slot, int row0, int lane) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const int r = row0 + i + 4 * t + (lane >> 3);
-      const uint4 raw = *reinterpret_cast<const uint4*>(slot + HALF + r * 128 + ((c ^ (r & 7)) << 4));
+      const uint32_t sc = scale[r], s_hi = __byte_perm(sc, 0, 0x1010), s_lo = __byte_perm(sc, 0, 0x3232);
+      uint4 raw = *reinterpret_cast<const uint4*>(slot + HALF + r * 128 + ((c ^ (r & 7)) << 4));
+      if (sc == 0) raw = make_uint4(0, 0, 0, 0);  // a row that no query sees may hold NaN codes
       const uint32_t w[4] = {hi ? raw.z : raw.x, hi ? raw.w : raw.y, hi ? raw.x : raw.z, hi ? raw.y : raw.w};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) expand4<DT>(w[k], h[t][2 * k], h[t][2 * k + 1]);
+      for (int k = 0; k < 4; ++k) expand4<DT>(w[k], s_hi, s_lo, h[t][2 * k], h[t][2 * k + 1]);
     }
     __syncwarp();
 #pragma unroll
@@ -244,6 +266,37 @@ __device__ __forceinline__ void expand_rows(uint8_t* slot, int row0, int lane) {
       *reinterpret_cast<uint4*>(row + (first << 4)) = make_uint4(h[t][0], h[t][1], h[t][2], h[t][3]);
       *reinterpret_cast<uint4*>(row + ((first ^ 1) << 4)) = make_uint4(h[t][4], h[t][5], h[t][6], h[t][7]);
     }
+  }
+}
+
+// Power of two at or above x (> 0), between 2^-122 and 2^122 (a row scale is below 2^122).
+__device__ __forceinline__ float pow2_above(float x) {
+  const uint32_t e = ((__float_as_uint(x) + 0x7FFFFFu) >> 23) << 23;
+  return fminf(fmaxf(__uint_as_float(e), 0x1p-122f), 0x1p122f);
+}
+
+// Q rows of one converter warp (32 of a sub-tile, swizzled bf16) to f16 in
+// place, each divided by the power of two above its largest value; the powers
+// go to qpow.  Half a warp to a row, 16 bytes a lane.
+__device__ __forceinline__ void expand_q(uint8_t* sub, int row0, int lane, float* qpow) {
+#pragma unroll 1
+  for (int i = 0; i < 32; i += 2) {
+    const int r = row0 + i + (lane >> 4);
+    uint4* at = reinterpret_cast<uint4*>(sub + ((lane >> 3) & 1) * HALF + r * 128 + (lane & 7) * 16);
+    const uint4 v = *at;
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    float m = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      m = fmaxf(m, fmaxf(fabsf(__uint_as_float(w[k] << 16)), fabsf(__uint_as_float(w[k] & 0xFFFF0000u))));
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float p = pow2_above(fminf(m, 0x1p122f)), inv = 1.f / p;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      w[k] = f16x2(__uint_as_float(w[k] << 16) * inv, __uint_as_float(w[k] & 0xFFFF0000u) * inv);
+    *at = make_uint4(w[0], w[1], w[2], w[3]);
+    if ((lane & 15) == 0) qpow[r] = p;
   }
 }
 
@@ -271,31 +324,42 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
   uint64_t* q_full = empty + NS;     // [2]
   uint64_t* q_empty = q_full + 2;    // [2] the item's last QK_u has completed
   uint64_t* bar_s = q_empty + 2;     // [2] S_u complete
-  uint64_t* bar_p = bar_s + 2;       // [2] P_u written
-  uint64_t* o_full = bar_p + 2;      // [2] the item's last PV_u has completed
+  uint64_t* bar_p = bar_s + 2;       // [2][2] P_u written, by halves of the keys
+  uint64_t* o_full = bar_p + 4;      // [2] the item's last PV_u has completed
   uint64_t* bar_fin = o_full + 2;
+  uint64_t* q_raw = bar_fin + 1;     // [2] 8-bit pages: Q_u landed (q_full: as f16)
+  uint64_t* marked = q_raw + 2;      // [META] 8-bit pages: a tile's scales are there
   uint32_t* live = reinterpret_cast<uint32_t*>(raw + Cfg<KV8>::NBARS);  // [META][4] live keys of a tile
-  float* scales = reinterpret_cast<float*>(live + META * 4);            // [META][2][BN], 8-bit pages
-  int* first_key = reinterpret_cast<int*>(scales + (KV8 ? META * 2 * BN : 0));  // [META] position of its first key
+  int* whole = reinterpret_cast<int*>(live + META * 4);                 // [META] every row sees all of it
+  float* kpow = reinterpret_cast<float*>(whole + META);                 // [META] power of two of the K tile
+  float* vpow = kpow + META;                                            // [META] and of V up to this tile
+  uint32_t* scales = reinterpret_cast<uint32_t*>(vpow + 2 * META);      // [META][2][BN] hi_lo_f16
+  float* qpow = reinterpret_cast<float*>(scales + META * 2 * BN);       // [2][2][BM], by turns of the sub-tile's items
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(live) + Cfg<KV8>::META_BYTES);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // Values that steer the roles are broadcast from lane 0, by which the compiler
+  // knows them to be the same in a warp: the MMA warp's operands then stay in
+  // uniform registers (issue at 115 clocks an instruction otherwise).
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const int G = qr.H / qr.group;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < NS; ++s) {
       mbar_init(&raw[s], 1);
-      mbar_init(&full[s], KV8 ? 129 : 1);
+      mbar_init(&full[s], KV8 ? 128 : 1);
       mbar_init(&empty[s], 1);
     }
     for (int u = 0; u < 2; ++u) {
-      mbar_init(&q_full[u], 1);
+      mbar_init(&q_full[u], KV8 ? 128 : 1);
+      mbar_init(&q_raw[u], 1);
       mbar_init(&q_empty[u], 1);
       mbar_init(&bar_s[u], 1);
-      mbar_init(&bar_p[u], 128);
+      mbar_init(&bar_p[2 * u], 128);
+      mbar_init(&bar_p[2 * u + 1], 128);
       mbar_init(&o_full[u], 1);
     }
+    for (int m = 0; m < META; ++m) mbar_init(&marked[m], 1);
     mbar_init(bar_fin, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -307,7 +371,7 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tbase = *tmem_slot;
+  const uint32_t tbase = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   const int n_tiles = count_tiles(ky, qr, tl, lane);
 
   auto teardown = [&]() {
@@ -332,10 +396,11 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
       uint32_t qn[2] = {0, 0};    // Q sub-tiles loaded
       bool ok = true;
       const int sub = lane;       // a lane to a page of the tile
+      // A lane's page of tile t, as the table has it (-1: not needed); checked when it is used.
       auto page_for = [&](int t, int& row) -> int {
         const TileAt a = tile_at(tl, t);
         row = a.row;
-        return sub < tl.ppt ? needed_page(ky, w, tl, a.page + sub) : -1;
+        return sub < tl.ppt && needed(w, tl, a.page + sub) ? page_id(ky, w.sp, w.b, a.page + sub) : -1;
       };
       auto load = [&](const CUtensorMap* map, int id, int row) -> bool {
         const uint32_t s = slot_n % NS, n = slot_n / NS;
@@ -361,31 +426,33 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
         for (int u = 0; ok && u < w.nsub; ++u) {
           if (qn[u] > 0 && !(ok = warp_wait(&q_empty[u], qn[u] - 1, abort_flag, ST_PAGED_PRODUCER))) break;
           if (lane == 0) {
-            mbar_arrive_expect_tx(&q_full[u], 2 * tl.tq * qr.group * 128);
+            uint64_t* bar = KV8 ? &q_raw[u] : &q_full[u];
+            mbar_arrive_expect_tx(bar, 2 * tl.tq * qr.group * 128);
             const int i = w.i0 + u * tl.tq, row = ky.cross ? i : w.sp.first + i, entry = ky.cross ? w.b : 0;
-            tma_load_4d(sQ + u * SLOT, &tmQ, &q_full[u], 0, w.hk * qr.group, row, entry);
-            tma_load_4d(sQ + u * SLOT + HALF, &tmQ, &q_full[u], 64, w.hk * qr.group, row, entry);
+            tma_load_4d(sQ + u * SLOT, &tmQ, bar, 0, w.hk * qr.group, row, entry);
+            tma_load_4d(sQ + u * SLOT + HALF, &tmQ, bar, 64, w.hk * qr.group, row, entry);
           }
           ++qn[u];
         }
         int row, next_row = 0, id, next_id = page_for(nth_tile(w, w.t0), next_row);
         for (int i = w.t0; ok && i < w.t1; ++i) {
-          id = next_id;
+          id = next_id >= 0 && next_id < ky.n_pages ? next_id : -1;
           row = next_row;
-          if (i + 1 < w.t1) next_id = page_for(nth_tile(w, i + 1), next_row);
-          ok = load(&tmK, id, row) && load(&tmV, id, row);
+          if (!(ok = load(&tmK, id, row) && load(&tmV, id, row))) break;
+          if (i + 1 < w.t1) next_id = page_for(nth_tile(w, i + 1), next_row);  // looked up under these loads
         }
       }
       if (*abort_flag && lane == 0) {
         // let the copies in flight land before the CTA exits
         for (int u = 0; u < 2; ++u)
-          if (qn[u] > 0) drain(&q_full[u], qn[u] - 1, 200000000ull);
+          if (qn[u] > 0) drain(KV8 ? &q_raw[u] : &q_full[u], qn[u] - 1, 200000000ull);
         for (uint32_t n = slot_n > NS ? slot_n - NS : 0; n < slot_n; ++n) drain(&raw[n % NS], n / NS, 200000000ull);
       }
     } else if (warp == 1) {
       // ----------------------------------------------------------------- MMA
-      constexpr uint32_t idesc_qk = make_idesc(1, FMT_BF16, FMT_BF16, 0, BM, BN);
-      constexpr uint32_t idesc_pv = make_idesc(1, FMT_BF16, FMT_BF16, 1, BM, HD);
+      constexpr uint32_t FMT = KV8 ? FMT_F16 : FMT_BF16;
+      constexpr uint32_t idesc_qk = make_idesc(1, FMT, FMT, 0, BM, BN);
+      constexpr uint32_t idesc_pv = make_idesc(1, FMT, FMT, 1, BM, HD);
       uint32_t slot_n = 0, items[2] = {0, 0}, pn[2] = {0, 0};
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
@@ -405,12 +472,24 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
         }
         __syncwarp();
       };
+      auto pv = [&](int u, uint32_t slot, int half, bool add) {
+        const uint64_t dV = desc_sw128(smem_u32(ring + (slot % NS) * SLOT), HALF, 1024);
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < BN / 32; ++k) {
+            const int kk = half * (BN / 32) + k;
+            umma_f16_ts(tbase + COL_O + u * HD, tbase + COL_S + u * BN + kk * 8, dV + kk * 128, idesc_pv,
+                        (add || k > 0) ? 1u : 0u);
+          }
+        }
+        __syncwarp();
+      };
       for (long long it = blockIdx.x; ok && find_work(w, ky, qr, tl, n_tiles, G, it, lane); it += gridDim.x) {
-        const int nt = w.t1 - w.t0;
+        const int nt = __shfl_sync(0xffffffffu, w.t1 - w.t0, 0);
         if (nt <= 0) continue;
-        const int last_u = w.nsub - 1;
+        const int nsub = __shfl_sync(0xffffffffu, w.nsub, 0), last_u = nsub - 1;
         if (!wait(&full[slot_n % NS], slot_n / NS)) break;
-        for (int u = 0; u < w.nsub; ++u) {
+        for (int u = 0; u < nsub; ++u) {
           if (!wait(&q_full[u], items[u])) break;
           tc_fence_after();
           qk(u, slot_n);
@@ -423,17 +502,16 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
           const uint32_t sv = slot_n, sk = slot_n + 1;
           const bool more = j + 1 < nt;
           if (!wait(&full[sv % NS], sv / NS)) break;
-          for (int u = 0; u < w.nsub; ++u) {
-            if (!wait(&bar_p[u], pn[u])) break;
-            ++pn[u];
+          for (int u = 0; u < nsub; ++u) {
             // P_u of an item's first tile also says that the last item's O_u has been read
+            if (!wait(&bar_p[2 * u], pn[u])) break;
             tc_fence_after();
-            const uint64_t dV = desc_sw128(smem_u32(ring + (sv % NS) * SLOT), HALF, 1024);
+            pv(u, sv, 0, j > 0);
+            if (!wait(&bar_p[2 * u + 1], pn[u])) break;
+            tc_fence_after();
+            pv(u, sv, 1, true);
+            ++pn[u];
             if (elect_one()) {
-#pragma unroll
-              for (int kk = 0; kk < BN / 16; ++kk)
-                umma_f16_ts(tbase + COL_O + u * HD, tbase + COL_S + u * BN + kk * 8, dV + kk * 128, idesc_pv,
-                            (j > 0 || kk > 0) ? 1u : 0u);
               if (u == last_u) umma_commit(&empty[sv % NS]);
               if (!more) umma_commit(&o_full[u]);
             }
@@ -450,7 +528,7 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
           }
           slot_n += more ? 2 : 1;
         }
-        for (int u = 0; u < w.nsub; ++u) ++items[u];
+        for (int u = 0; u < nsub; ++u) ++items[u];
       }
       // nothing of ours may still be running when TMEM is released
       if (elect_one()) {
@@ -459,56 +537,99 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
       }
     } else if (warp == 2) {
       // --------------------------------------------------------------- marks
+      // Page ids are fetched a tile ahead, scales and mask bytes before the
+      // wait for the tile's K, so that their latency lies under it.
       uint32_t slot_n = 0, tiles = 0;
       bool ok = true;
+      int ids[4];
+      auto spot = [&](const TileAt& a, int c, int& j, int& off) -> bool {  // key c * 32 + lane of a tile; seen at all?
+        const int r = c * 32 + lane;
+        off = a.row + r;
+        j = a.page;
+        bool in = off < tl.ps;
+        if (tl.ps < BN) {
+          const int p = r / tl.rows;
+          off = r - p * tl.rows;
+          j += p;
+          in = off < tl.ps && p < tl.ppt;
+        }
+        const int pos = j * tl.ps + off;
+        return in && ((pos < w.hi && pos >= w.lo) || pos < w.sink);
+      };
+      auto fetch_ids = [&](int i) {
+        const TileAt a = tile_at(tl, nth_tile(w, i));
+        int j, off;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) ids[c] = spot(a, c, j, off) ? page_id(ky, w.sp, w.b, j) : INT_MIN;
+      };
       for (long long it = blockIdx.x; ok && find_work(w, ky, qr, tl, n_tiles, G, it, lane); it += gridDim.x) {
+        float v_top = 0.f;  // power of two of V so far
+        if (w.t0 < w.t1) fetch_ids(w.t0);
         for (int i = w.t0; ok && i < w.t1; ++i, ++tiles) {
           const TileAt a = tile_at(tl, nth_tile(w, i));
-          uint32_t words[4];
+          bool in[4];
           float sk[KV8 ? 4 : 1], sv[KV8 ? 4 : 1];
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            const int r = c * 32 + lane;
-            int off = a.row + r, j = a.page;
-            bool in = off < tl.ps;
-            if (tl.ps < BN) {
-              const int p = r / tl.rows;
-              off = r - p * tl.rows;
-              j += p;
-              in = off < tl.ps && p < tl.ppt;
-            }
-            const int pos = j * tl.ps + off;
-            in = in && ((pos < w.hi && pos >= w.lo) || pos < w.sink);
-            const int id = in ? page_of(ky, w.sp, w.b, j) : -1;
-            in = in && id >= 0;
-            if (in && ky.mask) in = __ldg(ky.mask + id * ky.mask_stride + pos) != 0;
+            int j, off;
+            spot(a, c, j, off);
+            in[c] = ids[c] >= 0 && ids[c] < ky.n_pages;
+            if (!in[c] && ids[c] != INT_MIN) status_raise(ST_PAGE_ID);
             if constexpr (KV8) {
-              sk[c] = in ? __ldg(ky.ks + id * ky.ks_str[0] + w.hk * ky.ks_str[1] + off) : 0.f;
-              sv[c] = in ? __ldg(ky.vs + id * ky.vs_str[0] + w.hk * ky.vs_str[1] + off) : 0.f;
+              sk[c] = sv[c] = 0.f;
+              if (in[c]) {
+                sk[c] = __ldg(ky.ks + ids[c] * ky.ks_str[0] + w.hk * ky.ks_str[1] + off);
+                sv[c] = __ldg(ky.vs + ids[c] * ky.vs_str[0] + w.hk * ky.vs_str[1] + off);
+              }
+            } else if (ky.mask && in[c]) {
+              in[c] = __ldg(ky.mask + ids[c] * ky.mask_stride + off) != 0;
             }
-            words[c] = __ballot_sync(0xffffffffu, in);
           }
+          if (i + 1 < w.t1) fetch_ids(i + 1);
           // The marks of tile n - META are dead: its V slot (and with it its
           // P, which was formed with them) has been released before this
           // tile's K could land.
           uint32_t s = slot_n % NS;
           if (!(ok = warp_wait(&raw[s], slot_n / NS, abort_flag, ST_PAGED_MARK))) break;
           const uint32_t m = tiles % META;
+          uint32_t words[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) words[c] = __ballot_sync(0xffffffffu, in[c]);
+          // 128 live keys lie at consecutive positions, whatever the page size.
+          const bool all = (words[0] & words[1] & words[2] & words[3]) == 0xFFFFFFFFu && a.base + BN <= w.hi_min &&
+                           (a.base >= w.lo_max || a.base + BN <= w.sink_min);
           if (lane < 4) live[m * 4 + lane] = lane < 2 ? (lane ? words[1] : words[0]) : (lane & 1 ? words[3] : words[2]);
-          if (lane == 4) first_key[m] = a.base;
+          if (lane == 4) whole[m] = all;
           if constexpr (KV8) {
+            // Largest finite scales (non-negative floats order as integers).
+            // A row whose V is not finite makes its key's score NaN instead:
+            // the queries that see it become NaN, the others never meet it.
+            float tk = 0.f, tv = 0.f;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-              scales[m * 2 * BN + c * 32 + lane] = sk[c];
-              scales[m * 2 * BN + BN + c * 32 + lane] = sv[c];
+              if (!(fabsf(sv[c]) < INFINITY)) sk[c] = __uint_as_float(0x7FC00000u), sv[c] = 0.f;
+              tv = fmaxf(tv, fabsf(sv[c]));
+              tk = fmaxf(tk, fabsf(sk[c]) < INFINITY ? fabsf(sk[c]) : 0.f);
             }
+            tk = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(tk)));
+            tv = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(tv)));
+            const float kp = pow2_above(tk);
+            if (v_top == 0.f || tv > v_top) v_top = pow2_above(tv) * 8.f;  // room: it should grow rarely
+            const float ik = 1.f / kp, iv = 1.f / v_top;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              scales[m * 2 * BN + c * 32 + lane] = hi_lo_f16(sk[c] * ik);
+              scales[m * 2 * BN + BN + c * 32 + lane] = hi_lo_f16(sv[c] * iv);
+            }
+            if (lane == 5) kpow[m] = kp;
+            if (lane == 6) vpow[m] = v_top;
           }
           __syncwarp();
-          if (lane == 0) mbar_arrive(&full[s]);
-          ++slot_n;
-          s = slot_n % NS;
-          if (!(ok = warp_wait(&raw[s], slot_n / NS, abort_flag, ST_PAGED_MARK))) break;
+          if (lane == 0) mbar_arrive(KV8 ? &marked[m] : &full[s]);
+          slot_n += 2;
           if constexpr (!KV8) {
+            s = (slot_n - 1) % NS;
+            if (!(ok = warp_wait(&raw[s], (slot_n - 1) / NS, abort_flag, ST_PAGED_MARK))) break;
             if ((words[0] & words[1] & words[2] & words[3]) != 0xFFFFFFFFu) {
               uint8_t* v = ring + s * SLOT + (lane >> 4) * 128 + ((lane >> 3) & 1) * HALF + (lane & 7) * 16;
 #pragma unroll 1
@@ -523,9 +644,8 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
               fence_proxy_async_smem();
               __syncwarp();
             }
+            if (lane == 0) mbar_arrive(&full[s]);
           }
-          if (lane == 0) mbar_arrive(&full[s]);
-          ++slot_n;
         }
       }
     }
@@ -561,14 +681,14 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
       const int i = w.i0 + u * tl.tq + row / qr.group, h = w.hk * qr.group + row % qr.group;
       const bool has_row = row < tl.tq * qr.group && i < w.sp.n;
       const Sees se = sees(qr, w.sp, min(i, w.sp.n - 1));
-      float m_run = -INFINITY, l_run = 0.f;
+      float m_run = -INFINITY, l_run = 0.f, v_run = 1.f, q_scale = 0.f;
       for (int j = 0; j < nt; ++j, ++sn, ++tiles) {
         ok = warp_wait(&bar_s[u], sn, abort_flag, ST_PAGED_SOFTMAX);
         if (!ok) break;
         tc_fence_after();
+        if (KV8 && j == 0) q_scale = qr.scale_log2 * qpow[((items & 1) * 2 + u) * BM + row];
         const uint32_t m = tiles % META;
-        const uint4 lv = *reinterpret_cast<const uint4*>(live + m * 4);
-        const int k0 = first_key[m];
+        const bool masked = whole[m] == 0;
         float s[BN];
         {
           uint32_t r[64];
@@ -579,29 +699,15 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
 #pragma unroll
           for (int k = 0; k < 64; ++k) s[64 + k] = __uint_as_float(r[k]);
         }
-        if constexpr (KV8) {
-          const float4* ks = reinterpret_cast<const float4*>(scales + m * 2 * BN);
-#pragma unroll
-          for (int k = 0; k < BN / 4; ++k) {
-            const float4 x = ks[k];
-            const float2 a = fmul2(make_float2(s[4 * k], s[4 * k + 1]), make_float2(x.x, x.y));
-            const float2 b = fmul2(make_float2(s[4 * k + 2], s[4 * k + 3]), make_float2(x.z, x.w));
-            s[4 * k] = a.x, s[4 * k + 1] = a.y, s[4 * k + 2] = b.x, s[4 * k + 3] = b.y;
-          }
-        }
-        // Which of the tile's keys this row sees.  128 live keys lie at
-        // consecutive positions, whatever the page size.
-        const bool whole = (lv.x & lv.y & lv.z & lv.w) == 0xFFFFFFFFu && k0 + BN <= se.hi &&
-                           (k0 >= se.lo || k0 + BN <= se.sink);
-        const bool masked = !__all_sync(0xffffffffu, whole);
-        uint32_t keep[4] = {lv.x, lv.y, lv.z, lv.w};
+        // Which of the tile's keys this row sees.
+        uint32_t keep[4];
         if (masked) {
           const TileAt at = tile_at(tl, nth_tile(w, w.t0 + j));
           const int b_hi = rows_below(tl, at, se.hi), b_lo = rows_below(tl, at, se.lo);
           const int b_sink = rows_below(tl, at, se.sink);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            keep[c] &= bit_range(b_lo, b_hi, c * 32) | bit_range(0, b_sink, c * 32);
+            keep[c] = live[m * 4 + c] & (bit_range(b_lo, b_hi, c * 32) | bit_range(0, b_sink, c * 32));
 #pragma unroll
             for (int k = 0; k < 32; ++k)
               if (!(keep[c] >> k & 1)) s[c * 32 + k] = -INFINITY;
@@ -619,7 +725,8 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
             for (int c = 0; c < 4; ++c) mc[c] = max3_nan(mc[c], s[k + c], s[k + 4 + c]);
           mx = max3_nan(max3_nan(mc[0], mc[1], mc[2]), mc[3], mc[3]);
         }
-        const float mx2 = mx * qr.scale_log2;
+        const float scale = KV8 ? q_scale * kpow[m] : qr.scale_log2;
+        const float mx2 = mx * scale;
         // O is rescaled only when the maximum grows by more than 2^8; l and O
         // use the same stale maximum, so the quotient does not change.
         float m_new = m_run;
@@ -630,55 +737,66 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
         }
         if (!(mx2 < INFINITY)) m_new = __uint_as_float(0x7FC00000u);  // NaN or +inf score: the row is NaN from here on
         const float m_use = m_new == -INFINITY ? 0.f : m_new;         // nothing seen yet
-        const float2 sc2 = make_float2(qr.scale_log2, qr.scale_log2);
-        const float2 nm2 = make_float2(-m_use, -m_use);
-        float2 sum[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        uint32_t pk[BN / 2];
-        float4 vs;
-        // P = 2^(s * scale - m), 3 of 8 pairs on the FMA pipe's polynomial, the
-        // rest on MUFU; l sums P before its rounding to bf16.
-#pragma unroll
-        for (int k = 0; k < BN / 2; ++k) {
-          const float2 x = ffma2(make_float2(s[2 * k], s[2 * k + 1]), sc2, nm2);
-          float2 p;
-          if ((k & 7) < 3) {
-            p = exp2_poly2(x);
-          } else {
-            p.x = ex2_approx(x.x);
-            p.y = ex2_approx(x.y);
-          }
-          sum[k & 3] = fadd2(sum[k & 3], p);
-          if constexpr (KV8) {
-            if ((k & 1) == 0) vs = *reinterpret_cast<const float4*>(scales + m * 2 * BN + BN + 2 * k);
-            p = fmul2(p, (k & 1) ? make_float2(vs.z, vs.w) : make_float2(vs.x, vs.y));
-          }
-          pk[k] = pack_bf16x2(p.x, p.y);
-        }
-        if (masked) {  // the polynomial's smallest value, and a NaN scale, must not count
-#pragma unroll
-          for (int k = 0; k < BN / 2; ++k) {
-            const uint32_t two = keep[k >> 4] >> ((2 * k) & 31) & 3;
-            pk[k] &= ((two & 1) ? 0xFFFFu : 0u) | ((two & 2) ? 0xFFFF0000u : 0u);
-          }
-        }
-        const float2 s2 = fadd2(fadd2(sum[0], sum[1]), fadd2(sum[2], sum[3]));
         const float alpha = grow ? ex2_approx(m_run - m_new) : 1.f;
-        if (j > 0 && __any_sync(0xffffffffu, grow)) {
+        float o_alpha = alpha;
+        bool rescale = __any_sync(0xffffffffu, grow);
+        if constexpr (KV8) {
+          const float v_new = vpow[m];
+          if (j > 0 && v_new != v_run) {
+            o_alpha *= v_run / v_new;
+            rescale = true;
+          }
+          v_run = v_new;
+        }
+        if (j > 0 && rescale) {
 #pragma unroll
           for (int c = 0; c < HD; c += 32) {
             uint32_t r[32];
             tmem_ld32x32b_x32(tO + c, r);
 #pragma unroll
-            for (int k = 0; k < 32; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * alpha);
+            for (int k = 0; k < 32; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * o_alpha);
             tmem_st32x32b_x32(tO + c, r);
           }
         }
-        l_run = l_run * alpha + (s2.x + s2.y);
         m_run = m_new;
-        tmem_st32x32b_x64(tS, pk);
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(&bar_p[u]);
+        const float2 sc2 = make_float2(scale, scale);
+        const float2 nm2 = make_float2(-m_use, -m_use);
+        float2 sum[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        // P = 2^(s * scale - m), 3 of 8 pairs on the FMA pipe's polynomial, the
+        // rest on MUFU; l sums P before its rounding to bf16.  PV starts on the
+        // first half of the keys while the second is formed.
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t pk[BN / 4];
+#pragma unroll
+          for (int kk = 0; kk < BN / 4; ++kk) {
+            const int k = half * (BN / 4) + kk;
+            const float2 x = ffma2(make_float2(s[2 * k], s[2 * k + 1]), sc2, nm2);
+            float2 p;
+            if ((k & 7) < 3) {
+              p = exp2_poly2(x);
+            } else {
+              p.x = ex2_approx(x.x);
+              p.y = ex2_approx(x.y);
+            }
+            sum[k & 3] = fadd2(sum[k & 3], p);
+            pk[kk] = KV8 ? f16x2(p.x, p.y) : pack_bf16x2(p.x, p.y);
+          }
+          if (masked) {  // the polynomial's smallest value must not count
+#pragma unroll
+            for (int kk = 0; kk < BN / 4; ++kk) {
+              const int k = half * (BN / 4) + kk;
+              const uint32_t two = keep[k >> 4] >> ((2 * k) & 31) & 3;
+              pk[kk] &= ((two & 1) ? 0xFFFFu : 0u) | ((two & 2) ? 0xFFFF0000u : 0u);
+            }
+          }
+          tmem_st32x32b_x32(tS + half * (BN / 4), pk);
+          tmem_st_wait();
+          tc_fence_before();
+          mbar_arrive(&bar_p[2 * u + half]);
+        }
+        const float2 s2 = fadd2(fadd2(sum[0], sum[1]), fadd2(sum[2], sum[3]));
+        l_run = l_run * alpha + (s2.x + s2.y);
       }
       if (!ok) break;
       if (nt > 0) {
@@ -688,7 +806,7 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
         tc_fence_after();
       }
       const bool none = m_run == -INFINITY;
-      const float inv = none ? 0.f : m_run != m_run ? m_run : 1.f / l_run;
+      const float inv = none ? 0.f : m_run != m_run ? m_run : v_run / l_run;
       const int64_t packed = (int64_t)(w.sp.first + i) * qr.H + h;
       const float lse2 = none ? -INFINITY : m_run + log2f(l_run);
       if (tl.splits > 1) {
@@ -737,14 +855,27 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
       uint32_t slot_n = 0;
       bool ok = true;
       Work w;
+      uint32_t qn[2] = {0, 0}, tiles = 0;
+      const int row0 = (warp - 12) * 32;
       for (long long it = blockIdx.x; ok && find_work(w, ky, qr, tl, n_tiles, G, it, lane); it += gridDim.x) {
-        for (int n = 2 * (w.t1 - w.t0); ok && n > 0; --n) {
-          const uint32_t s = slot_n % NS;
-          if (!(ok = warp_wait(&raw[s], slot_n / NS, abort_flag, ST_PAGED_EXPAND))) break;
-          expand_rows<DT>(ring + s * SLOT, (warp - 12) * 32, lane);
+        if (w.t1 <= w.t0) continue;
+        for (int u = 0; ok && u < w.nsub; ++u) {
+          if (!(ok = warp_wait(&q_raw[u], qn[u], abort_flag, ST_PAGED_EXPAND))) break;
+          expand_q(sQ + u * SLOT, row0, lane, qpow + ((qn[u]++ & 1) * 2 + u) * BM);
           fence_proxy_async_smem();
-          mbar_arrive(&full[s]);
-          ++slot_n;
+          mbar_arrive(&q_full[u]);
+        }
+        for (int i = w.t0; ok && i < w.t1; ++i, ++tiles) {
+          const uint32_t m = tiles % META;
+          if (!(ok = warp_wait(&marked[m], tiles / META, abort_flag, ST_PAGED_EXPAND))) break;
+#pragma unroll 1
+          for (int kv = 0; kv < 2; ++kv, ++slot_n) {
+            const uint32_t s = slot_n % NS;
+            if (!(ok = warp_wait(&raw[s], slot_n / NS, abort_flag, ST_PAGED_EXPAND))) break;
+            expand_rows<DT>(ring + s * SLOT, row0, lane, scales + m * 2 * BN + kv * BN);
+            fence_proxy_async_smem();
+            mbar_arrive(&full[s]);
+          }
         }
       }
     }
