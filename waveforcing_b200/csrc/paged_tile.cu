@@ -681,7 +681,8 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
       const int i = w.i0 + u * tl.tq + row / qr.group, h = w.hk * qr.group + row % qr.group;
       const bool has_row = row < tl.tq * qr.group && i < w.sp.n;
       const Sees se = sees(qr, w.sp, min(i, w.sp.n - 1));
-      float m_run = -INFINITY, l_run = 0.f, v_run = 1.f, q_scale = 0.f;
+      float m_run = -INFINITY, m_use = 0.f;  // the maximum in use; 0 while nothing has been seen
+      float l_run = 0.f, v_run = 1.f, q_scale = 0.f;
       for (int j = 0; j < nt; ++j, ++sn, ++tiles) {
         ok = warp_wait(&bar_s[u], sn, abort_flag, ST_PAGED_SOFTMAX);
         if (!ok) break;
@@ -728,42 +729,38 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
         const float scale = KV8 ? q_scale * kpow[m] : qr.scale_log2;
         const float mx2 = mx * scale;
         // O is rescaled only when the maximum grows by more than 2^8; l and O
-        // use the same stale maximum, so the quotient does not change.
-        float m_new = m_run;
-        bool grow = false;
-        if (mx2 > m_run + 8.f || (m_run == -INFINITY && mx2 > -INFINITY)) {
-          m_new = mx2;
-          grow = true;
-        }
-        if (!(mx2 < INFINITY)) m_new = __uint_as_float(0x7FC00000u);  // NaN or +inf score: the row is NaN from here on
-        const float m_use = m_new == -INFINITY ? 0.f : m_new;         // nothing seen yet
-        const float alpha = grow ? ex2_approx(m_run - m_new) : 1.f;
-        float o_alpha = alpha;
-        bool rescale = __any_sync(0xffffffffu, grow);
-        if constexpr (KV8) {
-          const float v_new = vpow[m];
-          if (j > 0 && v_new != v_run) {
-            o_alpha *= v_run / v_new;
-            rescale = true;
+        // use the same stale maximum, so the quotient does not change.  A NaN
+        // or +inf score makes the row NaN from here on.
+        const bool grow = !(mx2 <= m_run + 8.f);
+        const float v_new = KV8 ? vpow[m] : 1.f;
+        if (__any_sync(0xffffffffu, grow) || (KV8 && v_new != v_run)) {
+          float alpha = 1.f;
+          if (grow) {
+            const float m_new = mx2 < INFINITY ? mx2 : __uint_as_float(0x7FC00000u);
+            alpha = ex2_approx(m_run - m_new);
+            m_run = m_use = m_new;
+            l_run *= alpha;
           }
+          if (KV8) alpha *= v_run / v_new;
           v_run = v_new;
-        }
-        if (j > 0 && rescale) {
+          if (j > 0) {
 #pragma unroll
-          for (int c = 0; c < HD; c += 32) {
-            uint32_t r[32];
-            tmem_ld32x32b_x32(tO + c, r);
+            for (int c = 0; c < HD; c += 32) {
+              uint32_t r[32];
+              tmem_ld32x32b_x32(tO + c, r);
 #pragma unroll
-            for (int k = 0; k < 32; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * o_alpha);
-            tmem_st32x32b_x32(tO + c, r);
+              for (int k = 0; k < 32; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * alpha);
+              tmem_st32x32b_x32(tO + c, r);
+            }
           }
         }
-        m_run = m_new;
         const float2 sc2 = make_float2(scale, scale);
         const float2 nm2 = make_float2(-m_use, -m_use);
         float2 sum[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-        // P = 2^(s * scale - m), 3 of 8 pairs on the FMA pipe's polynomial, the
-        // rest on MUFU; l sums P before its rounding to bf16.  PV starts on the
+        // P = 2^(s * scale - m), 2 of 8 pairs on the FMA pipe's polynomial, the
+        // rest on MUFU (9472 x 16384 x 4 heads, bf16 / e4m3 pages, us: 1 of 8 255 /
+        // 371, 2 of 8 257 / 366, 3 of 8 286 / 387, 4 of 8 288 / 390); l sums P
+        // before its rounding to 16 bits.  PV starts on the
         // first half of the keys while the second is formed.
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -773,7 +770,7 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
             const int k = half * (BN / 4) + kk;
             const float2 x = ffma2(make_float2(s[2 * k], s[2 * k + 1]), sc2, nm2);
             float2 p;
-            if ((k & 7) < 3) {
+            if ((k & 7) < 2) {
               p = exp2_poly2(x);
             } else {
               p.x = ex2_approx(x.x);
@@ -796,7 +793,7 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
           mbar_arrive(&bar_p[2 * u + half]);
         }
         const float2 s2 = fadd2(fadd2(sum[0], sum[1]), fadd2(sum[2], sum[3]));
-        l_run = l_run * alpha + (s2.x + s2.y);
+        l_run += s2.x + s2.y;
       }
       if (!ok) break;
       if (nt > 0) {
