@@ -110,13 +110,13 @@ def desc(**kw):
              dtype=L.WF_DTYPE_E4M3, k_stride=(4096, 2048, 128), v_stride=(4096, 2048, 128), k_scale_stride=(32, 16),
              v_scale_stride=(32, 16))
     d.update(kw)
-    return L.KvPagesDesc(**d)
+    return C.byref(L.KvPagesDesc(**d))
 
 
 def batch(**kw):
     d = dict(table=256, table_stride=4, cu=256, lens=256, seqs=2, max_pages=4, rows=8)
     d.update(kw)
-    return L.KvBatchDesc(**d)
+    return C.byref(L.KvBatchDesc(**d))
 
 
 BAD_PAGES = [(dict(k=None), 1), (dict(v=264), 1), (dict(head_dim=64), 2), (dict(dtype=9), 2), (dict(n_pages=0), 1),
@@ -187,7 +187,7 @@ def test_abi_cross_attention_refusals(args, code):
 
 
 def test_descriptors_match_the_header():
-    """The ctypes structures have the layout a C compiler gives the header's."""
+    """The packed bytes and the ctypes structures have the layout a C compiler gives the header's."""
     import os
     import subprocess
     import tempfile
@@ -199,5 +199,13 @@ def test_descriptors_match_the_header():
         subprocess.run(["gcc", "-I" + os.path.dirname(L.HEADER_PATH), os.path.join(d, "a.c"), "-o",
                         os.path.join(d, "a")], check=True)
         got = subprocess.run([os.path.join(d, "a")], check=True, capture_output=True, text=True).stdout.split()
+    assert [int(x) for x in got[:2]] == [len(K._PACK_PAGES(*range(19))), len(K._PACK_BATCH(*range(7)))]
+    for pack, desc, n in ((K._PACK_PAGES, L.KvPagesDesc, 19), (K._PACK_BATCH, L.KvBatchDesc, 7)):
+        d = desc.from_buffer_copy(pack(*range(1, n + 1)))
+        flat = []
+        for name, _ in desc._fields_:
+            x = getattr(d, name)
+            flat += list(x) if hasattr(x, "__len__") else [x]
+        assert flat == list(range(1, n + 1))
     assert [int(x) for x in got] == [C.sizeof(L.KvPagesDesc), C.sizeof(L.KvBatchDesc), L.KvPagesDesc.k_stride.offset,
                                      L.KvBatchDesc.rows.offset]

@@ -101,13 +101,14 @@ _SIGS = {
     "wf_qk_norm_rope_publish": (_i32, [_vp, _i64, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _i64, _i64, _f32,
                                        C.POINTER(KvPublishDst), C.POINTER(C.c_int32), _i32, _vp]),
     "wf_rms_norm": (_i32, [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _f32, _vp]),
-    "wf_paged_kv_write": (_i32, [C.POINTER(KvPagesDesc), C.POINTER(KvBatchDesc), _vp, _vp, _pi64, _pi64, _vp]),
-    "wf_paged_kv_read": (_i32, [C.POINTER(KvPagesDesc), C.POINTER(KvBatchDesc), _vp, _vp, _pi64, _pi64, _vp]),
-    "wf_paged_attn": (_i32, [C.POINTER(KvPagesDesc), C.POINTER(KvBatchDesc), _vp, _pi64, _vp, _pi64, _vp, _i32, _i32,
-                             _i32, _i32, _i64, _i64, _f32, _vp, _i64, _vp]),
-    "wf_paged_attn_workspace": (_i64, [C.POINTER(KvPagesDesc), C.POINTER(KvBatchDesc), _i32, _i32, _i32, _i64, _i64]),
-    "wf_cross_attn": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _pi64, _pi64, _pi64,
-                             _pi64, _vp, _vp, _vp, _i64, _f32, _vp, _i64, _vp]),
+    # descriptors and strides by address: a ctypes array or byref(...), or packed bytes
+    "wf_paged_kv_write": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "wf_paged_kv_read": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "wf_paged_attn": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i64, _i64, _f32, _vp, _i64,
+                             _vp]),
+    "wf_paged_attn_workspace": (_i64, [_vp, _vp, _i32, _i32, _i32, _i64, _i64]),
+    "wf_cross_attn": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp,
+                             _vp, _vp, _vp, _i64, _f32, _vp, _i64, _vp]),
     "wf_cross_attn_workspace": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32]),
     "wf_ipc_export": (_i32, [_vp, C.POINTER(C.c_uint8), C.POINTER(_u64)]),
     "wf_ipc_open": (_i32, [C.POINTER(C.c_uint8), C.POINTER(_vp)]),

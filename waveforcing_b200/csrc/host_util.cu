@@ -74,6 +74,7 @@ extern "C" unsigned int wfk_status_take_exchange(void);
 extern "C" unsigned int wfk_status_take_paged_kv(void);
 extern "C" unsigned int wfk_status_take_paged_attn(void);
 extern "C" unsigned int wfk_status_take_paged_tile(void);
+extern "C" unsigned int wfk_status_take_paged_rows(void);
 
 extern "C" const char* wf_last_error(void) { return wfk::g_last_error.c_str(); }
 
@@ -83,5 +84,5 @@ extern "C" unsigned int wf_status_take(void) {
   cudaDeviceSynchronize();
   return wfk_status_take_attn() | wfk_status_take_codec() | wfk_status_take_gemm() | wfk_status_take_exchange() |
          wfk_status_take_paged_kv() | wfk_status_take_paged_attn() |
-         wfk_status_take_paged_tile();
+         wfk_status_take_paged_tile() | wfk_status_take_paged_rows();
 }

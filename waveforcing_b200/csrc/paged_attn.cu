@@ -10,9 +10,63 @@
 namespace wfk {
 namespace paged {
 
+// ------------------------------------------------------------------- joining
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// One warp to an output row: the splits' outputs weighted by their sums.
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Keys ky, const __grid_constant__ Queries qr,
+                                                   const float* __restrict__ part_o,
+                                                   const float* __restrict__ part_l, int splits) {
+  const int64_t n = (int64_t)qr.rows * qr.H;
+  const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31;
+  if (at >= n) return;
+  const int r = (int)(at / qr.H), h = (int)(at - (int64_t)r * qr.H);
+  int64_t orow;
+  if (ky.cross) {
+    const int b = r / qr.Lq;
+    orow = b * qr.o_str[0] + (r - b * qr.Lq) * qr.o_str[1];
+  } else {
+    if (r < __ldg(qr.cu) || r >= __ldg(qr.cu + qr.seqs)) return;  // behind the last sequence
+    orow = r * qr.o_str[1];
+  }
+  float m = -INFINITY;
+  for (int s = 0; s < splits; ++s) m = max_nan(m, part_l[s * n + at]);
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float l = 0.f;
+  if (m != -INFINITY)
+    for (int s = 0; s < splits; ++s) {
+      const float ls = part_l[s * n + at];
+      if (ls == -INFINITY) continue;  // its output was not written
+      const float w = exp2f(ls - m);
+      const float4 x = __ldcs(reinterpret_cast<const float4*>(part_o + (s * n + at) * HD) + lane);
+      o.x += w * x.x, o.y += w * x.y, o.z += w * x.z, o.w += w * x.w;
+      l += w;
+    }
+  const float inv = m == -INFINITY ? 0.f : 1.f / l;
+  *reinterpret_cast<uint2*>(qr.o + orow + h * qr.o_str[2] + lane * 4) =
+      make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+  if (qr.lse && lane == 0) qr.lse[at] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+
+int join(const Keys& ky, const Queries& qr, const float* part_o, const float* part_l, int splits, cudaStream_t st) {
+  join_kernel<<<(unsigned)(((int64_t)qr.rows * qr.H + 7) / 8), 256, 0, st>>>(ky, qr, part_o, part_l, splits);
+  WFK_CUDA_TRY(cudaGetLastError());
+  return WF_OK;
+}
+
+// ------------------------------------------------------------- entry points
+// Up to 16 rows to a K/V head read K and V once; more would read them again for
+// each 16, where the tile kernel takes 128 rows at a time.
+static bool few_rows(const Shape& sh) { return sh.max_new * sh.group <= 16; }
+
 // Partial rows of split keys: f32 [splits][rows][H][128 + 1].
 static int64_t workspace_need(const Shape& sh) {
-  const int splits = tile::tile_splits(sh);
+  const int splits = few_rows(sh) ? rows::splits(sh) : tile::splits(sh);
   return splits > 1 ? (int64_t)splits * sh.rows * sh.H * (HD + 1) * 4 : 0;
 }
 
@@ -26,7 +80,7 @@ static int launch(const char* who, const Keys& ky, const Queries& qr, const Shap
   if (need > 0 && (workspace_bytes < need || !workspace || !aligned16(workspace)))
     return fail(WF_ERR_INVALID_ARG, "%s: %lld bytes of 16-byte aligned workspace needed, %lld given", who,
                 (long long)need, (long long)workspace_bytes);
-  return tile::tile_launch(ky, qr, sh, workspace, static_cast<cudaStream_t>(stream));
+  return (few_rows(sh) ? rows::launch : tile::launch)(ky, qr, sh, workspace, static_cast<cudaStream_t>(stream));
 }
 
 static int check_rows(const char* who, const void* q, const void* o, const int64_t* qs, const int64_t* os, int n,
@@ -54,6 +108,7 @@ static Shape paged_shape(const wf_kv_pages* pages, const wf_kv_batch* batch, int
   sh.keys = max_len < cap ? max_len : cap;
   if (window > 0 && (int64_t)window + sink + 256 < sh.keys) sh.keys = (int64_t)window + sink + 256;
   if (sh.keys < 1) sh.keys = 1;
+  sh.kv8 = pages->dtype != WF_DTYPE_BF16;
   return sh;
 }
 

@@ -104,14 +104,21 @@ struct Shape {
   int64_t rows, keys;  // packed rows; keys an item of work may see
   int64_t max_new;
   int seqs, H, group, page_size, Lq;
-  bool cross;
+  bool cross, kv8;
 };
 constexpr int SMS = 148;  // B200
 
+// Many rows to a K/V head (paged_tile.cu); few (paged_rows.cu).  `splits`: runs
+// of keys whose partial rows the workspace holds for `join` (1: none).
 namespace tile {
-int tile_splits(const Shape& sh);
-int tile_launch(const Keys& ky, const Queries& qr, const Shape& sh, void* workspace, cudaStream_t st);
+int splits(const Shape& sh);
+int launch(const Keys& ky, const Queries& qr, const Shape& sh, void* workspace, cudaStream_t st);
 }  // namespace tile
+namespace rows {
+int splits(const Shape& sh);
+int launch(const Keys& ky, const Queries& qr, const Shape& sh, void* workspace, cudaStream_t st);
+}  // namespace rows
+int join(const Keys& ky, const Queries& qr, const float* part_o, const float* part_l, int splits, cudaStream_t st);
 
 }  // namespace paged
 }  // namespace wfk

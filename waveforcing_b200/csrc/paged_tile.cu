@@ -880,43 +880,6 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
   }
 }
 
-// ------------------------------------------------------------------- joining
-// One warp to an output row: the splits' outputs weighted by their sums.
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Keys ky, const __grid_constant__ Queries qr,
-                                                   const float* __restrict__ part_o,
-                                                   const float* __restrict__ part_l, int splits) {
-  const int64_t n = (int64_t)qr.rows * qr.H;
-  const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (at >= n) return;
-  const int r = (int)(at / qr.H), h = (int)(at - (int64_t)r * qr.H);
-  int64_t orow;
-  if (ky.cross) {
-    const int b = r / qr.Lq;
-    orow = b * qr.o_str[0] + (r - b * qr.Lq) * qr.o_str[1];
-  } else {
-    if (r < __ldg(qr.cu) || r >= __ldg(qr.cu + qr.seqs)) return;  // behind the last sequence
-    orow = r * qr.o_str[1];
-  }
-  float m = -INFINITY;
-  for (int s = 0; s < splits; ++s) m = max3_nan(m, part_l[s * n + at], -INFINITY);
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  float l = 0.f;
-  if (m != -INFINITY)
-    for (int s = 0; s < splits; ++s) {
-      const float ls = part_l[s * n + at];
-      if (ls == -INFINITY) continue;  // its output was not written
-      const float w = exp2f(ls - m);
-      const float4 x = __ldcs(reinterpret_cast<const float4*>(part_o + (s * n + at) * HD) + lane);
-      o.x += w * x.x, o.y += w * x.y, o.z += w * x.z, o.w += w * x.w;
-      l += w;
-    }
-  const float inv = m == -INFINITY ? 0.f : 1.f / l;
-  *reinterpret_cast<uint2*>(qr.o + orow + h * qr.o_str[2] + lane * 4) =
-      make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
-  if (qr.lse && lane == 0) qr.lse[at] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
-}
-
 // --------------------------------------------------------------------- host
 // What the host knows of a call's size.
 static int64_t tiles_bound(const Shape& sh) {
@@ -934,7 +897,7 @@ static int64_t key_tiles(const Shape& sh) {
 // Splits of the keys: the count that gives the least time for the slowest SM,
 // one key tile taking about 1.4 us, an item's start and end about two tiles,
 // and the join its launch and one f32 row written and read a split.
-int tile_splits(const Shape& sh) {
+int splits(const Shape& sh) {
   const int64_t items = tiles_bound(sh) * (sh.H / sh.group), nt = key_tiles(sh);
   int best = 1;
   double best_us = 1e30;
@@ -963,7 +926,7 @@ static int start(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap
   return WF_OK;
 }
 
-int tile_launch(const Keys& ky, const Queries& qr, const Shape& sh, void* workspace, cudaStream_t st) {
+int launch(const Keys& ky, const Queries& qr, const Shape& sh, void* workspace, cudaStream_t st) {
   const int G = qr.H / qr.group, ps = ky.page_size;
   Tiling tl;
   tl.ps = ps;
@@ -971,7 +934,7 @@ int tile_launch(const Keys& ky, const Queries& qr, const Shape& sh, void* worksp
   tl.rows = ps >= BN ? BN : (ps + 7) & ~7;
   tl.ppt = ps >= BN ? 1 : BN / tl.rows;
   tl.tq = BM / qr.group;
-  tl.splits = tile_splits(sh);
+  tl.splits = splits(sh);
   const bool kv8 = ky.dtype != WF_DTYPE_BF16;
   CUtensorMap tq, tk, tv;
   int rc;
@@ -1010,9 +973,7 @@ int tile_launch(const Keys& ky, const Queries& qr, const Shape& sh, void* worksp
        : ky.dtype == WF_DTYPE_E4M3 ? start<WF_DTYPE_E4M3>(tq, tk, tv, ky, qr, tl, grid, part_o, part_l, st)
                                    : start<WF_DTYPE_S8>(tq, tk, tv, ky, qr, tl, grid, part_o, part_l, st);
   if (rc != WF_OK || tl.splits == 1) return rc;
-  join_kernel<<<(unsigned)(((int64_t)qr.rows * qr.H + 7) / 8), 256, 0, st>>>(ky, qr, part_o, part_l, tl.splits);
-  WFK_CUDA_TRY(cudaGetLastError());
-  return WF_OK;
+  return join(ky, qr, part_o, part_l, tl.splits, st);
 }
 
 }  // namespace tile
