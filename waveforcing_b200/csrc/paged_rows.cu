@@ -33,7 +33,7 @@ constexpr int META_BYTES = 2 * 32 * 4 + 128;  // scales of K and V, the live key
 constexpr int STAGE = KV_BYTES + META_BYTES;
 constexpr int O_PITCH = 132;               // floats of a row of partial sums, off the banks of the next
 constexpr int SMEM = WARPS * ST * STAGE + 128;
-static_assert(16 * (O_PITCH + 2) * 4 <= ST * STAGE, "a warp's sums fit its ring");
+static_assert(16 * (O_PITCH + 3) * 4 <= ST * STAGE, "a warp's sums fit its ring");
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -162,6 +162,9 @@ __global__ void __launch_bounds__(THREADS, 2)
     const int i0 = rt * 16 / qr.group, i1 = min((rt * 16 + 15) / qr.group, sp.n - 1);
     const Sees first = sees(qr, sp, max(i0, min(-sp.pos0, i1))), last = sees(qr, sp, i1);
     const int hi = last.hi, lo = first.lo, sink = min(last.sink, hi);
+    const int hi_min = i0 + sp.pos0 < 0 ? 0 : first.hi, lo_max = last.lo, sink_min = first.sink;
+    const int n_rows = min(16, sp.n * qr.group - rt * 16);
+    const float q_scale[2] = {q_pow[0] * qr.scale_log2, q_pow[1] * qr.scale_log2};
     int n_sink = 0, c_lo = 0, n = 0;
     if (hi > 0) {
       c_lo = lo / KC;
@@ -204,19 +207,20 @@ __global__ void __launch_bounds__(THREADS, 2)
           cp4(at + KV_BYTES + 128 + lane * 4, ky.vs + (id >= 0 ? id * ky.vs_str[0] + hk * ky.vs_str[1] + off : 0),
               id >= 0);
         }
-        constexpr int CH = ROWB / 16, RPI = 32 / CH;  // 16-byte pieces of a row, rows an instruction covers
+        // Row offsets (bytes) of this lane's key, then each lane's share of 16-byte pieces.
+        constexpr int CH = ROWB / 16, RPI = 32 / CH;  // pieces of a row, rows that an instruction covers
         constexpr int ES = KV8 ? 1 : 2;
+        const int64_t kr = id >= 0 ? (id * ky.k_str[0] + hk * ky.k_str[1] + off * ky.k_str[2]) * ES : -1;
+        const int64_t vr = (id * ky.v_str[0] + hk * ky.v_str[1] + off * ky.v_str[2]) * ES;
         const int c = lane % CH;
+        const uint8_t *kb = static_cast<const uint8_t*>(ky.k) + c * 16, *vb = static_cast<const uint8_t*>(ky.v) + c * 16;
 #pragma unroll
         for (int k = 0; k < KC / RPI; ++k) {
           const int r = k * RPI + lane / CH;
-          const int rid = __shfl_sync(0xffffffffu, id, r), roff = __shfl_sync(0xffffffffu, off, r);
-          const int64_t kr = rid * ky.k_str[0] + hk * ky.k_str[1] + roff * ky.k_str[2];
-          const int64_t vr = rid * ky.v_str[0] + hk * ky.v_str[1] + roff * ky.v_str[2];
-          const uint8_t* kp = static_cast<const uint8_t*>(ky.k) + (rid >= 0 ? kr * ES + c * 16 : 0);
-          const uint8_t* vp = static_cast<const uint8_t*>(ky.v) + (rid >= 0 ? vr * ES + c * 16 : 0);
-          cp16(at + r * ROWB + ((c ^ ((r & 1) << 2)) << 4), kp, rid >= 0);
-          cp16(at + KC * ROWB + r * ROWB + ((c ^ (r & 7)) << 4), vp, rid >= 0);
+          const int64_t ko = __shfl_sync(0xffffffffu, kr, r), vo = __shfl_sync(0xffffffffu, vr, r);
+          const bool take = ko >= 0;
+          cp16(at + r * ROWB + ((c ^ ((r & 1) << 2)) << 4), kb + (take ? ko : 0), take);
+          cp16(at + KC * ROWB + r * ROWB + ((c ^ (r & 7)) << 4), vb + (take ? vo : 0), take);
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
@@ -269,18 +273,20 @@ __global__ void __launch_bounds__(THREADS, 2)
       }
       // Scores in log2 units, -inf where the row does not see the key.
       const int pos0 = (i < n_sink ? i : i - n_sink + c_lo) * KC;
+      const bool whole = live == (KC == 32 ? 0xFFFFFFFFu : (1u << (KC & 31)) - 1) && pos0 + KC <= hi_min &&
+                         (pos0 >= lo_max || pos0 + KC <= sink_min);
       float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const float2 ks = KV8 ? *reinterpret_cast<const float2*>(scale + nt * 8 + 2 * t) : make_float2(1.f, 1.f);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int k = nt * 8 + 2 * t + (e & 1), pos = pos0 + k;
-          const Sees& v = se[e >> 1];
-          const bool keep = (live >> k & 1) && pos < v.hi && (pos >= v.lo || pos < v.sink);
-          float x = s[nt][e] * qr.scale_log2;
-          if (KV8) x *= q_pow[e >> 1] * ((e & 1) ? ks.y : ks.x);
-          s[nt][e] = keep ? x : -INFINITY;
+          s[nt][e] *= KV8 ? q_scale[e >> 1] * ((e & 1) ? ks.y : ks.x) : qr.scale_log2;
+          if (!whole) {
+            const int k = nt * 8 + 2 * t + (e & 1), pos = pos0 + k;
+            const Sees& v = se[e >> 1];
+            if (!((live >> k & 1) && pos < v.hi && (pos >= v.lo || pos < v.sink))) s[nt][e] = -INFINITY;
+          }
           mx[e >> 1] = max_nan(mx[e >> 1], s[nt][e]);
         }
       }
@@ -383,6 +389,7 @@ __global__ void __launch_bounds__(THREADS, 2)
     for (int e = 0; e < 2; ++e) {
       l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 1);
       l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 2);
+      if (g + e * 8 >= n_rows) continue;
       if (t == 0) {
         mine[16 * O_PITCH + g + e * 8] = m_run[e];
         mine[16 * O_PITCH + 16 + g + e * 8] = l_run[e];
@@ -396,59 +403,55 @@ __global__ void __launch_bounds__(THREADS, 2)
         }
     }
     __syncthreads();
-    // Thread x sums dim x of every row over the warps (into warp 0's place:
-    // each element is read and written by one thread), with weights for all.
+    // The CTA's sums, into warp 0's place: first each row's maximum, l and the
+    // warps' weights (in place of their maxima), then thread x dim x of the rows.
     constexpr int PITCH_W = ST * STAGE / 4;
     float* base = reinterpret_cast<float*>(smem);
     const int dim = threadIdx.x;
-    float m_all[16], l_all[16];
+    if (dim < n_rows) {
+      float* at = base + 16 * O_PITCH + dim;
+      float m = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      float m = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) m = max_nan(m, base[w * PITCH_W + 16 * O_PITCH + r]);
+      for (int w = 0; w < WARPS; ++w) m = max_nan(m, at[w * PITCH_W]);
       const float mu = m == -INFINITY ? 0.f : m;
-      float l = 0.f, x = 0.f;
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) {
-        const float wt = exp2f(base[w * PITCH_W + 16 * O_PITCH + r] - mu);
-        l += wt * base[w * PITCH_W + 16 * O_PITCH + 16 + r];
-        x += wt * base[w * PITCH_W + r * O_PITCH + dim];
+        const float wt = exp2f(at[w * PITCH_W] - mu);
+        l += wt * at[w * PITCH_W + 16];
+        at[w * PITCH_W] = wt;
       }
-      base[r * O_PITCH + dim] = x;
-      m_all[r] = m;
-      l_all[r] = l;
+      at[16] = l;
+      at[32] = m;
     }
     __syncthreads();
-    if (dim < 16) {
+#pragma unroll 2
+    for (int r = 0; r < n_rows; ++r) {
+      float x = 0.f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (r == dim) {
-          base[16 * O_PITCH + r] = m_all[r];
-          base[16 * O_PITCH + 16 + r] = l_all[r];
-        }
+      for (int w = 0; w < WARPS; ++w)
+        x += base[w * PITCH_W + 16 * O_PITCH + r] * base[w * PITCH_W + r * O_PITCH + dim];
+      base[r * O_PITCH + dim] = x;
     }
     if (cut.cluster > 1)
       cluster_sync();
     else
       __syncthreads();
     // CTA `rank` finishes rows rank, rank + cluster, ...: the CTAs' sums joined.
-    for (int r = rank; r < 16; r += cut.cluster) {
+    for (int r = rank; r < n_rows; r += cut.cluster) {
       const int rg = rt * 16 + r, i = rg / qr.group;
-      if (i >= sp.n) break;
       const int h = hk * qr.group + rg - i * qr.group;
-      const uint32_t am = smem_u32(base + 16 * O_PITCH + r), ao = smem_u32(base + r * O_PITCH + dim);
+      const uint32_t am = smem_u32(base + 16 * O_PITCH + 32 + r), ao = smem_u32(base + r * O_PITCH + dim);
       float m = -INFINITY, l = 0.f, x = 0.f;
       if (cut.cluster > 1) {
         for (int c = 0; c < cut.cluster; ++c) m = max_nan(m, cluster_load(am, c));
         const float mu = m == -INFINITY ? 0.f : m;
         for (int c = 0; c < cut.cluster; ++c) {
           const float wt = exp2f(cluster_load(am, c) - mu);
-          l += wt * cluster_load(am + 64, c);
+          l += wt * cluster_load(am - 64, c);
           x += wt * cluster_load(ao, c);
         }
       } else {
-        m = base[16 * O_PITCH + r];
+        m = base[16 * O_PITCH + 32 + r];
         l = base[16 * O_PITCH + 16 + r];
         x = base[r * O_PITCH + dim];
       }
@@ -475,16 +478,16 @@ __global__ void __launch_bounds__(THREADS, 2)
 }
 
 // --------------------------------------------------------------------- host
-// Enough CTAs for four on every SM's two places, as long as each keeps two
-// chunks to a warp; what a cluster cannot give, clusters joined afterwards do
-// as far as one CTA to each place.
+// Enough CTAs for every SM's two places, as long as each keeps two chunks to a
+// warp; what a cluster cannot give, clusters joined afterwards do as far as one
+// CTA to each SM.
 static Cut cut_of(const Shape& sh, bool kv8) {
   const int64_t chunk = kv8 ? 32 : 16;
   Cut c{1, 1, (int)((sh.max_new * sh.group + 15) / 16)};
   if (c.row_tiles < 1) c.row_tiles = 1;
   const int64_t seqs = sh.seqs < sh.rows ? sh.seqs : sh.rows;
   const int64_t items = seqs * (sh.H / sh.group) * c.row_tiles, most = sh.keys / (chunk * WARPS * 2);
-  while (c.cluster < MAX_CLUSTER && items * c.cluster < 4 * SMS && 2 * c.cluster <= most) c.cluster *= 2;
+  while (c.cluster < MAX_CLUSTER && items * c.cluster < 2 * SMS && 2 * c.cluster <= most) c.cluster *= 2;
   if (c.cluster == MAX_CLUSTER)
     while (c.outer < 16 && items * c.cluster * c.outer < SMS && 2 * c.outer * c.cluster <= most) c.outer *= 2;
   return c;
