@@ -11,12 +11,6 @@ namespace wfk {
 namespace paged {
 
 // ------------------------------------------------------------------- joining
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 // One warp to an output row: the splits' outputs weighted by their sums.
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Keys ky, const __grid_constant__ Queries qr,
                                                    const float* __restrict__ part_o,
@@ -56,6 +50,21 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Keys 
 int join(const Keys& ky, const Queries& qr, const float* part_o, const float* part_l, int splits, cudaStream_t st) {
   join_kernel<<<(unsigned)(((int64_t)qr.rows * qr.H + 7) / 8), 256, 0, st>>>(ky, qr, part_o, part_l, splits);
   WFK_CUDA_TRY(cudaGetLastError());
+  return WF_OK;
+}
+
+int page_maps(CUtensorMap* k, CUtensorMap* v, const Keys& ky, int kv_heads, int rows) {
+  const bool kv8 = ky.dtype != WF_DTYPE_BF16;
+  const uint64_t dim[4] = {HD, (uint64_t)ky.page_size, (uint64_t)kv_heads, (uint64_t)ky.n_pages};
+  const uint32_t box[4] = {kv8 ? 128u : 64u, (uint32_t)rows, 1, 1};
+  const uint64_t elem = kv8 ? 1 : 2;
+  for (int i = 0; i < 2; ++i) {
+    const int64_t* s = i ? ky.v_str : ky.k_str;
+    const uint64_t str[3] = {(uint64_t)s[2] * elem, (uint64_t)s[1] * elem, (uint64_t)s[0] * elem};
+    const int rc = encode_tiled(i ? v : k, kv8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                                i ? ky.v : ky.k, dim, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc != WF_OK) return rc;
+  }
   return WF_OK;
 }
 

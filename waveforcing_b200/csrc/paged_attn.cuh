@@ -9,6 +9,7 @@
 #pragma once
 
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <climits>
@@ -98,6 +99,111 @@ __device__ __forceinline__ int page_id(const Keys& ky, const Span& s, int b, int
   return ky.cross ? s.state : __ldg(ky.table + b * ky.table_stride + j);
 }
 
+// How the keys of a sequence fall into tiles of BN: pages of at least BN rows
+// give ceil(page_size / BN) tiles each, smaller ones share a tile, a page on
+// every `rows` tile rows (page_size rounded up to the swizzle's 8).
+struct Tiling {
+  int ps, tpp, ppt, rows;  // page size; tiles per page (large pages); pages per tile (small); tile rows of a page
+  int tq, splits;          // tokens of a sub-tile and runs of keys (paged_tile.cu)
+};
+inline Tiling tiling_of(int ps, int bn) {
+  const int rows = ps >= bn ? bn : (ps + 7) & ~7;
+  return Tiling{ps, (ps + bn - 1) / bn, ps >= bn ? 1 : bn / rows, rows, 0, 1};
+}
+template <int BN>
+__device__ __forceinline__ int tile_of(const Tiling& tl, int pos) {
+  const int j = pos / tl.ps;
+  return tl.ps < BN ? j / tl.ppt : j * tl.tpp + (pos - j * tl.ps) / BN;
+}
+struct TileAt {
+  int page, row, base;  // first page, row in it, position of the tile's first key
+};
+template <int BN>
+__device__ __forceinline__ TileAt tile_at(const Tiling& tl, int t) {
+  TileAt a;
+  if (tl.ps < BN) {
+    a.page = t * tl.ppt;
+    a.row = 0;
+  } else {
+    a.page = t / tl.tpp;
+    a.row = (t - a.page * tl.tpp) * BN;
+  }
+  a.base = a.page * tl.ps + a.row;
+  return a;
+}
+// Tile rows whose position is below x.
+template <int BN>
+__device__ __forceinline__ int rows_below(const Tiling& tl, const TileAt& a, int x) {
+  const int d = x - a.base;
+  if (d <= 0) return 0;
+  if (tl.ps >= BN) return min(d, min(BN, tl.ps - a.row));
+  const int j = d / tl.ps;
+  return min(j, tl.ppt) * tl.rows + (j < tl.ppt ? d - j * tl.ps : 0);
+}
+// Bits [a, b) of a 32-bit word that starts at bit `at`.
+__device__ __forceinline__ uint32_t bit_range(int a, int b, int at) {
+  const int lo = min(max(a - at, 0), 32), hi = min(max(b - at, 0), 32);
+  if (hi <= lo) return 0;
+  return (0xFFFFFFFFu >> (32 - (hi - lo))) << lo;
+}
+
+// The keys that tokens [i0, i1] of a sequence see, and the list of their tiles:
+// n_sink tiles from the first, then those from t_lo on.
+struct Range {
+  int hi, lo, sink;              // seen by some token: [0, sink) and [lo, hi)
+  int hi_min, lo_max, sink_min;  // and by every one
+  int n_sink, t_lo, n;
+};
+template <int BN>
+__device__ __forceinline__ Range range_of(const Queries& qr, const Span& sp, const Tiling& tl, int i0, int i1) {
+  const Sees last = sees(qr, sp, i1);
+  const Sees first = sees(qr, sp, max(i0, min(-sp.pos0, i1)));  // earlier rows have no position
+  Range r;
+  r.hi = last.hi;
+  r.lo = first.lo;
+  r.sink = min(last.sink, r.hi);
+  r.hi_min = i0 + sp.pos0 < 0 ? 0 : first.hi;
+  r.lo_max = last.lo;
+  r.sink_min = first.sink;
+  r.n_sink = r.t_lo = r.n = 0;
+  if (r.hi > 0) {
+    r.t_lo = tile_of<BN>(tl, r.lo);
+    r.n_sink = r.sink > 0 ? min(tile_of<BN>(tl, r.sink - 1) + 1, r.t_lo) : 0;
+    r.n = r.n_sink + tile_of<BN>(tl, r.hi - 1) + 1 - r.t_lo;
+  }
+  return r;
+}
+__device__ __forceinline__ int nth_tile(const Range& r, int i) { return i < r.n_sink ? i : i - r.n_sink + r.t_lo; }
+// Whether some token sees a key of its sequence's page j.
+__device__ __forceinline__ bool needed(const Range& r, const Tiling& tl, int j) {
+  const long long p0 = (long long)j * tl.ps;
+  return (p0 < r.hi && p0 + tl.ps > r.lo) || p0 < r.sink;
+}
+
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, uint32_t code) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity & 1, abort, code));
+}
+// Maximum of two or three, NaN if one is NaN (a NaN score must reach the row's result).
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// Power of two at or above x (> 0), between 2^-122 and 2^122 (a row scale is below 2^122).
+__device__ __forceinline__ float pow2_above(float x) {
+  const uint32_t e = ((__float_as_uint(x) + 0x7FFFFFu) >> 23) << 23;
+  return fminf(fmaxf(__uint_as_float(e), 0x1p-122f), 0x1p122f);
+}
+
 // What the host knows of a call: the rows and lengths' upper bounds, from which
 // it cuts the work (and sizes the workspace of the cut).
 struct Shape {
@@ -107,6 +213,11 @@ struct Shape {
   bool cross, kv8;
 };
 constexpr int SMS = 148;  // B200
+inline int64_t tiles_of_keys(const Shape& sh, int bn) {
+  const Tiling tl = tiling_of(sh.page_size, bn);
+  const int64_t pages = (sh.keys + sh.page_size - 1) / sh.page_size;
+  return sh.page_size >= bn ? pages * tl.tpp : (pages + tl.ppt - 1) / tl.ppt;
+}
 
 // Many rows to a K/V head (paged_tile.cu); few (paged_rows.cu).  `splits`: runs
 // of keys whose partial rows the workspace holds for `join` (1: none).
@@ -118,6 +229,9 @@ namespace rows {
 int splits(const Shape& sh);
 int launch(const Keys& ky, const Queries& qr, const Shape& sh, void* workspace, cudaStream_t st);
 }  // namespace rows
+// Tensor maps of the K and V pages, a box of `rows` rows of one page and head (64
+// bf16 or 128 codes wide, 128-byte swizzle).
+int page_maps(CUtensorMap* k, CUtensorMap* v, const Keys& ky, int kv_heads, int rows);
 int join(const Keys& ky, const Queries& qr, const float* part_o, const float* part_l, int splits, cudaStream_t st);
 
 }  // namespace paged

@@ -4,16 +4,19 @@
 // Rows of one K/V head (tokens x the query heads that share it) come in tiles
 // of 16, the height of mma.sync's A operand, which here only has to keep up
 // with the loads: 32 instructions to 8 KB of K and V.  A cluster of up to 8
-// CTAs takes one tile of rows, each CTA a share of the keys, each warp every
-// fourth chunk of that share: its K and V rows arrive by cp.async in a ring of
-// its own (no CTA barrier in the loop, 2 x 8 KB a warp in flight, 128 KB an
-// SM), are multiplied straight from shared memory, and the warps' and CTAs'
-// sums are joined through (distributed) shared memory at the end.
+// CTAs takes one tile of rows, each CTA a share of the key tiles.  Warp 4 loads
+// tiles by TMA into a ring of three (64 KB in flight, two CTAs to an SM); warps
+// 0-3 take a quarter of a tile's keys each, multiply them straight from shared
+// memory and keep sums of their own, which are joined through (distributed)
+// shared memory at the end.  (With every warp loading its own chunks, issuing
+// four TMA copies cost 600 of 1700 clocks a chunk.)
 //
 // A contraction does not mind in which order its dimension is taken, so a
 // thread loads 16 consecutive bytes of a K row and feeds them to the k indices
 // it owns, with Q's fragments gathered in the same order; for 8-bit V it takes
 // 16 consecutive dims of four keys, and byte j of each makes output tile j.
+// Column n of a score tile is key n ^ 4 (n & 1): with the 128-byte swizzle the
+// eight lanes of a 16-byte read then meet eight bank groups for K and for V.
 // 8-bit pages: codes are exact in f16; a key's scale multiplies its score and
 // its P in f32 before P is rounded to f16 (2^-11), V's scales relative to the
 // largest power of two so far; Q rows are scaled by powers of two to f16.
@@ -27,13 +30,17 @@ namespace wfk {
 namespace paged {
 namespace rows {
 
-constexpr int WARPS = 4, THREADS = WARPS * 32, ST = 3, MAX_CLUSTER = 8;
-constexpr int KV_BYTES = 8192;             // K and V rows of a chunk
-constexpr int META_BYTES = 2 * 32 * 4 + 128;  // scales of K and V, the live keys
-constexpr int STAGE = KV_BYTES + META_BYTES;
+constexpr int WARPS = 4, THREADS = (WARPS + 1) * 32, ST = 3, MAX_CLUSTER = 8;
+constexpr int STAGE = 32768;               // a tile's K and V rows
+constexpr int MAX_BN = 128;
+constexpr int META = 2 * MAX_BN * 4 + 32;  // scales of K and V, live keys, whether every row sees all, the tile
 constexpr int O_PITCH = 132;               // floats of a row of partial sums, off the banks of the next
-constexpr int SMEM = WARPS * ST * STAGE + 128;
-static_assert(16 * (O_PITCH + 3) * 4 <= ST * STAGE, "a warp's sums fit its ring");
+constexpr int PART = 16 * (O_PITCH + 3) * 4;  // a warp's sums: O, m, l, and the CTA's m
+constexpr int SMEM = 1024 + ST * (STAGE + META + 16) + 16;
+static_assert(WARPS * PART <= ST * STAGE, "the sums lie over the ring");
+
+// Key of column n of an 8-key score tile.
+__device__ __forceinline__ int key_of(int n) { return n ^ ((n & 1) << 2); }
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -44,16 +51,6 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool take) {  // zeros when not taken
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool take) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(take ? 4 : 0) : "memory");
-}
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  const __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
 }
 // Two codes (low halves' bytes 0 and 1) -> f16x2, exact.
 template <int DT>
@@ -66,15 +63,6 @@ __device__ __forceinline__ uint32_t codes_f16(uint32_t two) {
   }
   return r;
 }
-__device__ __forceinline__ float pow2_above(float x) {  // power of two at or above x (> 0), within 2^+-122
-  const uint32_t e = ((__float_as_uint(x) + 0x7FFFFFu) >> 23) << 23;
-  return fminf(fmaxf(__uint_as_float(e), 0x1p-122f), 0x1p122f);
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 __device__ __forceinline__ float cluster_load(uint32_t saddr, uint32_t rank) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(saddr, rank)) : "memory");
@@ -82,30 +70,138 @@ __device__ __forceinline__ float cluster_load(uint32_t saddr, uint32_t rank) {
 }
 
 struct Cut {
+  Tiling tl;
   int cluster, outer;  // CTAs of a cluster; clusters to a tile of rows (joined through the workspace)
   int row_tiles;       // tiles of rows that the grid has to a sequence and K/V head
 };
 
 template <int DT>
 __global__ void __launch_bounds__(THREADS, 2)
-    rows_kernel(const __grid_constant__ Keys ky, const __grid_constant__ Queries qr, const __grid_constant__ Cut cut,
+    rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                const __grid_constant__ Keys ky, const __grid_constant__ Queries qr, const __grid_constant__ Cut cut,
                 float* part_o, float* part_l) {
   constexpr bool KV8 = DT != WF_DTYPE_BF16;
-  constexpr int KC = KV8 ? 32 : 16;        // keys of a chunk
+  constexpr int BN = KV8 ? 128 : 64;       // keys of a tile
+  constexpr int KC = BN / WARPS;           // keys of a warp
   constexpr int ROWB = KV8 ? 128 : 256;    // bytes of a row
-  constexpr int NT = KC / 8;               // score tiles of a chunk
-  extern __shared__ __align__(128) uint8_t smem[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  constexpr int NT = KC / 8;               // score tiles of a warp
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const uint32_t rank = cut.cluster > 1 ? cluster_ctarank() : 0;
   const int item = blockIdx.x / cut.cluster;
   const int G = qr.H / qr.group;
   const int rt0 = item % cut.row_tiles, hk = item / cut.row_tiles % G, b = item / cut.row_tiles / G;
   const Span sp = span_of(ky, qr, b);
-  uint8_t* ring = smem + warp * ST * STAGE;
-  const uint32_t ring_s = smem_u32(ring);
-  const int ps = ky.page_size;
+  const Tiling& tl = cut.tl;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + ST * (STAGE + META));
+  uint64_t* empty = full + ST;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + ST);
+  if (threadIdx.x == 0) {
+    for (int k = 0; k < ST; ++k) {
+      mbar_init(&full[k], 1);
+      mbar_init(&empty[k], WARPS);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  uint32_t done = 0;  // tiles through the ring
 
   for (int rt = rt0; rt * 16 < sp.n * qr.group; rt += cut.row_tiles) {
+    const int i0 = rt * 16 / qr.group, i1 = min((rt * 16 + 15) / qr.group, sp.n - 1);
+    const Range rg = range_of<BN>(qr, sp, tl, i0, i1);
+    const int n_rows = min(16, sp.n * qr.group - rt * 16);
+    const int parts = cut.cluster * cut.outer, part = blockIdx.y * cut.cluster + rank;
+    const int p0 = (int)((long long)rg.n * part / parts), p1 = (int)((long long)rg.n * (part + 1) / parts);
+    if (warp == WARPS) {
+      // ---------------------------------------------------------- producer
+      // Page ids (a lane to a page for the copies, four keys to a lane for the
+      // marks) are fetched a tile ahead, scales under the wait for the stage.
+      constexpr int KL = BN / 32;
+      int box_id = -1, ids[KL];
+      auto spot = [&](const TileAt& a, int c, int& j, int& off) -> bool {  // key c * 32 + lane of a tile; seen at all?
+        const int r = c * 32 + lane;
+        off = a.row + r;
+        j = a.page;
+        bool in = off < tl.ps;
+        if (tl.ps < BN) {
+          const int p = r / tl.rows;
+          off = r - p * tl.rows;
+          j += p;
+          in = off < tl.ps && p < tl.ppt;
+        }
+        const int pos = j * tl.ps + off;
+        return in && ((pos < rg.hi && pos >= rg.lo) || pos < rg.sink);
+      };
+      auto look = [&](int i) {
+        const TileAt a = tile_at<BN>(tl, nth_tile(rg, i));
+        box_id = lane < tl.ppt && needed(rg, tl, a.page + lane) ? page_id(ky, sp, b, a.page + lane) : -1;
+        int j, off;
+#pragma unroll
+        for (int c = 0; c < KL; ++c) ids[c] = spot(a, c, j, off) ? page_id(ky, sp, b, j) : INT_MIN;
+      };
+      if (p0 < p1) look(p0);
+      for (int i = p0; i < p1; ++i, ++done) {
+        const TileAt a = tile_at<BN>(tl, nth_tile(rg, i));
+        const int box = box_id >= 0 && box_id < ky.n_pages ? box_id : -1;
+        bool in[KL];
+        float sk[KL], sv[KL];
+#pragma unroll
+        for (int c = 0; c < KL; ++c) {
+          int j, off;
+          spot(a, c, j, off);
+          in[c] = ids[c] >= 0 && ids[c] < ky.n_pages;
+          if (!in[c] && ids[c] != INT_MIN) status_raise(ST_PAGE_ID);
+          sk[c] = sv[c] = 0.f;
+          if constexpr (KV8) {
+            if (in[c]) {
+              sk[c] = __ldg(ky.ks + ids[c] * ky.ks_str[0] + hk * ky.ks_str[1] + off);
+              sv[c] = __ldg(ky.vs + ids[c] * ky.vs_str[0] + hk * ky.vs_str[1] + off);
+            }
+          } else if (ky.mask && in[c]) {
+            in[c] = __ldg(ky.mask + ids[c] * ky.mask_stride + off) != 0;
+          }
+        }
+        if (i + 1 < p1) look(i + 1);
+        const uint32_t st = done % ST, turn = done / ST;
+        if (turn > 0 && !warp_wait(&empty[st], turn - 1, abort_flag, ST_PAGED_ROWS)) break;
+        uint8_t *at = smem + st * STAGE, *mt = smem + ST * STAGE + st * META;
+        uint32_t all = 0xFFFFFFFFu;
+#pragma unroll
+        for (int c = 0; c < KL; ++c) {
+          const uint32_t word = __ballot_sync(0xffffffffu, in[c]);
+          all &= word;
+          if (lane == c) reinterpret_cast<uint32_t*>(mt + 2 * MAX_BN * 4)[c] = word;
+          if constexpr (KV8) {
+            reinterpret_cast<float*>(mt)[c * 32 + lane] = sk[c];
+            reinterpret_cast<float*>(mt)[MAX_BN + c * 32 + lane] = sv[c];
+          }
+        }
+        const bool whole = all == 0xFFFFFFFFu && a.base + BN <= rg.hi_min &&
+                           (a.base >= rg.lo_max || a.base + BN <= rg.sink_min);
+        if (lane == 4) *reinterpret_cast<uint2*>(mt + 2 * MAX_BN * 4 + 16) = make_uint2(whole, nth_tile(rg, i));
+        const uint32_t boxes = __ballot_sync(0xffffffffu, box >= 0), bytes = (uint32_t)tl.rows * 128;
+        if (lane == 0) mbar_arrive_expect_tx(&full[st], __popc(boxes) * bytes * (KV8 ? 2 : 4));
+        __syncwarp();
+        if (box >= 0) {
+          uint8_t* k = at + lane * bytes;
+          uint8_t* v = k + STAGE / 2;
+          tma_load_4d(k, &tmK, &full[st], 0, a.row, hk, box);
+          if constexpr (!KV8) tma_load_4d(k + STAGE / 4, &tmK, &full[st], 64, a.row, hk, box);
+          tma_load_4d(v, &tmV, &full[st], 0, a.row, hk, box);
+          if constexpr (!KV8) tma_load_4d(v + STAGE / 4, &tmV, &full[st], 64, a.row, hk, box);
+        }
+        __syncwarp();
+      }
+      if (*abort_flag && lane == 0) {  // let the loads in flight land before their place is used again
+        const uint64_t t0 = globaltimer_ns();
+        for (uint32_t k = done > ST ? done - ST : 0; k < done; ++k)
+          while (!mbar_try_wait(&full[k % ST], (k / ST) & 1) && globaltimer_ns() - t0 < 200000000ull) {
+          }
+      }
+      __syncwarp();
+    } else {
     // This thread's two rows, g and g + 8.
     int tok[2], head[2];
     bool has[2];
@@ -149,82 +245,15 @@ __global__ void __launch_bounds__(THREADS, 2)
         for (int e = 0; e < 2; ++e) {
           if constexpr (KV8) {
             const float inv = 1.f / q_pow[e];
-            a[s][e] = pack_f16(__uint_as_float(v[s][e].x << 16) * inv, __uint_as_float(v[s][e].x & 0xFFFF0000u) * inv);
-            a[s][2 + e] = pack_f16(__uint_as_float(v[s][e].y << 16) * inv, __uint_as_float(v[s][e].y & 0xFFFF0000u) * inv);
+            a[s][e] = f16x2(__uint_as_float(v[s][e].x << 16) * inv, __uint_as_float(v[s][e].x & 0xFFFF0000u) * inv);
+            a[s][2 + e] = f16x2(__uint_as_float(v[s][e].y << 16) * inv, __uint_as_float(v[s][e].y & 0xFFFF0000u) * inv);
           } else {
             a[s][e] = v[s][e].x;
             a[s][2 + e] = v[s][e].y;
           }
         }
     }
-    // The keys that the tile's rows see together, in chunks of consecutive
-    // positions, and this warp's share of them.
-    const int i0 = rt * 16 / qr.group, i1 = min((rt * 16 + 15) / qr.group, sp.n - 1);
-    const Sees first = sees(qr, sp, max(i0, min(-sp.pos0, i1))), last = sees(qr, sp, i1);
-    const int hi = last.hi, lo = first.lo, sink = min(last.sink, hi);
-    const int hi_min = i0 + sp.pos0 < 0 ? 0 : first.hi, lo_max = last.lo, sink_min = first.sink;
-    const int n_rows = min(16, sp.n * qr.group - rt * 16);
     const float q_scale[2] = {q_pow[0] * qr.scale_log2, q_pow[1] * qr.scale_log2};
-    int n_sink = 0, c_lo = 0, n = 0;
-    if (hi > 0) {
-      c_lo = lo / KC;
-      n_sink = sink > 0 ? min((sink - 1) / KC + 1, c_lo) : 0;
-      n = n_sink + (hi - 1) / KC + 1 - c_lo;
-    }
-    const int parts = cut.cluster * cut.outer, part = blockIdx.y * cut.cluster + rank;
-    const int p0 = (int)((long long)n * part / parts) + warp, p1 = (int)((long long)n * (part + 1) / parts);
-
-    // Key lane % KC of a chunk: page and row, fetched a chunk ahead of its loads.
-    int nx_id = -1, nx_off = 0;
-    bool nx_in = false;
-    auto look = [&](int i) {
-      nx_in = false;
-      nx_id = -1;
-      if (i < p1) {
-        const int pos = (i < n_sink ? i : i - n_sink + c_lo) * KC + (lane % KC);
-        if ((pos < hi && pos >= lo) || pos < sink) {
-          const int j = pos / ps;
-          nx_off = pos - j * ps;
-          nx_id = page_id(ky, sp, b, j);
-          nx_in = !(ky.mask && nx_id >= 0) || __ldg(ky.mask + nx_id * ky.mask_stride + pos) != 0;
-        }
-      }
-    };
-    auto issue = [&](int i, int stage) {
-      const uint32_t at = ring_s + stage * STAGE;
-      if (i < p1) {
-        int id = nx_id;
-        const int off = nx_off;
-        if (nx_in && (id < 0 || id >= ky.n_pages)) {
-          status_raise(ST_PAGE_ID);
-          id = -1;
-        }
-        if (!nx_in) id = -1;
-        const uint32_t live = __ballot_sync(0xffffffffu, id >= 0);
-        if (lane == 0) *reinterpret_cast<uint32_t*>(ring + stage * STAGE + KV_BYTES + 256) = live;
-        if constexpr (KV8) {
-          cp4(at + KV_BYTES + lane * 4, ky.ks + (id >= 0 ? id * ky.ks_str[0] + hk * ky.ks_str[1] + off : 0), id >= 0);
-          cp4(at + KV_BYTES + 128 + lane * 4, ky.vs + (id >= 0 ? id * ky.vs_str[0] + hk * ky.vs_str[1] + off : 0),
-              id >= 0);
-        }
-        // Row offsets (bytes) of this lane's key, then each lane's share of 16-byte pieces.
-        constexpr int CH = ROWB / 16, RPI = 32 / CH;  // pieces of a row, rows that an instruction covers
-        constexpr int ES = KV8 ? 1 : 2;
-        const int64_t kr = id >= 0 ? (id * ky.k_str[0] + hk * ky.k_str[1] + off * ky.k_str[2]) * ES : -1;
-        const int64_t vr = (id * ky.v_str[0] + hk * ky.v_str[1] + off * ky.v_str[2]) * ES;
-        const int c = lane % CH;
-        const uint8_t *kb = static_cast<const uint8_t*>(ky.k) + c * 16, *vb = static_cast<const uint8_t*>(ky.v) + c * 16;
-#pragma unroll
-        for (int k = 0; k < KC / RPI; ++k) {
-          const int r = k * RPI + lane / CH;
-          const int64_t ko = __shfl_sync(0xffffffffu, kr, r), vo = __shfl_sync(0xffffffffu, vr, r);
-          const bool take = ko >= 0;
-          cp16(at + r * ROWB + ((c ^ ((r & 1) << 2)) << 4), kb + (take ? ko : 0), take);
-          cp16(at + KC * ROWB + r * ROWB + ((c ^ (r & 7)) << 4), vb + (take ? vo : 0), take);
-        }
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
 
     float o[16][4];
 #pragma unroll
@@ -233,60 +262,64 @@ __global__ void __launch_bounds__(THREADS, 2)
       for (int e = 0; e < 4; ++e) o[k][e] = 0.f;
     float m_run[2] = {-INFINITY, -INFINITY}, m_use[2] = {0.f, 0.f}, l_run[2] = {0.f, 0.f}, v_top = 0.f;
 
-    look(p0);
+    for (int i = p0; i < p1; ++i, ++done) {
+      const uint32_t st = done % ST;
+      if (!warp_wait(&full[st], done / ST, abort_flag, ST_PAGED_ROWS)) break;
+      uint8_t* K = smem + st * STAGE + warp * KC * 128;
+      uint8_t* V = K + STAGE / 2;
+      const uint8_t* mt = smem + ST * STAGE + st * META;
+      const float* scale = reinterpret_cast<const float*>(mt) + warp * KC;
+      const uint2 mark = *reinterpret_cast<const uint2*>(mt + 2 * MAX_BN * 4 + 16);
+      const bool whole = mark.x != 0;
+      uint32_t keep[2] = {~0u, ~0u}, live = ~0u;  // by key of this warp
+      if (!whole) {
+        const int k0 = warp * KC;
+        live = reinterpret_cast<const uint32_t*>(mt + 2 * MAX_BN * 4)[k0 >> 5] >> (k0 & 31);
+        const TileAt a = tile_at<BN>(tl, mark.y);
 #pragma unroll
-    for (int k = 0; k < ST - 1; ++k) {
-      issue(p0 + k * WARPS, k);
-      look(p0 + (k + 1) * WARPS);
-    }
-    int stage = 0;
-    for (int i = p0; i < p1; i += WARPS) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(ST - 2) : "memory");
-      __syncwarp();
-      // the stage that the last chunk used is free: all lanes are past it
-      issue(i + (ST - 1) * WARPS, stage == 0 ? ST - 1 : stage - 1);
-      look(i + ST * WARPS);
-      const uint8_t* K = ring + stage * STAGE;
-      const uint8_t* V = K + KC * ROWB;
-      const float* scale = reinterpret_cast<const float*>(K + KV_BYTES);
-      const uint32_t live = *reinterpret_cast<const uint32_t*>(K + KV_BYTES + 256);
+        for (int e = 0; e < 2; ++e)
+          keep[e] = live & (bit_range(rows_below<BN>(tl, a, se[e].lo), rows_below<BN>(tl, a, se[e].hi), k0) |
+                            bit_range(0, rows_below<BN>(tl, a, se[e].sink), k0));
+        // V rows that no query sees may hold NaN
+        constexpr int PER = ROWB / 16;  // 16-byte pieces of a row
+        for (int r = lane / PER; r < KC; r += 32 / PER)
+          if (!(live >> r & 1))
+            *reinterpret_cast<uint4*>(V + (lane % PER / 8) * (STAGE / 4) + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async_smem();  // the ring's next TMA comes after these writes
+        __syncwarp();
+      }
 
       float s[NT][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
-        const int r = nt * 8 + g;
+        float c0[4] = {0.f, 0.f, 0.f, 0.f}, c1[4] = {0.f, 0.f, 0.f, 0.f};  // two chains to a tile
+        const int r = nt * 8 + key_of(g);
 #pragma unroll
         for (int c = 0; c < ROWB / 64; ++c) {
-          const uint4 w = *reinterpret_cast<const uint4*>(K + r * ROWB + (((t + 4 * c) ^ ((r & 1) << 2)) << 4));
+          const uint4 w = *reinterpret_cast<const uint4*>(K + (c >> 1) * (STAGE / 4) + r * 128 +
+                                                          (((t + 4 * (c & 1)) ^ (r & 7)) << 4));
           if constexpr (KV8) {
             const uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-              mma_f16(s[nt], a[c * 4 + k], codes_f16<DT>(x[k] & 0xFFFFu), codes_f16<DT>(x[k] >> 16));
+              mma_f16(k & 1 ? c1 : c0, a[c * 4 + k], codes_f16<DT>(x[k] & 0xFFFFu), codes_f16<DT>(x[k] >> 16));
           } else {
-            mma_bf16(s[nt], a[2 * c], w.x, w.y);
-            mma_bf16(s[nt], a[2 * c + 1], w.z, w.w);
+            mma_bf16(c0, a[2 * c], w.x, w.y);
+            mma_bf16(c1, a[2 * c + 1], w.z, w.w);
           }
         }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[nt][e] = c0[e] + c1[e];
       }
       // Scores in log2 units, -inf where the row does not see the key.
-      const int pos0 = (i < n_sink ? i : i - n_sink + c_lo) * KC;
-      const bool whole = live == (KC == 32 ? 0xFFFFFFFFu : (1u << (KC & 31)) - 1) && pos0 + KC <= hi_min &&
-                         (pos0 >= lo_max || pos0 + KC <= sink_min);
       float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const float2 ks = KV8 ? *reinterpret_cast<const float2*>(scale + nt * 8 + 2 * t) : make_float2(1.f, 1.f);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          s[nt][e] *= KV8 ? q_scale[e >> 1] * ((e & 1) ? ks.y : ks.x) : qr.scale_log2;
-          if (!whole) {
-            const int k = nt * 8 + 2 * t + (e & 1), pos = pos0 + k;
-            const Sees& v = se[e >> 1];
-            if (!((live >> k & 1) && pos < v.hi && (pos >= v.lo || pos < v.sink))) s[nt][e] = -INFINITY;
-          }
+          const int k = nt * 8 + key_of(2 * t + (e & 1));
+          s[nt][e] *= KV8 ? q_scale[e >> 1] * scale[k] : qr.scale_log2;
+          if (!whole && !(keep[e >> 1] >> k & 1)) s[nt][e] = -INFINITY;
           mx[e >> 1] = max_nan(mx[e >> 1], s[nt][e]);
         }
       }
@@ -299,7 +332,7 @@ __global__ void __launch_bounds__(THREADS, 2)
       }
       float v_new = v_top;
       if constexpr (KV8) {
-        float top = live >> lane & 1 ? fabsf(scale[32 + lane]) : 0.f;
+        float top = fabsf(scale[MAX_BN + lane]);  // 0 where a key is not seen at all
         if (!(top < INFINITY)) top = 0.f;
         top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
         if (v_top == 0.f || top > v_top) v_new = pow2_above(top) * 8.f;
@@ -337,12 +370,11 @@ __global__ void __launch_bounds__(THREADS, 2)
           l_run[e >> 1] += x[e];
         }
         if constexpr (KV8) {
-          const float2 vs = *reinterpret_cast<const float2*>(scale + 32 + nt * 8 + 2 * t);
 #pragma unroll
           for (int e = 0; e < 4; ++e)  // a key that is not seen does not count, whatever its scale
-            x[e] = s[nt][e] == -INFINITY ? 0.f : x[e] * (((e & 1) ? vs.y : vs.x) * v_inv);
-          p[nt >> 1][(nt & 1) * 2] = pack_f16(x[0], x[1]);
-          p[nt >> 1][(nt & 1) * 2 + 1] = pack_f16(x[2], x[3]);
+            x[e] = s[nt][e] == -INFINITY ? 0.f : x[e] * (scale[MAX_BN + nt * 8 + key_of(2 * t + (e & 1))] * v_inv);
+          p[nt >> 1][(nt & 1) * 2] = f16x2(x[0], x[1]);
+          p[nt >> 1][(nt & 1) * 2 + 1] = f16x2(x[2], x[3]);
         } else {
           p[nt >> 1][(nt & 1) * 2] = pack_bf16x2(x[0], x[1]);
           p[nt >> 1][(nt & 1) * 2 + 1] = pack_bf16x2(x[2], x[3]);
@@ -351,11 +383,11 @@ __global__ void __launch_bounds__(THREADS, 2)
 #pragma unroll
       for (int k16 = 0; k16 < NT / 2; ++k16) {
         if constexpr (KV8) {
-          uint4 w[4];  // dims 16 g .. 16 g + 15 of keys 2t, 2t + 1, 2t + 8, 2t + 9
+          uint4 w[4];  // dims 16 g .. 16 g + 15 of the keys of columns 2t, 2t + 1, 2t + 8, 2t + 9
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int r = k16 * 16 + 2 * t + (e & 1) + (e >> 1) * 8;
-            w[e] = *reinterpret_cast<const uint4*>(V + r * ROWB + ((g ^ (r & 7)) << 4));
+            const int r = k16 * 16 + key_of(2 * t + (e & 1)) + (e >> 1) * 8;
+            w[e] = *reinterpret_cast<const uint4*>(V + r * 128 + ((g ^ (r & 7)) << 4));
           }
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
@@ -365,25 +397,26 @@ __global__ void __launch_bounds__(THREADS, 2)
                     codes_f16<DT>(__byte_perm(word(w[2]), word(w[3]), sel) & 0xFFFFu));
           }
         } else {
-          const int mat = lane >> 3, r = (lane & 7) + (mat & 1) * 8;
+          const int mat = lane >> 3, r = key_of(lane & 7) + (mat & 1) * 8;
 #pragma unroll
           for (int d = 0; d < 8; ++d) {
             uint32_t v0, v1, v2, v3;
             asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                          : "=r"(v0), "=r"(v1), "=r"(v2), "=r"(v3)
-                         : "r"(smem_u32(V + r * ROWB + (((2 * d + (mat >> 1)) ^ (r & 7)) << 4)))
+                         : "r"(smem_u32(V + (d >> 2) * (STAGE / 4) + r * 128 +
+                                        (((2 * (d & 3) + (mat >> 1)) ^ (r & 7)) << 4)))
                          : "memory");
             mma_bf16(o[2 * d], p[0], v0, v1);
             mma_bf16(o[2 * d + 1], p[0], v2, v3);
           }
         }
       }
-      stage = stage + 1 == ST ? 0 : stage + 1;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
-    __syncwarp();
+    named_bar_sync(1, WARPS * 32);  // the sums lie over the ring: every warp is past it
     // ---- the warps' sums: O [16][O_PITCH], then m[16], l[16], over the ring
-    float* mine = reinterpret_cast<float*>(ring);
+    float* mine = reinterpret_cast<float*>(smem + warp * PART);
     if (KV8 && v_top == 0.f) v_top = 1.f;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -402,10 +435,11 @@ __global__ void __launch_bounds__(THREADS, 2)
           mine[(g + e * 8) * O_PITCH + d] = KV8 ? o[k][2 * e + f] * v_top : o[k][2 * e + f];
         }
     }
+    }
     __syncthreads();
     // The CTA's sums, into warp 0's place: first each row's maximum, l and the
     // warps' weights (in place of their maxima), then thread x dim x of the rows.
-    constexpr int PITCH_W = ST * STAGE / 4;
+    constexpr int PITCH_W = PART / 4;
     float* base = reinterpret_cast<float*>(smem);
     const int dim = threadIdx.x;
     if (dim < n_rows) {
@@ -424,6 +458,7 @@ __global__ void __launch_bounds__(THREADS, 2)
       at[32] = m;
     }
     __syncthreads();
+    if (dim < HD)
 #pragma unroll 2
     for (int r = 0; r < n_rows; ++r) {
       float x = 0.f;
@@ -437,9 +472,9 @@ __global__ void __launch_bounds__(THREADS, 2)
     else
       __syncthreads();
     // CTA `rank` finishes rows rank, rank + cluster, ...: the CTAs' sums joined.
-    for (int r = rank; r < n_rows; r += cut.cluster) {
-      const int rg = rt * 16 + r, i = rg / qr.group;
-      const int h = hk * qr.group + rg - i * qr.group;
+    for (int r = rank; r < n_rows && dim < HD; r += cut.cluster) {
+      const int row = rt * 16 + r, i = row / qr.group;
+      const int h = hk * qr.group + row - i * qr.group;
       const uint32_t am = smem_u32(base + 16 * O_PITCH + 32 + r), ao = smem_u32(base + r * O_PITCH + dim);
       float m = -INFINITY, l = 0.f, x = 0.f;
       if (cut.cluster > 1) {
@@ -469,7 +504,8 @@ __global__ void __launch_bounds__(THREADS, 2)
         if (qr.lse && dim == 0) qr.lse[packed] = lse2 * 0.6931471805599453f;
       }
     }
-    // the others may still read this CTA's sums
+    // the others may still read this CTA's sums; the next rows' TMA comes after
+    fence_proxy_async_smem();
     if (cut.cluster > 1)
       cluster_sync();
     else
@@ -478,25 +514,34 @@ __global__ void __launch_bounds__(THREADS, 2)
 }
 
 // --------------------------------------------------------------------- host
-// Enough CTAs for every SM's two places, as long as each keeps two chunks to a
-// warp; what a cluster cannot give, clusters joined afterwards do as far as one
-// CTA to each SM.
+// The cut of the keys with the least estimated time, in tiles: those of all
+// waves of CTAs with about six for a CTA's
+// start and end, half of one CTA's again because sequences differ in length,
+// and four for the join of clusters.
+constexpr int PLACES = 2 * SMS;
 static Cut cut_of(const Shape& sh, bool kv8) {
-  const int64_t chunk = kv8 ? 32 : 16;
-  Cut c{1, 1, (int)((sh.max_new * sh.group + 15) / 16)};
+  const int bn = kv8 ? 128 : 64;
+  Cut c{tiling_of(sh.page_size, bn), 1, 1, (int)((sh.max_new * sh.group + 15) / 16)};
   if (c.row_tiles < 1) c.row_tiles = 1;
   const int64_t seqs = sh.seqs < sh.rows ? sh.seqs : sh.rows;
-  const int64_t items = seqs * (sh.H / sh.group) * c.row_tiles, most = sh.keys / (chunk * WARPS * 2);
-  while (c.cluster < MAX_CLUSTER && items * c.cluster < 2 * SMS && 2 * c.cluster <= most) c.cluster *= 2;
-  if (c.cluster == MAX_CLUSTER)
-    while (c.outer < 16 && items * c.cluster * c.outer < SMS && 2 * c.outer * c.cluster <= most) c.outer *= 2;
+  const int64_t items = seqs * (sh.H / sh.group) * c.row_tiles;
+  const int64_t n = tiles_of_keys(sh, bn);
+  double best = 1e30;
+  for (int cluster = 1; cluster <= MAX_CLUSTER; cluster *= 2)
+    for (int outer = 1; outer <= 16 && (cluster == MAX_CLUSTER || outer == 1); ++outer) {
+      if (cluster * outer > 1 && n < (int64_t)cluster * outer * 2) break;
+      const double rounds = (double)((n + cluster * outer - 1) / (cluster * outer));
+      const double cost = (double)((items * cluster * outer + PLACES - 1) / PLACES) * (rounds + 6) + 0.5 * rounds +
+                          (outer > 1 ? 4 : 0);
+      if (cost < best) best = cost, c.cluster = cluster, c.outer = outer;
+    }
   return c;
 }
 
 int splits(const Shape& sh) { return cut_of(sh, sh.kv8).outer; }
 
 template <int DT>
-static int start(const Keys& ky, const Queries& qr, const Cut& cut, float* part_o, float* part_l, cudaStream_t st) {
+static int start(const CUtensorMap& tk, const CUtensorMap& tv, const Keys& ky, const Queries& qr, const Cut& cut, float* part_o, float* part_l, cudaStream_t st) {
   static thread_local int configured = -1;
   int dev = 0;
   WFK_CUDA_TRY(cudaGetDevice(&dev));
@@ -514,7 +559,7 @@ static int start(const Keys& ky, const Queries& qr, const Cut& cut, float* part_
   at.val.clusterDim = {(unsigned)cut.cluster, 1, 1};
   cfg.attrs = &at;
   cfg.numAttrs = cut.cluster > 1 ? 1 : 0;
-  WFK_CUDA_TRY(cudaLaunchKernelEx(&cfg, rows_kernel<DT>, ky, qr, cut, part_o, part_l));
+  WFK_CUDA_TRY(cudaLaunchKernelEx(&cfg, rows_kernel<DT>, tk, tv, ky, qr, cut, part_o, part_l));
   return WF_OK;
 }
 
@@ -527,9 +572,12 @@ int launch(const Keys& ky, const Queries& qr, const Shape& sh, void* workspace, 
     part_o = static_cast<float*>(workspace);
     part_l = part_o + (int64_t)cut.outer * qr.rows * qr.H * HD;
   }
-  const int rc = ky.dtype == WF_DTYPE_BF16   ? start<WF_DTYPE_BF16>(ky, qr, cut, part_o, part_l, st)
-                 : ky.dtype == WF_DTYPE_E4M3 ? start<WF_DTYPE_E4M3>(ky, qr, cut, part_o, part_l, st)
-                                             : start<WF_DTYPE_S8>(ky, qr, cut, part_o, part_l, st);
+  CUtensorMap tk, tv;
+  int rc;
+  if ((rc = page_maps(&tk, &tv, ky, qr.H / qr.group, cut.tl.rows)) != WF_OK) return rc;
+  rc = ky.dtype == WF_DTYPE_BF16   ? start<WF_DTYPE_BF16>(tk, tv, ky, qr, cut, part_o, part_l, st)
+       : ky.dtype == WF_DTYPE_E4M3 ? start<WF_DTYPE_E4M3>(tk, tv, ky, qr, cut, part_o, part_l, st)
+                                   : start<WF_DTYPE_S8>(tk, tv, ky, qr, cut, part_o, part_l, st);
   if (rc != WF_OK || cut.outer == 1) return rc;
   return join(ky, qr, part_o, part_l, cut.outer, st);
 }

@@ -41,7 +41,7 @@ constexpr int SLOT = 2 * HALF;    // a K or V tile, or a Q sub-tile: [d 0-63][d 
 constexpr int META = 3;           // tiles whose marks (and scales) are kept
 constexpr uint32_t COL_S = 0, COL_O = 256;
 
-constexpr int WORK_BYTES = 80;
+constexpr int WORK_BYTES = 96;
 template <bool KV8>
 struct Cfg {
   static constexpr int NS = KV8 ? 4 : 5;  // ring slots
@@ -52,52 +52,12 @@ struct Cfg {
   static_assert(SMEM <= 232448, "shared memory of one CTA");
 };
 
-// How the keys of a sequence fall into tiles: pages of at least 128 rows give
-// ceil(page_size / 128) tiles each, smaller ones share a tile, a page on every
-// `rows` tile rows (page_size rounded up to the swizzle's 8).
-struct Tiling {
-  int ps, tpp, ppt, rows;  // tiles per page (large pages), pages per tile (small), tile rows of a page
-  int tq;                  // tokens of a sub-tile
-  int splits;
-};
-__device__ __forceinline__ int tile_of(const Tiling& tl, int pos) {
-  const int j = pos / tl.ps;
-  return tl.ps < BN ? j / tl.ppt : j * tl.tpp + (pos - j * tl.ps) / BN;
-}
-struct TileAt {
-  int page, row, base;  // first page, row in it, position of the tile's first key
-};
-__device__ __forceinline__ TileAt tile_at(const Tiling& tl, int t) {
-  TileAt a;
-  if (tl.ps < BN) {
-    a.page = t * tl.ppt;
-    a.row = 0;
-  } else {
-    a.page = t / tl.tpp;
-    a.row = (t - a.page * tl.tpp) * BN;
-  }
-  a.base = a.page * tl.ps + a.row;
-  return a;
-}
-// Tile rows whose position is below x.
-__device__ __forceinline__ int rows_below(const Tiling& tl, const TileAt& a, int x) {
-  const int d = x - a.base;
-  if (d <= 0) return 0;
-  if (tl.ps >= BN) return min(d, min(BN, tl.ps - a.row));
-  const int j = d / tl.ps;
-  return min(j, tl.ppt) * tl.rows + (j < tl.ppt ? d - j * tl.ps : 0);
-}
-
-struct Work {
+struct Work : Range {
   int b, hk, split;
   int i0, nsub;  // first token, sub-tiles with rows
   Span sp;
-  int hi, lo, sink;  // keys the item's rows see together: [0, sink) and [lo, hi)
-  int hi_min, lo_max, sink_min;  // and those that each of them sees
-  int n_sink, t_lo;  // tiles of the sink range; first tile of the other
-  int t0, t1;        // this item's share of the tile list
+  int t0, t1;    // this item's share of the tile list
 };
-
 static_assert(sizeof(Work) <= WORK_BYTES, "a softmax warp's item");
 
 // Query tiles of the launch over all sequences (one warp).
@@ -153,37 +113,12 @@ __device__ __forceinline__ bool find_work(Work& w, const Keys& ky, const Queries
   w.i0 = tile * 2 * tl.tq;
   const int i1 = min(w.i0 + 2 * tl.tq, w.sp.n) - 1;  // last token
   w.nsub = i1 >= w.i0 + tl.tq ? 2 : 1;
-  const Sees last = sees(qr, w.sp, i1);
-  const Sees first = sees(qr, w.sp, max(w.i0, min(-w.sp.pos0, i1)));  // earlier rows have no position
-  w.hi = last.hi;
-  w.lo = first.lo;
-  w.sink = min(last.sink, w.hi);
-  w.hi_min = w.i0 + w.sp.pos0 < 0 ? 0 : first.hi;
-  w.lo_max = last.lo;
-  w.sink_min = first.sink;
-  int n = 0;
-  w.n_sink = w.t_lo = 0;
-  if (w.hi > 0) {
-    const int t_hi = tile_of(tl, w.hi - 1) + 1;
-    w.t_lo = tile_of(tl, w.lo);
-    w.n_sink = w.sink > 0 ? min(tile_of(tl, w.sink - 1) + 1, w.t_lo) : 0;
-    n = w.n_sink + t_hi - w.t_lo;
-  }
-  w.t0 = (int)((long long)n * w.split / tl.splits);
-  w.t1 = (int)((long long)n * (w.split + 1) / tl.splits);
+  static_cast<Range&>(w) = range_of<BN>(qr, w.sp, tl, w.i0, i1);
+  w.t0 = (int)((long long)w.n * w.split / tl.splits);
+  w.t1 = (int)((long long)w.n * (w.split + 1) / tl.splits);
   return true;
 }
-__device__ __forceinline__ int nth_tile(const Work& w, int i) { return i < w.n_sink ? i : i - w.n_sink + w.t_lo; }
 
-// Whether some row of the item sees a key of its sequence's page j.
-__device__ __forceinline__ bool needed(const Work& w, const Tiling& tl, int j) {
-  const long long p0 = (long long)j * tl.ps;
-  return (p0 < w.hi && p0 + tl.ps > w.lo) || p0 < w.sink;
-}
-
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, uint32_t code) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity & 1, abort, code));
-}
 __device__ __forceinline__ bool drain(uint64_t* bar, uint32_t parity, uint64_t ns) {
   const uint64_t t0 = globaltimer_ns();
   while (!mbar_try_wait(bar, parity & 1))
@@ -194,17 +129,6 @@ __device__ __forceinline__ bool drain(uint64_t* bar, uint32_t parity, uint64_t n
   return true;
 }
 
-// Maximum of three, NaN if one is NaN (a NaN score must reach the row's result).
-__device__ __forceinline__ float max3_nan(float a, float b, float c) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-
-__device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
-  const __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
 // c * (hi + lo) for a pair of codes: the row's scale in 22 bits, so that its
 // rounding does not shift all of a key's products the same way.
 __device__ __forceinline__ uint32_t scaled_f16x2(uint32_t c, uint32_t hi, uint32_t lo) {
@@ -269,12 +193,6 @@ __device__ __forceinline__ void expand_rows(uint8_t* slot, int row0, int lane, c
   }
 }
 
-// Power of two at or above x (> 0), between 2^-122 and 2^122 (a row scale is below 2^122).
-__device__ __forceinline__ float pow2_above(float x) {
-  const uint32_t e = ((__float_as_uint(x) + 0x7FFFFFu) >> 23) << 23;
-  return fminf(fmaxf(__uint_as_float(e), 0x1p-122f), 0x1p122f);
-}
-
 // Q rows of one converter warp (32 of a sub-tile, swizzled bf16) to f16 in
 // place, each divided by the power of two above its largest value; the powers
 // go to qpow.  Half a warp to a row, 16 bytes a lane.
@@ -298,13 +216,6 @@ __device__ __forceinline__ void expand_q(uint8_t* sub, int row0, int lane, float
     *at = make_uint4(w[0], w[1], w[2], w[3]);
     if ((lane & 15) == 0) qpow[r] = p;
   }
-}
-
-// Bits [a, b) of a 32-bit word that starts at bit `at`.
-__device__ __forceinline__ uint32_t bit_range(int a, int b, int at) {
-  const int lo = min(max(a - at, 0), 32), hi = min(max(b - at, 0), 32);
-  if (hi <= lo) return 0;
-  return (0xFFFFFFFFu >> (32 - (hi - lo))) << lo;
 }
 
 template <int DT>
@@ -398,7 +309,7 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
       const int sub = lane;       // a lane to a page of the tile
       // A lane's page of tile t, as the table has it (-1: not needed); checked when it is used.
       auto page_for = [&](int t, int& row) -> int {
-        const TileAt a = tile_at(tl, t);
+        const TileAt a = tile_at<BN>(tl, t);
         row = a.row;
         return sub < tl.ppt && needed(w, tl, a.page + sub) ? page_id(ky, w.sp, w.b, a.page + sub) : -1;
       };
@@ -557,7 +468,7 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
         return in && ((pos < w.hi && pos >= w.lo) || pos < w.sink);
       };
       auto fetch_ids = [&](int i) {
-        const TileAt a = tile_at(tl, nth_tile(w, i));
+        const TileAt a = tile_at<BN>(tl, nth_tile(w, i));
         int j, off;
 #pragma unroll
         for (int c = 0; c < 4; ++c) ids[c] = spot(a, c, j, off) ? page_id(ky, w.sp, w.b, j) : INT_MIN;
@@ -566,7 +477,7 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
         float v_top = 0.f;  // power of two of V so far
         if (w.t0 < w.t1) fetch_ids(w.t0);
         for (int i = w.t0; ok && i < w.t1; ++i, ++tiles) {
-          const TileAt a = tile_at(tl, nth_tile(w, i));
+          const TileAt a = tile_at<BN>(tl, nth_tile(w, i));
           bool in[4];
           float sk[KV8 ? 4 : 1], sv[KV8 ? 4 : 1];
 #pragma unroll
@@ -703,9 +614,9 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
         // Which of the tile's keys this row sees.
         uint32_t keep[4];
         if (masked) {
-          const TileAt at = tile_at(tl, nth_tile(w, w.t0 + j));
-          const int b_hi = rows_below(tl, at, se.hi), b_lo = rows_below(tl, at, se.lo);
-          const int b_sink = rows_below(tl, at, se.sink);
+          const TileAt at = tile_at<BN>(tl, nth_tile(w, w.t0 + j));
+          const int b_hi = rows_below<BN>(tl, at, se.hi), b_lo = rows_below<BN>(tl, at, se.lo);
+          const int b_sink = rows_below<BN>(tl, at, se.sink);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             keep[c] = live[m * 4 + c] & (bit_range(b_lo, b_hi, c * 32) | bit_range(0, b_sink, c * 32));
@@ -888,11 +799,7 @@ static int64_t tiles_bound(const Shape& sh) {
   const int64_t seqs = sh.rows < sh.seqs ? sh.rows : sh.seqs;
   return (sh.rows + seqs * (step - 1)) / step;
 }
-static int64_t key_tiles(const Shape& sh) {
-  const int rows = (sh.page_size + 7) & ~7;
-  const int64_t pages = (sh.keys + sh.page_size - 1) / sh.page_size;
-  return sh.page_size >= BN ? pages * ((sh.page_size + BN - 1) / BN) : (pages + BN / rows - 1) / (BN / rows);
-}
+static int64_t key_tiles(const Shape& sh) { return tiles_of_keys(sh, BN); }
 
 // Splits of the keys: the count that gives the least time for the slowest SM,
 // one key tile taking about 1.4 us, an item's start and end about two tiles,
@@ -928,14 +835,9 @@ static int start(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap
 
 int launch(const Keys& ky, const Queries& qr, const Shape& sh, void* workspace, cudaStream_t st) {
   const int G = qr.H / qr.group, ps = ky.page_size;
-  Tiling tl;
-  tl.ps = ps;
-  tl.tpp = (ps + BN - 1) / BN;
-  tl.rows = ps >= BN ? BN : (ps + 7) & ~7;
-  tl.ppt = ps >= BN ? 1 : BN / tl.rows;
+  Tiling tl = tiling_of(ps, BN);
   tl.tq = BM / qr.group;
   tl.splits = splits(sh);
-  const bool kv8 = ky.dtype != WF_DTYPE_BF16;
   CUtensorMap tq, tk, tv;
   int rc;
   {
@@ -948,16 +850,7 @@ int launch(const Keys& ky, const Queries& qr, const Shape& sh, void* workspace, 
                            CU_TENSOR_MAP_SWIZZLE_128B)) != WF_OK)
       return rc;
   }
-  const uint64_t dim[4] = {HD, (uint64_t)ps, (uint64_t)G, (uint64_t)ky.n_pages};
-  const uint32_t box[4] = {kv8 ? 128u : 64u, (uint32_t)tl.rows, 1, 1};
-  const uint64_t elem = kv8 ? 1 : 2;
-  for (int i = 0; i < 2; ++i) {
-    const int64_t* s = i ? ky.v_str : ky.k_str;
-    const uint64_t str[3] = {(uint64_t)s[2] * elem, (uint64_t)s[1] * elem, (uint64_t)s[0] * elem};
-    if ((rc = encode_tiled(i ? &tv : &tk, kv8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
-                           i ? ky.v : ky.k, dim, str, box, CU_TENSOR_MAP_SWIZZLE_128B)) != WF_OK)
-      return rc;
-  }
+  if ((rc = page_maps(&tk, &tv, ky, G, tl.rows)) != WF_OK) return rc;
   const int64_t items = tiles_bound(sh) * G * tl.splits;
   if (items > INT_MAX) return fail(WF_ERR_INVALID_ARG, "attention: too many query tiles (%lld)", (long long)items);
   // Few key tiles to an item: one CTA per SM walks the items, the next one's
