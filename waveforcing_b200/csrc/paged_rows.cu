@@ -52,6 +52,9 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool take) {  // zero when not taken
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(take ? 4 : 0) : "memory");
+}
 // Two codes (low halves' bytes 0 and 1) -> f16x2, exact.
 template <int DT>
 __device__ __forceinline__ uint32_t codes_f16(uint32_t two) {
@@ -94,16 +97,19 @@ __global__ void __launch_bounds__(THREADS, 2)
   const int rt0 = item % cut.row_tiles, hk = item / cut.row_tiles % G, b = item / cut.row_tiles / G;
   const Span sp = span_of(ky, qr, b);
   const Tiling& tl = cut.tl;
+  const int ps = tl.ps;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + ST * (STAGE + META));
   uint64_t* empty = full + ST;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + ST);
   if (threadIdx.x == 0) {
     for (int k = 0; k < ST; ++k) {
-      mbar_init(&full[k], 1);
+      mbar_init(&full[k], KV8 ? 33 : 1);
       mbar_init(&empty[k], WARPS);
     }
     *abort_flag = 0;
     fence_mbar_init();
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
   }
   __syncthreads();
   uint32_t done = 0;  // tiles through the ring
@@ -116,81 +122,74 @@ __global__ void __launch_bounds__(THREADS, 2)
     const int p0 = (int)((long long)rg.n * part / parts), p1 = (int)((long long)rg.n * (part + 1) / parts);
     if (warp == WARPS) {
       // ---------------------------------------------------------- producer
-      // Page ids (a lane to a page for the copies, four keys to a lane for the
-      // marks) are fetched a tile ahead, scales under the wait for the stage.
+      // A tile's page ids (a lane to a page) are fetched a tile ahead; scales go
+      // to shared memory by cp.async: no latency lies between the waits.
       constexpr int KL = BN / 32;
-      int box_id = -1, ids[KL];
-      auto spot = [&](const TileAt& a, int c, int& j, int& off) -> bool {  // key c * 32 + lane of a tile; seen at all?
+      const bool small = ps < BN;
+      int sub[KL];  // page of key c * 32 + lane among the tile's, and for small pages its row there
+      int at_row[KL];
+#pragma unroll
+      for (int c = 0; c < KL; ++c) {
         const int r = c * 32 + lane;
-        off = a.row + r;
-        j = a.page;
-        bool in = off < tl.ps;
-        if (tl.ps < BN) {
-          const int p = r / tl.rows;
-          off = r - p * tl.rows;
-          j += p;
-          in = off < tl.ps && p < tl.ppt;
-        }
-        const int pos = j * tl.ps + off;
-        return in && ((pos < rg.hi && pos >= rg.lo) || pos < rg.sink);
-      };
+        sub[c] = small ? min(r / tl.rows, tl.ppt) : 0;
+        at_row[c] = small && sub[c] < tl.ppt ? r - sub[c] * tl.rows : small ? ps : r;
+      }
+      TileAt nx_at;
+      int nx_box = -1;  // this lane's page of the next tile, as the table has it
       auto look = [&](int i) {
-        const TileAt a = tile_at<BN>(tl, nth_tile(rg, i));
-        box_id = lane < tl.ppt && needed(rg, tl, a.page + lane) ? page_id(ky, sp, b, a.page + lane) : -1;
-        int j, off;
-#pragma unroll
-        for (int c = 0; c < KL; ++c) ids[c] = spot(a, c, j, off) ? page_id(ky, sp, b, j) : INT_MIN;
+        if (i >= p1) return;
+        nx_at = tile_at<BN>(tl, nth_tile(rg, i));
+        nx_box = lane < tl.ppt && needed(rg, tl, nx_at.page + lane) ? page_id(ky, sp, b, nx_at.page + lane) : INT_MIN;
       };
-      if (p0 < p1) look(p0);
+      look(p0);
       for (int i = p0; i < p1; ++i, ++done) {
-        const TileAt a = tile_at<BN>(tl, nth_tile(rg, i));
-        const int box = box_id >= 0 && box_id < ky.n_pages ? box_id : -1;
-        bool in[KL];
-        float sk[KL], sv[KL];
-#pragma unroll
-        for (int c = 0; c < KL; ++c) {
-          int j, off;
-          spot(a, c, j, off);
-          in[c] = ids[c] >= 0 && ids[c] < ky.n_pages;
-          if (!in[c] && ids[c] != INT_MIN) status_raise(ST_PAGE_ID);
-          sk[c] = sv[c] = 0.f;
-          if constexpr (KV8) {
-            if (in[c]) {
-              sk[c] = __ldg(ky.ks + ids[c] * ky.ks_str[0] + hk * ky.ks_str[1] + off);
-              sv[c] = __ldg(ky.vs + ids[c] * ky.vs_str[0] + hk * ky.vs_str[1] + off);
-            }
-          } else if (ky.mask && in[c]) {
-            in[c] = __ldg(ky.mask + ids[c] * ky.mask_stride + off) != 0;
-          }
-        }
-        if (i + 1 < p1) look(i + 1);
+        const TileAt a = nx_at;
+        const bool bad = nx_box != INT_MIN && (nx_box < 0 || nx_box >= ky.n_pages);
+        if (bad) status_raise(ST_PAGE_ID);
+        const int box = bad || nx_box == INT_MIN ? -1 : nx_box;
+        look(i + 1);
         const uint32_t st = done % ST, turn = done / ST;
         if (turn > 0 && !warp_wait(&empty[st], turn - 1, abort_flag, ST_PAGED_ROWS)) break;
         uint8_t *at = smem + st * STAGE, *mt = smem + ST * STAGE + st * META;
         uint32_t all = 0xFFFFFFFFu;
 #pragma unroll
         for (int c = 0; c < KL; ++c) {
-          const uint32_t word = __ballot_sync(0xffffffffu, in[c]);
+          const int id = __shfl_sync(0xffffffffu, box, sub[c] & 31), off = a.row + at_row[c];
+          const int pos = a.base + (small ? sub[c] * ps : 0) + at_row[c];
+          bool in = id >= 0 && off < ps && sub[c] < tl.ppt && ((pos < rg.hi && pos >= rg.lo) || pos < rg.sink);
+          if (ky.mask && in) in = __ldg(ky.mask + id * ky.mask_stride + off) != 0;
+          if constexpr (KV8) {
+            const uint32_t to = smem_u32(mt) + (c * 32 + lane) * 4;
+            cp4(to, ky.ks + (in ? id * ky.ks_str[0] + hk * ky.ks_str[1] + off : 0), in);
+            cp4(to + MAX_BN * 4, ky.vs + (in ? id * ky.vs_str[0] + hk * ky.vs_str[1] + off : 0), in);
+          }
+          const uint32_t word = __ballot_sync(0xffffffffu, in);
           all &= word;
           if (lane == c) reinterpret_cast<uint32_t*>(mt + 2 * MAX_BN * 4)[c] = word;
-          if constexpr (KV8) {
-            reinterpret_cast<float*>(mt)[c * 32 + lane] = sk[c];
-            reinterpret_cast<float*>(mt)[MAX_BN + c * 32 + lane] = sv[c];
-          }
         }
+        if constexpr (KV8) asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(&full[st])) : "memory");
+        // BN live keys lie at consecutive positions, whatever the page size
         const bool whole = all == 0xFFFFFFFFu && a.base + BN <= rg.hi_min &&
                            (a.base >= rg.lo_max || a.base + BN <= rg.sink_min);
         if (lane == 4) *reinterpret_cast<uint2*>(mt + 2 * MAX_BN * 4 + 16) = make_uint2(whole, nth_tile(rg, i));
-        const uint32_t boxes = __ballot_sync(0xffffffffu, box >= 0), bytes = (uint32_t)tl.rows * 128;
-        if (lane == 0) mbar_arrive_expect_tx(&full[st], __popc(boxes) * bytes * (KV8 ? 2 : 4));
         __syncwarp();
-        if (box >= 0) {
-          uint8_t* k = at + lane * bytes;
-          uint8_t* v = k + STAGE / 2;
-          tma_load_4d(k, &tmK, &full[st], 0, a.row, hk, box);
-          if constexpr (!KV8) tma_load_4d(k + STAGE / 4, &tmK, &full[st], 64, a.row, hk, box);
-          tma_load_4d(v, &tmV, &full[st], 0, a.row, hk, box);
-          if constexpr (!KV8) tma_load_4d(v + STAGE / 4, &tmV, &full[st], 64, a.row, hk, box);
+        auto copy = [&](uint8_t* k, int id) {
+          tma_load_4d(k, &tmK, &full[st], 0, a.row, hk, id);
+          if constexpr (!KV8) tma_load_4d(k + STAGE / 4, &tmK, &full[st], 64, a.row, hk, id);
+          tma_load_4d(k + STAGE / 2, &tmV, &full[st], 0, a.row, hk, id);
+          if constexpr (!KV8) tma_load_4d(k + 3 * STAGE / 4, &tmV, &full[st], 64, a.row, hk, id);
+        };
+        if (!small) {  // one page: operands in uniform registers
+          const int id = __shfl_sync(0xffffffffu, box, 0);
+          if (elect_one()) {
+            mbar_arrive_expect_tx(&full[st], id >= 0 ? STAGE : 0);
+            if (id >= 0) copy(at, id);
+          }
+        } else {
+          const uint32_t boxes = __ballot_sync(0xffffffffu, box >= 0), bytes = (uint32_t)tl.rows * 128;
+          if (lane == 0) mbar_arrive_expect_tx(&full[st], __popc(boxes) * bytes * (KV8 ? 2 : 4));
+          __syncwarp();
+          if (box >= 0) copy(at + lane * bytes, box);
         }
         __syncwarp();
       }
