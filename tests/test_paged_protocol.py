@@ -1,7 +1,7 @@
 """Model check of the synchronisation of waveforcing_b200/csrc/paged_tile.cu (CPU).
 
-The kernel's roles (TMA producer, MMA issue, marks, two softmax warpgroups,
-code expansion) meet on mbarriers by parity.  The model transcribes every
+The kernel's roles (item finder, TMA producer, MMA issue, marks, two softmax
+warpgroups, code expansion) meet on mbarriers by parity.  The model transcribes every
 wait, arrival, load, MMA and commit with the kernel's phase formulas and runs
 the roles under random interleavings: copies land in any order, the tensor
 pipe runs in issue order.  Items have one or two sub-tiles and any number of
@@ -14,7 +14,7 @@ import pytest
 
 from tests.test_attn_protocol import Bar
 
-META = 3
+META, WORKS = 3, 4
 
 
 class Sim:
@@ -32,6 +32,9 @@ class Sim:
             for n in ("q_raw", "q_full", "q_empty", "s", "p0", "p1", "o_full"):
                 B[f"{n}{u}"] = Bar(1)
         self.b = B
+        for k in range(WORKS):
+            B[f"work_full{k}"], B[f"work_empty{k}"] = Bar(1), Bar(6 if kv8 else 5)
+        self.works = [None] * WORKS
         self.slot = [None] * self.NS     # what a ring slot holds: (kind, item, tile, state)
         self.users = [0] * self.NS       # MMAs issued that will read it
         self.q = [None, None]
@@ -45,9 +48,31 @@ class Sim:
         while not self.b[name].done(n & 1):
             yield
 
+    def finder(self):
+        for k, item in enumerate(list(enumerate(self.items)) + [None]):
+            if k >= WORKS and self.wrong != "works":
+                yield from self.wait(f"work_empty{k % WORKS}", k // WORKS - 1)
+            self.works[k % WORKS] = (k, item)
+            self.b[f"work_full{k % WORKS}"].arrive()
+            yield
+
+    def take(self, k, keep=False):
+        """The k-th item (None at the end); its place is freed at once unless kept."""
+        yield from self.wait(f"work_full{k % WORKS}", k // WORKS)
+        n, item = self.works[k % WORKS]
+        assert n == k, "item overwritten"
+        if item is not None and not keep:
+            self.b[f"work_empty{k % WORKS}"].arrive()
+        return item
+
     def producer(self):
-        n, qn = 0, [0, 0]
-        for i, (nsub, nt) in enumerate(self.items):
+        n, qn, work_n = 0, [0, 0], 0
+        while True:
+            item = yield from self.take(work_n)
+            work_n += 1
+            if item is None:
+                return
+            i, (nsub, nt) = item
             if nt == 0:
                 continue
             for u in range(nsub):
@@ -80,8 +105,13 @@ class Sim:
         self.pipe.append(("commit", f"s{u}"))
 
     def mma(self):
-        n, items, pn = 0, [0, 0], [0, 0]
-        for i, (nsub, nt) in enumerate(self.items):
+        n, items, pn, work_n = 0, [0, 0], [0, 0], 0
+        while True:
+            item = yield from self.take(work_n)
+            work_n += 1
+            if item is None:
+                return
+            i, (nsub, nt) = item
             if nt == 0:
                 continue
             yield from self.wait(f"full{n % self.NS}", n // self.NS)
@@ -130,8 +160,13 @@ class Sim:
         self.b[f"full{s}"].arrive()
 
     def mark(self):
-        n = tiles = 0
-        for i, (_, nt) in enumerate(self.items):
+        n = tiles = work_n = 0
+        while True:
+            item = yield from self.take(work_n)
+            work_n += 1
+            if item is None:
+                return
+            i, (nsub, nt) = item
             for j in range(nt):
                 s = n % self.NS
                 yield from self.wait(f"raw{s}", n // self.NS)
@@ -149,8 +184,13 @@ class Sim:
                 tiles += 1
 
     def expand(self):
-        n, tiles, qn = 0, 0, [0, 0]
-        for i, (nsub, nt) in enumerate(self.items):
+        n, tiles, qn, work_n = 0, 0, [0, 0], 0
+        while True:
+            item = yield from self.take(work_n)
+            work_n += 1
+            if item is None:
+                return
+            i, (nsub, nt) = item
             if nt == 0:
                 continue
             for u in range(nsub):
@@ -174,10 +214,16 @@ class Sim:
                 tiles += 1
 
     def softmax(self, u):
-        sn = items = tiles = 0
-        for i, (nsub, nt) in enumerate(self.items):
+        sn = items = tiles = work_n = 0
+        while True:
+            item = yield from self.take(work_n, keep=True)
+            if item is None:
+                return
+            i, (nsub, nt) = item
             if u >= nsub:
                 tiles += nt
+                self.b[f"work_empty{work_n % WORKS}"].arrive()
+                work_n += 1
                 continue
             for j in range(nt):
                 yield from self.wait(f"s{u}", sn)
@@ -202,6 +248,9 @@ class Sim:
                 for _ in range(2):
                     assert self.O[u] == (i, nt), (self.O[u], i, nt)
                     yield
+            assert self.works[work_n % WORKS][0] == work_n, "item overwritten while in use"
+            self.b[f"work_empty{work_n % WORKS}"].arrive()
+            work_n += 1
 
     def step_tma(self):
         kind, at, what, bar = self.tma.pop(self.rnd.randrange(len(self.tma)))
@@ -236,7 +285,7 @@ class Sim:
                     self.S[u] = ("P0 read", i, j)
 
     def run(self):
-        roles = [self.producer(), self.mma(), self.mark(), self.softmax(0), self.softmax(1)]
+        roles = [self.finder(), self.producer(), self.mma(), self.mark(), self.softmax(0), self.softmax(1)]
         if self.kv8:
             roles.append(self.expand())
         idle = 0
@@ -258,7 +307,7 @@ class Sim:
 
 
 def random_items(rnd):
-    return [(rnd.choice([1, 2, 2]), rnd.choice([0, 1, 1, 2, 3, 5])) for _ in range(rnd.randrange(1, 7))]
+    return [(rnd.choice([1, 2, 2]), rnd.choice([0, 1, 1, 2, 3, 5])) for _ in range(rnd.randrange(1, 12))]
 
 
 @pytest.mark.parametrize("kv8", [False, True])
@@ -267,7 +316,7 @@ def test_protocol(kv8):
         Sim(random_items(random.Random(seed)), kv8, seed).run()
 
 
-@pytest.mark.parametrize("wrong", ["p", "meta", "qpow"])
+@pytest.mark.parametrize("wrong", ["p", "meta", "qpow", "works"])
 def test_protocol_errors_are_caught(wrong):
     class Bad(Sim):
         pass
@@ -275,4 +324,4 @@ def test_protocol_errors_are_caught(wrong):
     Bad.wrong = wrong
     with pytest.raises(AssertionError):
         for seed in range(200):
-            Bad([(2, 4), (2, 1), (1, 1), (2, 1), (2, 3)], wrong == "qpow", seed).run()
+            Bad([(2, 4), (2, 1), (1, 1), (2, 1), (2, 3), (2, 2), (1, 1)], wrong == "qpow", seed).run()

@@ -73,10 +73,8 @@ int page_maps(CUtensorMap* k, CUtensorMap* v, const Keys& ky, int kv_heads, int 
 // each 16, where the tile kernel takes 128 rows at a time.
 static bool few_rows(const Shape& sh) { return sh.max_new * sh.group <= 16; }
 
-// Partial rows of split keys: f32 [splits][rows][H][128 + 1].
 static int64_t workspace_need(const Shape& sh) {
-  const int splits = few_rows(sh) ? rows::splits(sh) : tile::splits(sh);
-  return splits > 1 ? (int64_t)splits * sh.rows * sh.H * (HD + 1) * 4 : 0;
+  return (few_rows(sh) ? rows::parts(sh) : tile::parts(sh)) * (HD + 1) * 4;
 }
 
 int check_pages(const char* who, const wf_kv_pages* p);

@@ -104,11 +104,11 @@ __device__ __forceinline__ int page_id(const Keys& ky, const Span& s, int b, int
 // every `rows` tile rows (page_size rounded up to the swizzle's 8).
 struct Tiling {
   int ps, tpp, ppt, rows;  // page size; tiles per page (large pages); pages per tile (small); tile rows of a page
-  int tq, splits;          // tokens of a sub-tile and runs of keys (paged_tile.cu)
+  int tq, splits, even;    // paged_tile.cu: tokens of a sub-tile, runs of keys, whether tiles are dealt evenly
 };
 inline Tiling tiling_of(int ps, int bn) {
   const int rows = ps >= bn ? bn : (ps + 7) & ~7;
-  return Tiling{ps, (ps + bn - 1) / bn, ps >= bn ? 1 : bn / rows, rows, 0, 1};
+  return Tiling{ps, (ps + bn - 1) / bn, ps >= bn ? 1 : bn / rows, rows, 0, 1, 0};
 }
 template <int BN>
 __device__ __forceinline__ int tile_of(const Tiling& tl, int pos) {
@@ -219,14 +219,14 @@ inline int64_t tiles_of_keys(const Shape& sh, int bn) {
   return sh.page_size >= bn ? pages * tl.tpp : (pages + tl.ppt - 1) / tl.ppt;
 }
 
-// Many rows to a K/V head (paged_tile.cu); few (paged_rows.cu).  `splits`: runs
-// of keys whose partial rows the workspace holds for `join` (1: none).
+// Many rows to a K/V head (paged_tile.cu); few (paged_rows.cu).  `parts`: f32
+// rows of 128 + 1 that the workspace holds (0: none).
 namespace tile {
-int splits(const Shape& sh);
+int64_t parts(const Shape& sh);
 int launch(const Keys& ky, const Queries& qr, const Shape& sh, void* workspace, cudaStream_t st);
 }  // namespace tile
 namespace rows {
-int splits(const Shape& sh);
+int64_t parts(const Shape& sh);
 int launch(const Keys& ky, const Queries& qr, const Shape& sh, void* workspace, cudaStream_t st);
 }  // namespace rows
 // Tensor maps of the K and V pages, a box of `rows` rows of one page and head (64

@@ -537,7 +537,10 @@ static Cut cut_of(const Shape& sh, bool kv8) {
   return c;
 }
 
-int splits(const Shape& sh) { return cut_of(sh, sh.kv8).outer; }
+int64_t parts(const Shape& sh) {
+  const int outer = cut_of(sh, sh.kv8).outer;
+  return outer > 1 ? (int64_t)outer * sh.rows * sh.H : 0;
+}
 
 template <int DT>
 static int start(const CUtensorMap& tk, const CUtensorMap& tv, const Keys& ky, const Queries& qr, const Cut& cut, float* part_o, float* part_l, cudaStream_t st) {

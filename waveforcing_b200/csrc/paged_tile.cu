@@ -7,6 +7,7 @@
 //   warp 1       MMA issue: S_u = Q_u K_j^T (M=N=K=128), O_u += P_u V_j
 //   warp 2       marks the live keys of each tile, zeroes the V rows of the
 //                others (their P is 0, but 0 * NaN is not), fetches scales
+//   warp 3       finds the CTA's items ahead of the other roles
 //   warps 4-11   softmax; warpgroup u owns sub-tile u, a thread a row
 //   warps 12-15  (8-bit pages) expand codes to f16
 // TMEM columns: S_0 [0,128) S_1 [128,256) O_0 [256,384) O_1 [384,512); P_u
@@ -41,24 +42,26 @@ constexpr int SLOT = 2 * HALF;    // a K or V tile, or a Q sub-tile: [d 0-63][d 
 constexpr int META = 3;           // tiles whose marks (and scales) are kept
 constexpr uint32_t COL_S = 0, COL_O = 256;
 
-constexpr int WORK_BYTES = 96;
+constexpr int WORK_BYTES = 96, WORKS = 4;  // items found ahead
 template <bool KV8>
 struct Cfg {
   static constexpr int NS = KV8 ? 4 : 5;  // ring slots
   static constexpr int THREADS = KV8 ? 512 : 384;
-  static constexpr int NBARS = (3 * NS + 14 + META + 1 + 1) & ~1;  // even: what follows is 16-byte aligned
+  static constexpr int READERS = KV8 ? 15 : 11;  // warps that an item goes to
+  static constexpr int NBARS = (3 * NS + 14 + META + 2 * WORKS + 1 + 1) & ~1;  // even: what follows is 16-byte aligned
   static constexpr int META_BYTES = META * (16 + (KV8 ? 2 * BN * 4 : 0) + 16) + (KV8 ? 4 * BM * 4 : 0);
-  static constexpr int SMEM = 1024 + 2 * SLOT + NS * SLOT + NBARS * 8 + META_BYTES + 16 + 8 * WORK_BYTES;
+  static constexpr int SMEM = 1024 + 2 * SLOT + NS * SLOT + NBARS * 8 + META_BYTES + 16 + WORKS * WORK_BYTES;
   static_assert(SMEM <= 232448, "shared memory of one CTA");
 };
 
 struct Work : Range {
-  int b, hk, split;
-  int i0, nsub;  // first token, sub-tiles with rows
+  int b, hk, split;  // b < 0: no more items
+  int i0, nsub;      // first token, sub-tiles with rows
   Span sp;
-  int t0, t1;    // this item's share of the tile list
+  int t0, t1;        // this item's share of the tile list
+  int slot;          // its partial rows' place in the workspace, -1: none (see Deal)
 };
-static_assert(sizeof(Work) <= WORK_BYTES, "a softmax warp's item");
+static_assert(sizeof(Work) <= WORK_BYTES, "room for an item");
 
 // Query tiles of the launch over all sequences (one warp).
 __device__ __forceinline__ int count_tiles(const Keys& ky, const Queries& qr, const Tiling& tl, int lane) {
@@ -71,12 +74,15 @@ __device__ __forceinline__ int count_tiles(const Keys& ky, const Queries& qr, co
   return __reduce_add_sync(0xffffffffu, n);
 }
 
+// Run p of s of n tiles starts here.
+__device__ __forceinline__ int run_start(int n, int p, int s) { return n / s * p + n % s * p / s; }
+
 // Item `it` of the launch (one warp, same result in every lane).
 __device__ __forceinline__ bool find_work(Work& w, const Keys& ky, const Queries& qr, const Tiling& tl, int n_tiles,
-                                          int G, long long it, int lane) {
-  if (n_tiles == 0 || it >= (long long)n_tiles * G * tl.splits) return false;
-  int tile = (int)(it % n_tiles);
-  const int rest = (int)(it / n_tiles);
+                                          int G, unsigned it, int lane) {
+  if (n_tiles == 0 || it >= (unsigned)n_tiles * G * tl.splits) return false;
+  int tile = it % (unsigned)n_tiles;
+  const int rest = it / (unsigned)n_tiles;
   w.hk = rest % G;
   w.split = rest / G;
   int nq = 0;
@@ -114,11 +120,52 @@ __device__ __forceinline__ bool find_work(Work& w, const Keys& ky, const Queries
   const int i1 = min(w.i0 + 2 * tl.tq, w.sp.n) - 1;  // last token
   w.nsub = i1 >= w.i0 + tl.tq ? 2 : 1;
   static_cast<Range&>(w) = range_of<BN>(qr, w.sp, tl, w.i0, i1);
-  w.t0 = (int)((long long)w.n * w.split / tl.splits);
-  w.t1 = (int)((long long)w.n * (w.split + 1) / tl.splits);
+  w.t0 = 0;
+  w.t1 = w.n;
+  w.slot = -1;
+  if (tl.splits > 1) {  // at most 32 of them
+    w.t0 = run_start(w.n, w.split, tl.splits);
+    w.t1 = run_start(w.n, w.split + 1, tl.splits);
+  }
   return true;
 }
 
+// One sequence whose rows all see the same keys: its items take the same time,
+// n tiles each.  Whole rounds of them go to the CTAs in turn; the `left` others
+// are cut into `parts` runs of keys and those dealt in turn, run by run, so that
+// the CTAs of a moment share K and V through L2 (with one contiguous stretch of
+// tiles to a CTA instead, the loads of 12 heads came from HBM: 833 against 605
+// us).  4680 rows and 12 heads are 228 items: 148, then 80 in parts.
+struct Deal {
+  bool even;
+  int n, full, left, parts;  // tiles of an item; items dealt whole, the others, their parts
+};
+constexpr int MAX_SLOTS = 4 * SMS;  // parts that the workspace holds
+// The number of parts with the least estimated time, in hundredths of a tile's:
+// four tiles for a part's start and end, then the join's launch and traffic.
+__host__ __device__ inline int parts_of(int left, int n, int ctas) {
+  int best = 1;
+  long long least = 0;
+  for (int s = 1; s <= 32 && (s == 1 || (2 * s <= n && left * s <= MAX_SLOTS)); ++s) {
+    const long long cost = (left * s + ctas - 1) / ctas * ((n + s - 1) / s + 4) * 100ll + (s > 1 ? 200 + left * s : 0);
+    if (s == 1 || cost < least) least = cost, best = s;
+  }
+  return best;
+}
+__device__ __forceinline__ Deal deal_of(const Keys& ky, const Queries& qr, const Tiling& tl, int n_tiles, int G,
+                                        int ctas) {
+  Deal d{false, 0, 0, 0, 1};
+  if (!tl.even || n_tiles == 0) return d;
+  const Span sp = span_of(ky, qr, 0);
+  const Sees a = sees(qr, sp, 0), z = sees(qr, sp, sp.n - 1);
+  if (sp.pos0 < 0 || a.hi != z.hi || a.lo != z.lo || a.hi == 0) return d;
+  d.even = true;
+  d.n = range_of<BN>(qr, sp, tl, 0, sp.n - 1).n;
+  d.full = n_tiles * G / ctas * ctas;
+  d.left = n_tiles * G - d.full;
+  if (d.left > 0) d.parts = parts_of(d.left, d.n, ctas);
+  return d;
+}
 __device__ __forceinline__ bool drain(uint64_t* bar, uint32_t parity, uint64_t ns) {
   const uint64_t t0 = globaltimer_ns();
   while (!mbar_try_wait(bar, parity & 1))
@@ -240,6 +287,8 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
   uint64_t* bar_fin = o_full + 2;
   uint64_t* q_raw = bar_fin + 1;     // [2] 8-bit pages: Q_u landed (q_full: as f16)
   uint64_t* marked = q_raw + 2;      // [META] 8-bit pages: a tile's scales are there
+  uint64_t* work_full = marked + META;     // [WORKS] an item is there
+  uint64_t* work_empty = work_full + WORKS;
   uint32_t* live = reinterpret_cast<uint32_t*>(raw + Cfg<KV8>::NBARS);  // [META][4] live keys of a tile
   int* whole = reinterpret_cast<int*>(live + META * 4);                 // [META] every row sees all of it
   float* kpow = reinterpret_cast<float*>(whole + META);                 // [META] power of two of the K tile
@@ -248,6 +297,7 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
   float* qpow = reinterpret_cast<float*>(scales + META * 2 * BN);       // [2][2][BM], by turns of the sub-tile's items
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(live) + Cfg<KV8>::META_BYTES);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  Work* works = reinterpret_cast<Work*>(reinterpret_cast<uint8_t*>(tmem_slot) + 16);  // [WORKS]
 
   // Values that steer the roles are broadcast from lane 0, by which the compiler
   // knows them to be the same in a warp: the MMA warp's operands then stay in
@@ -271,6 +321,10 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
       mbar_init(&o_full[u], 1);
     }
     for (int m = 0; m < META; ++m) mbar_init(&marked[m], 1);
+    for (int k = 0; k < WORKS; ++k) {
+      mbar_init(&work_full[k], 1);
+      mbar_init(&work_empty[k], Cfg<KV8>::READERS);
+    }
     mbar_init(bar_fin, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -283,7 +337,25 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tbase = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-  const int n_tiles = count_tiles(ky, qr, tl, lane);
+  // Items, as warp 3 found them: `take` copies the next one and frees its place;
+  // `next_work` leaves it there until `done_with`.
+  uint32_t work_n = 0;
+  auto next_work = [&]() -> bool {
+    const uint32_t k = work_n % WORKS;
+    if (!warp_wait(&work_full[k], work_n / WORKS, abort_flag, ST_PAGED_WORK)) return false;
+    ++work_n;
+    return works[k].b >= 0;
+  };
+  auto done_with = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&work_empty[(work_n - 1) % WORKS]);
+  };
+  auto take = [&](Work& w) -> bool {
+    if (!next_work()) return false;
+    w = works[(work_n - 1) % WORKS];
+    done_with();
+    return true;
+  };
 
   auto teardown = [&]() {
     tc_fence_before();
@@ -332,7 +404,7 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
         ++slot_n;
         return true;
       };
-      for (long long it = blockIdx.x; ok && find_work(w, ky, qr, tl, n_tiles, G, it, lane); it += gridDim.x) {
+      for (; ok && take(w); ) {
         if (w.t1 <= w.t0) continue;
         for (int u = 0; ok && u < w.nsub; ++u) {
           if (qn[u] > 0 && !(ok = warp_wait(&q_empty[u], qn[u] - 1, abort_flag, ST_PAGED_PRODUCER))) break;
@@ -395,7 +467,7 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
         }
         __syncwarp();
       };
-      for (long long it = blockIdx.x; ok && find_work(w, ky, qr, tl, n_tiles, G, it, lane); it += gridDim.x) {
+      for (; ok && take(w); ) {
         const int nt = __shfl_sync(0xffffffffu, w.t1 - w.t0, 0);
         if (nt <= 0) continue;
         const int nsub = __shfl_sync(0xffffffffu, w.nsub, 0), last_u = nsub - 1;
@@ -473,7 +545,7 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
 #pragma unroll
         for (int c = 0; c < 4; ++c) ids[c] = spot(a, c, j, off) ? page_id(ky, w.sp, w.b, j) : INT_MIN;
       };
-      for (long long it = blockIdx.x; ok && find_work(w, ky, qr, tl, n_tiles, G, it, lane); it += gridDim.x) {
+      for (; ok && take(w); ) {
         float v_top = 0.f;  // power of two of V so far
         if (w.t0 < w.t1) fetch_ids(w.t0);
         for (int i = w.t0; ok && i < w.t1; ++i, ++tiles) {
@@ -560,6 +632,36 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
         }
       }
     }
+    if (warp == 3) {
+      // --------------------------------------------------------------- items
+      const int n_tiles = count_tiles(ky, qr, tl, lane), ctas = gridDim.x, c = blockIdx.x;
+      const Deal d = deal_of(ky, qr, tl, n_tiles, G, ctas);
+      bool ok = true;
+      auto give = [&]() {
+        const uint32_t k = work_n % WORKS;
+        ok = ok && (work_n < WORKS || warp_wait(&work_empty[k], work_n / WORKS - 1, abort_flag, ST_PAGED_WORK));
+        if (ok && lane == 0) {
+          works[k] = w;
+          mbar_arrive(&work_full[k]);
+        }
+        __syncwarp();
+        ++work_n;
+      };
+      const unsigned whole = d.even ? d.full : 0xFFFFFFFFu;
+      for (unsigned it = c; ok && it < whole && find_work(w, ky, qr, tl, n_tiles, G, it, lane); it += ctas) give();
+      for (int v = c; ok && d.even && v < d.left * d.parts; v += ctas) {
+        const int p = v / d.left, r = v - p * d.left;
+        find_work(w, ky, qr, tl, n_tiles, G, d.full + r, lane);
+        if (d.parts > 1) {
+          w.t0 = run_start(d.n, p, d.parts);
+          w.t1 = run_start(d.n, p + 1, d.parts);
+          w.slot = v;
+        }
+        give();
+      }
+      w.b = -1;
+      give();
+    }
     __syncwarp();
     teardown();
   } else if (warp < 12) {
@@ -574,19 +676,13 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
     const uint32_t tS = tbase + lane_off + COL_S + u * BN, tO = tbase + lane_off + COL_O + u * HD;
     uint32_t sn = 0, items = 0, tiles = 0;  // S_u consumed, items with keys, tiles of the CTA
     bool ok = true;
-    // The item lies in shared memory: the loop over its tiles has no registers to spare.
-    Work& w = *reinterpret_cast<Work*>(reinterpret_cast<uint8_t*>(tmem_slot) + 16 + (warp - 4) * WORK_BYTES);
-    for (long long it = blockIdx.x; ok; it += gridDim.x) {
-      {
-        Work next;
-        if (!find_work(next, ky, qr, tl, n_tiles, G, it, lane)) break;
-        __syncwarp();
-        if (lane == 0) w = next;
-        __syncwarp();
-      }
+    // The item stays in shared memory: the loop over its tiles has no registers to spare.
+    for (;; done_with()) {
+      if (!ok || !next_work()) break;
+      const Work& w = works[(work_n - 1) % WORKS];
       const int nt = w.t1 - w.t0;
       if (u >= w.nsub) {
-        tiles += max(nt, 0);
+        tiles += nt;
         continue;
       }
       const int i = w.i0 + u * tl.tq + row / qr.group, h = w.hk * qr.group + row % qr.group;
@@ -717,8 +813,9 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
       const float inv = none ? 0.f : m_run != m_run ? m_run : v_run / l_run;
       const int64_t packed = (int64_t)(w.sp.first + i) * qr.H + h;
       const float lse2 = none ? -INFINITY : m_run + log2f(l_run);
-      if (tl.splits > 1) {
-        const int64_t at = (int64_t)w.split * qr.rows * qr.H + packed;
+      if (tl.splits > 1 || w.slot >= 0) {
+        const int64_t at = w.slot >= 0 ? (int64_t)w.slot * (2 * BM) + u * BM + row
+                                       : (int64_t)w.split * qr.rows * qr.H + packed;
         if (has_row) part_l[at] = lse2;
         if (nt > 0) {
 #pragma unroll
@@ -765,7 +862,7 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
       Work w;
       uint32_t qn[2] = {0, 0}, tiles = 0;
       const int row0 = (warp - 12) * 32;
-      for (long long it = blockIdx.x; ok && find_work(w, ky, qr, tl, n_tiles, G, it, lane); it += gridDim.x) {
+      for (; ok && take(w); ) {
         if (w.t1 <= w.t0) continue;
         for (int u = 0; ok && u < w.nsub; ++u) {
           if (!(ok = warp_wait(&q_raw[u], qn[u], abort_flag, ST_PAGED_EXPAND))) break;
@@ -791,6 +888,45 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
   }
 }
 
+// Joins the parts of items that were dealt out in parts: blocks (item, run
+// of rows), a warp to a row at a time.
+__global__ void __launch_bounds__(256) join_dealt_kernel(const __grid_constant__ Keys ky,
+                                                         const __grid_constant__ Queries qr,
+                                                         const __grid_constant__ Tiling tl,
+                                                         const float* __restrict__ part_o,
+                                                         const float* __restrict__ part_l, int ctas) {
+  const int lane = threadIdx.x & 31;
+  const int G = qr.H / qr.group, n_tiles = count_tiles(ky, qr, tl, lane);
+  const Deal d = deal_of(ky, qr, tl, n_tiles, G, ctas);
+  for (int r = blockIdx.x; d.even && d.parts > 1 && r < d.left; r += gridDim.x) {
+    Work w;
+    find_work(w, ky, qr, tl, n_tiles, G, d.full + r, lane);
+    for (int row = blockIdx.y * 8 + (threadIdx.x >> 5); row < 2 * BM; row += gridDim.y * 8) {
+      const int u = row / BM, rr = row % BM, i = w.i0 + u * tl.tq + rr / qr.group, h = w.hk * qr.group + rr % qr.group;
+      if (rr >= tl.tq * qr.group || i >= w.sp.n) continue;
+      float m = -INFINITY;
+      for (int p = 0; p < d.parts; ++p) m = max_nan(m, part_l[(int64_t)(p * d.left + r) * (2 * BM) + row]);
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      float l = 0.f;
+      for (int p = 0; p < d.parts && m != -INFINITY; ++p) {
+        const int64_t at = (int64_t)(p * d.left + r) * (2 * BM) + row;
+        const float ls = part_l[at];
+        if (ls == -INFINITY) continue;
+        const float x = exp2f(ls - m);
+        const float4 v = __ldcs(reinterpret_cast<const float4*>(part_o + at * HD) + lane);
+        o.x += x * v.x, o.y += x * v.y, o.z += x * v.z, o.w += x * v.w;
+        l += x;
+      }
+      const float inv = m == -INFINITY ? 0.f : 1.f / l;
+      const int64_t packed = (int64_t)(w.sp.first + i) * qr.H + h;
+      const int64_t orow = ky.cross ? w.b * qr.o_str[0] + i * qr.o_str[1] : (int64_t)(w.sp.first + i) * qr.o_str[1];
+      *reinterpret_cast<uint2*>(qr.o + orow + h * qr.o_str[2] + lane * 4) =
+          make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+      if (qr.lse && lane == 0) qr.lse[packed] = m == -INFINITY ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+    }
+  }
+}
+
 // --------------------------------------------------------------------- host
 // What the host knows of a call's size.
 static int64_t tiles_bound(const Shape& sh) {
@@ -801,10 +937,16 @@ static int64_t tiles_bound(const Shape& sh) {
 }
 static int64_t key_tiles(const Shape& sh) { return tiles_of_keys(sh, BN); }
 
-// Splits of the keys: the count that gives the least time for the slowest SM,
-// one key tile taking about 1.4 us, an item's start and end about two tiles,
-// and the join its launch and one f32 row written and read a split.
-int splits(const Shape& sh) {
+// Whether the launch is one sequence on a CTA per SM, dealt out as Deal says
+// (should its rows see different keys after all, whole items in turn); worth it
+// where the key tiles are many beside a part's start, end and join.
+static bool dealt(const Shape& sh) { return sh.seqs == 1 && key_tiles(sh) >= 16; }
+
+// Splits of the keys otherwise: the count that gives the least time for the
+// slowest SM, one key tile taking about 1.4 us, an item's start and end about
+// two tiles, and the join its launch and one f32 row written and read a split.
+static int splits(const Shape& sh) {
+  if (dealt(sh)) return 1;
   const int64_t items = tiles_bound(sh) * (sh.H / sh.group), nt = key_tiles(sh);
   int best = 1;
   double best_us = 1e30;
@@ -815,6 +957,14 @@ int splits(const Shape& sh) {
     if (us < best_us * 0.98) best_us = us, best = s;
   }
   return best;
+}
+int64_t parts(const Shape& sh) {
+  if (dealt(sh)) {  // rows that turn out fewer leave other items
+    const int64_t items = tiles_bound(sh) * (sh.H / sh.group);
+    return (items < SMS ? (items * 32 < MAX_SLOTS ? items * 32 : MAX_SLOTS) : MAX_SLOTS) * 2 * BM;
+  }
+  const int s = splits(sh);
+  return s > 1 ? (int64_t)s * sh.rows * sh.H : 0;
 }
 
 template <int DT>
@@ -838,6 +988,7 @@ int launch(const Keys& ky, const Queries& qr, const Shape& sh, void* workspace, 
   Tiling tl = tiling_of(ps, BN);
   tl.tq = BM / qr.group;
   tl.splits = splits(sh);
+  tl.even = dealt(sh);
   CUtensorMap tq, tk, tv;
   int rc;
   {
@@ -852,20 +1003,24 @@ int launch(const Keys& ky, const Queries& qr, const Shape& sh, void* workspace, 
   }
   if ((rc = page_maps(&tk, &tv, ky, G, tl.rows)) != WF_OK) return rc;
   const int64_t items = tiles_bound(sh) * G * tl.splits;
-  if (items > INT_MAX) return fail(WF_ERR_INVALID_ARG, "attention: too many query tiles (%lld)", (long long)items);
+  if (items > INT_MAX / 4) return fail(WF_ERR_INVALID_ARG, "attention: too many query tiles (%lld)", (long long)items);
   // Few key tiles to an item: one CTA per SM walks the items, the next one's
   // loads under the last one's end.  Many: a CTA per item, so that the SM that
   // is done first takes the next.
-  const unsigned grid = (unsigned)(key_tiles(sh) / tl.splits < 8 && items > SMS ? SMS : items);
-  float *part_o = nullptr, *part_l = nullptr;
-  if (tl.splits > 1) {
-    part_o = static_cast<float*>(workspace);
-    part_l = part_o + (int64_t)tl.splits * qr.rows * qr.H * HD;
-  }
+  const unsigned grid = (unsigned)(tl.even || (key_tiles(sh) / tl.splits < 8 && items > SMS) ? SMS : items);
+  const int64_t n_parts = parts(sh);
+  float* part_o = static_cast<float*>(workspace);
+  float* part_l = part_o + n_parts * HD;
   rc = ky.dtype == WF_DTYPE_BF16   ? start<WF_DTYPE_BF16>(tq, tk, tv, ky, qr, tl, grid, part_o, part_l, st)
        : ky.dtype == WF_DTYPE_E4M3 ? start<WF_DTYPE_E4M3>(tq, tk, tv, ky, qr, tl, grid, part_o, part_l, st)
                                    : start<WF_DTYPE_S8>(tq, tk, tv, ky, qr, tl, grid, part_o, part_l, st);
-  if (rc != WF_OK || tl.splits == 1) return rc;
+  if (rc != WF_OK || n_parts == 0) return rc;
+  if (tl.even) {
+    const int64_t left = items % SMS;  // with rows behind the sequence the device may have others
+    join_dealt_kernel<<<dim3((unsigned)(left ? left : 1), 8), 256, 0, st>>>(ky, qr, tl, part_o, part_l, SMS);
+    WFK_CUDA_TRY(cudaGetLastError());
+    return WF_OK;
+  }
   return join(ky, qr, part_o, part_l, tl.splits, st);
 }
 

@@ -23,6 +23,7 @@ enum StatusCode : uint32_t {
   ST_PAGED_SOFTMAX = 1u << 13,
   ST_PAGED_EXPAND = 1u << 14,
   ST_PAGED_ROWS = 1u << 15,
+  ST_PAGED_WORK = 1u << 16,
   ST_PAGE_ID = 1u << 9,  // a page id outside the pool, or a length past the page table
 };
 
