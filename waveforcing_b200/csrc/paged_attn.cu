@@ -53,17 +53,24 @@ int join(const Keys& ky, const Queries& qr, const float* part_o, const float* pa
   return WF_OK;
 }
 
-int page_maps(CUtensorMap* k, CUtensorMap* v, const Keys& ky, int kv_heads, int rows) {
+int page_maps(PageMaps* m, const Keys& ky, int kv_heads, const Tiling& tl, int bn) {
   const bool kv8 = ky.dtype != WF_DTYPE_BF16;
   const uint64_t dim[4] = {HD, (uint64_t)ky.page_size, (uint64_t)kv_heads, (uint64_t)ky.n_pages};
-  const uint32_t box[4] = {kv8 ? 128u : 64u, (uint32_t)rows, 1, 1};
   const uint64_t elem = kv8 ? 1 : 2;
   for (int i = 0; i < 2; ++i) {
     const int64_t* s = i ? ky.v_str : ky.k_str;
     const uint64_t str[3] = {(uint64_t)s[2] * elem, (uint64_t)s[1] * elem, (uint64_t)s[0] * elem};
-    const int rc = encode_tiled(i ? v : k, kv8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
-                                i ? ky.v : ky.k, dim, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (rc != WF_OK) return rc;
+    for (int rows : {bn, tl.rows}) {
+      CUtensorMap* to = rows == bn ? (i ? &m->v_tile : &m->k_tile) : (i ? &m->v : &m->k);
+      const uint32_t box[4] = {kv8 ? 128u : 64u, (uint32_t)rows, 1, 1};
+      const int rc = encode_tiled(to, kv8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                                  i ? ky.v : ky.k, dim, str, box, CU_TENSOR_MAP_SWIZZLE_128B);
+      if (rc != WF_OK) return rc;
+      if (tl.rows == bn) {
+        (i ? m->v : m->k) = *to;
+        break;
+      }
+    }
   }
   return WF_OK;
 }

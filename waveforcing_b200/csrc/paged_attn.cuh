@@ -99,30 +99,47 @@ __device__ __forceinline__ int page_id(const Keys& ky, const Span& s, int b, int
   return ky.cross ? s.state : __ldg(ky.table + b * ky.table_stride + j);
 }
 
-// How the keys of a sequence fall into tiles of BN: pages of at least BN rows
-// give ceil(page_size / BN) tiles each, smaller ones share a tile, a page on
-// every `rows` tile rows (page_size rounded up to the swizzle's 8).
+// How the keys of a sequence fall into tiles of BN rows, and those into boxes (one
+// TMA copy each, a multiple of the swizzle's 8 rows, in one page).  Page sizes
+// that are multiples of 8 give dense tiles of BN consecutive positions, in boxes
+// of the largest power of two that divides the page size (one box where the
+// whole tile lies in a page).  Others leave holes: pages of at least BN rows
+// give ceil(page_size / BN) tiles each, smaller ones share a tile, a page to a
+// box.
 struct Tiling {
-  int ps, tpp, ppt, rows;  // page size; tiles per page (large pages); pages per tile (small); tile rows of a page
-  int tq, splits, even;    // paged_tile.cu: tokens of a sub-tile, runs of keys, whether tiles are dealt evenly
+  int ps, dense, tpp, boxes, rows;  // page size; tiles per page (large, not dense); boxes of a tile, their rows
+  int tq, splits, even, bulk;       // paged_tile.cu: tokens of a sub-tile, runs of keys, whether items are dealt
+                                    // evenly, whether scales can be fetched by bulk copies
 };
 inline Tiling tiling_of(int ps, int bn) {
-  const int rows = ps >= bn ? bn : (ps + 7) & ~7;
-  return Tiling{ps, (ps + bn - 1) / bn, ps >= bn ? 1 : bn / rows, rows, 0, 1, 0};
+  Tiling t{ps, ps % 8 == 0, (ps + bn - 1) / bn, 1, bn, 0, 1, 0, 0};
+  if (t.dense)
+    while (ps % t.rows) t.rows /= 2;
+  else if (ps < bn)
+    t.rows = (ps + 7) & ~7;
+  t.boxes = bn / t.rows;
+  return t;
 }
 template <int BN>
 __device__ __forceinline__ int tile_of(const Tiling& tl, int pos) {
+  if (tl.dense) return pos / BN;
   const int j = pos / tl.ps;
-  return tl.ps < BN ? j / tl.ppt : j * tl.tpp + (pos - j * tl.ps) / BN;
+  return tl.ps < BN ? j / tl.boxes : j * tl.tpp + (pos - j * tl.ps) / BN;
 }
 struct TileAt {
-  int page, row, base;  // first page, row in it, position of the tile's first key
+  int page, row, base;  // page and row of the tile's first key, its position
 };
 template <int BN>
 __device__ __forceinline__ TileAt tile_at(const Tiling& tl, int t) {
   TileAt a;
+  if (tl.dense) {
+    a.base = t * BN;
+    a.page = a.base / tl.ps;
+    a.row = a.base - a.page * tl.ps;
+    return a;
+  }
   if (tl.ps < BN) {
-    a.page = t * tl.ppt;
+    a.page = t * tl.boxes;
     a.row = 0;
   } else {
     a.page = t / tl.tpp;
@@ -136,9 +153,48 @@ template <int BN>
 __device__ __forceinline__ int rows_below(const Tiling& tl, const TileAt& a, int x) {
   const int d = x - a.base;
   if (d <= 0) return 0;
+  if (tl.dense) return min(d, BN);
   if (tl.ps >= BN) return min(d, min(BN, tl.ps - a.row));
   const int j = d / tl.ps;
-  return min(j, tl.ppt) * tl.rows + (j < tl.ppt ? d - j * tl.ps : 0);
+  return min(j, tl.boxes) * tl.rows + (j < tl.boxes ? d - j * tl.ps : 0);
+}
+// The tile after a (of consecutive tiles).
+template <int BN>
+__device__ __forceinline__ void next_tile(const Tiling& tl, TileAt& a) {
+  a.base += BN;
+  a.row += BN;
+  if (tl.dense) {
+    while (a.row >= tl.ps) a.row -= tl.ps, ++a.page;
+  } else if (tl.ps < BN) {
+    a.page += tl.boxes;
+    a.row = 0;
+    a.base = a.page * tl.ps;
+  } else if (a.row >= tl.ps) {
+    a.row = 0;
+    ++a.page;
+    a.base = a.page * tl.ps;
+  }
+}
+// Whether the tile lies in one page and one copy of BN rows fetches it.
+template <int BN>
+__device__ __forceinline__ bool one_box(const Tiling& tl, const TileAt& a) {
+  return tl.boxes == 1 || (tl.dense && a.row + BN <= tl.ps);
+}
+struct Box {
+  int page, row, pos;  // page (of the sequence), row in it, position of the box's first key
+};
+template <int BN>
+__device__ __forceinline__ Box box_at(const Tiling& tl, const TileAt& a, int i) {
+  Box x{a.page, a.row, a.base};
+  if (tl.dense) {
+    x.pos += i * tl.rows;
+    x.page = x.pos / tl.ps;
+    x.row = x.pos - x.page * tl.ps;
+  } else if (tl.ps < BN) {
+    x.page += i;
+    x.pos += i * tl.ps;
+  }
+  return x;
 }
 // Bits [a, b) of a 32-bit word that starts at bit `at`.
 __device__ __forceinline__ uint32_t bit_range(int a, int b, int at) {
@@ -174,11 +230,32 @@ __device__ __forceinline__ Range range_of(const Queries& qr, const Span& sp, con
   return r;
 }
 __device__ __forceinline__ int nth_tile(const Range& r, int i) { return i < r.n_sink ? i : i - r.n_sink + r.t_lo; }
-// Whether some token sees a key of its sequence's page j.
-__device__ __forceinline__ bool needed(const Range& r, const Tiling& tl, int j) {
-  const long long p0 = (long long)j * tl.ps;
-  return (p0 < r.hi && p0 + tl.ps > r.lo) || p0 < r.sink;
+// Whether some token sees a key of [pos, pos + rows).
+__device__ __forceinline__ bool needed(const Range& r, int pos, int rows) {
+  return (pos < r.hi && pos + rows > r.lo) || pos < r.sink;
 }
+// Walks the tiles of a list from its i-th on.
+template <int BN>
+struct Walk {
+  const Range& r;
+  const Tiling& tl;
+  int i;
+  TileAt a;
+  __device__ __forceinline__ Walk(const Range& r, const Tiling& tl, int i)
+      : r(r), tl(tl), i(i), a(tile_at<BN>(tl, nth_tile(r, i))) {}
+  __device__ __forceinline__ void next() {
+    if (++i == r.n_sink)
+      a = tile_at<BN>(tl, r.t_lo);
+    else
+      next_tile<BN>(tl, a);
+  }
+};
+// Whether every key of a one-box tile is seen by some token.
+template <int BN>
+__device__ __forceinline__ bool inside(const Range& r, const TileAt& a) {
+  return (a.base >= r.lo && a.base + BN <= r.hi) || a.base + BN <= r.sink;
+}
+__device__ __forceinline__ bool seen(const Range& r, int pos) { return (pos < r.hi && pos >= r.lo) || pos < r.sink; }
 
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, uint32_t code) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity & 1, abort, code));
@@ -198,6 +275,15 @@ __device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool take) {  // zero when not taken
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(take ? 4 : 0) : "memory");
+}
+// Untiled bulk copy (16-byte aligned, a multiple of 16 bytes) counted on `bar`.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
 // Power of two at or above x (> 0), between 2^-122 and 2^122 (a row scale is below 2^122).
 __device__ __forceinline__ float pow2_above(float x) {
   const uint32_t e = ((__float_as_uint(x) + 0x7FFFFFu) >> 23) << 23;
@@ -215,8 +301,9 @@ struct Shape {
 constexpr int SMS = 148;  // B200
 inline int64_t tiles_of_keys(const Shape& sh, int bn) {
   const Tiling tl = tiling_of(sh.page_size, bn);
+  if (tl.dense) return (sh.keys + bn - 1) / bn;
   const int64_t pages = (sh.keys + sh.page_size - 1) / sh.page_size;
-  return sh.page_size >= bn ? pages * tl.tpp : (pages + tl.ppt - 1) / tl.ppt;
+  return sh.page_size >= bn ? pages * tl.tpp : (pages + tl.boxes - 1) / tl.boxes;
 }
 
 // Many rows to a K/V head (paged_tile.cu); few (paged_rows.cu).  `parts`: f32
@@ -229,9 +316,12 @@ namespace rows {
 int64_t parts(const Shape& sh);
 int launch(const Keys& ky, const Queries& qr, const Shape& sh, void* workspace, cudaStream_t st);
 }  // namespace rows
-// Tensor maps of the K and V pages, a box of `rows` rows of one page and head (64
-// bf16 or 128 codes wide, 128-byte swizzle).
-int page_maps(CUtensorMap* k, CUtensorMap* v, const Keys& ky, int kv_heads, int rows);
+// Tensor maps of the K and V pages: boxes of the tiling's rows of one page and
+// head, and of whole tiles (64 bf16 or 128 codes wide, 128-byte swizzle).
+struct PageMaps {
+  CUtensorMap k, v, k_tile, v_tile;
+};
+int page_maps(PageMaps* m, const Keys& ky, int kv_heads, const Tiling& tl, int bn);
 int join(const Keys& ky, const Queries& qr, const float* part_o, const float* part_l, int splits, cudaStream_t st);
 
 }  // namespace paged

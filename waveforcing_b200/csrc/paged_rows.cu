@@ -52,9 +52,6 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool take) {  // zero when not taken
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(take ? 4 : 0) : "memory");
-}
 // Two codes (low halves' bytes 0 and 1) -> f16x2, exact.
 template <int DT>
 __device__ __forceinline__ uint32_t codes_f16(uint32_t two) {
@@ -80,7 +77,7 @@ struct Cut {
 
 template <int DT>
 __global__ void __launch_bounds__(THREADS, 2)
-    rows_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+    rows_kernel(const __grid_constant__ PageMaps tm,
                 const __grid_constant__ Keys ky, const __grid_constant__ Queries qr, const __grid_constant__ Cut cut,
                 float* part_o, float* part_l) {
   constexpr bool KV8 = DT != WF_DTYPE_BF16;
@@ -108,8 +105,8 @@ __global__ void __launch_bounds__(THREADS, 2)
     }
     *abort_flag = 0;
     fence_mbar_init();
-    tma_prefetch_desc(&tmK);
-    tma_prefetch_desc(&tmV);
+    tma_prefetch_desc(&tm.k_tile);
+    tma_prefetch_desc(&tm.v_tile);
   }
   __syncthreads();
   uint32_t done = 0;  // tiles through the ring
@@ -122,74 +119,90 @@ __global__ void __launch_bounds__(THREADS, 2)
     const int p0 = (int)((long long)rg.n * part / parts), p1 = (int)((long long)rg.n * (part + 1) / parts);
     if (warp == WARPS) {
       // ---------------------------------------------------------- producer
-      // A tile's page ids (a lane to a page) are fetched a tile ahead; scales go
+      // A tile's page ids (a lane to a box) are fetched a tile ahead; scales go
       // to shared memory by cp.async: no latency lies between the waits.
       constexpr int KL = BN / 32;
-      const bool small = ps < BN;
-      int sub[KL];  // page of key c * 32 + lane among the tile's, and for small pages its row there
-      int at_row[KL];
+      int sub[KL], at_row[KL];  // of key c * 32 + lane: its box, and the row in it
 #pragma unroll
       for (int c = 0; c < KL; ++c) {
         const int r = c * 32 + lane;
-        sub[c] = small ? min(r / tl.rows, tl.ppt) : 0;
-        at_row[c] = small && sub[c] < tl.ppt ? r - sub[c] * tl.rows : small ? ps : r;
+        sub[c] = min(r / tl.rows, tl.boxes);  // behind the last box: a hole
+        at_row[c] = r - sub[c] * tl.rows;
       }
-      TileAt nx_at;
-      int nx_box = -1;  // this lane's page of the next tile, as the table has it
-      auto look = [&](int i) {
-        if (i >= p1) return;
-        nx_at = tile_at<BN>(tl, nth_tile(rg, i));
-        nx_box = lane < tl.ppt && needed(rg, tl, nx_at.page + lane) ? page_id(ky, sp, b, nx_at.page + lane) : INT_MIN;
+      Box nx{};             // the next tile, or this lane's box of it
+      int nx_id = INT_MIN;  // and its page, as the table has it (INT_MIN: not needed)
+      auto look = [&](const TileAt& a) {
+        const bool one = one_box<BN>(tl, a);
+        nx = one ? Box{a.page, a.row, a.base} : box_at<BN>(tl, a, lane);
+        nx_id = one || (lane < tl.boxes && needed(rg, nx.pos, min(tl.rows, ps - nx.row))) ? page_id(ky, sp, b, nx.page)
+                                                                                          : INT_MIN;
       };
-      look(p0);
+      Walk<BN> walk(rg, tl, min(p0, max(p1 - 1, 0)));
+      if (p0 < p1) look(walk.a);
       for (int i = p0; i < p1; ++i, ++done) {
-        const TileAt a = nx_at;
-        const bool bad = nx_box != INT_MIN && (nx_box < 0 || nx_box >= ky.n_pages);
+        const TileAt a = walk.a;
+        const bool bad = nx_id != INT_MIN && (nx_id < 0 || nx_id >= ky.n_pages), one = one_box<BN>(tl, a);
         if (bad) status_raise(ST_PAGE_ID);
-        const int box = bad || nx_box == INT_MIN ? -1 : nx_box;
-        look(i + 1);
+        const int box = bad || nx_id == INT_MIN ? -1 : nx_id;
+        const Box x = nx;
+        if (i + 1 < p1) {
+          walk.next();
+          look(walk.a);
+        }
         const uint32_t st = done % ST, turn = done / ST;
         if (turn > 0 && !warp_wait(&empty[st], turn - 1, abort_flag, ST_PAGED_ROWS)) break;
         uint8_t *at = smem + st * STAGE, *mt = smem + ST * STAGE + st * META;
+        const uint32_t to = smem_u32(mt) + lane * 4;
         uint32_t all = 0xFFFFFFFFu;
+        const int64_t ko = KV8 ? box * ky.ks_str[0] + hk * ky.ks_str[1] + x.row : 0;
+        const int64_t vo = KV8 ? box * ky.vs_str[0] + hk * ky.vs_str[1] + x.row : 0;
+        const bool easy = __all_sync(0xffffffffu, (one || lane < tl.boxes) ? box >= 0 : true) && inside<BN>(rg, a) &&
+                          !ky.mask && (tl.dense || (one && x.row + BN <= ps));  // every key of the tile
 #pragma unroll
         for (int c = 0; c < KL; ++c) {
-          const int id = __shfl_sync(0xffffffffu, box, sub[c] & 31), off = a.row + at_row[c];
-          const int pos = a.base + (small ? sub[c] * ps : 0) + at_row[c];
-          bool in = id >= 0 && off < ps && sub[c] < tl.ppt && ((pos < rg.hi && pos >= rg.lo) || pos < rg.sink);
-          if (ky.mask && in) in = __ldg(ky.mask + id * ky.mask_stride + off) != 0;
-          if constexpr (KV8) {
-            const uint32_t to = smem_u32(mt) + (c * 32 + lane) * 4;
-            cp4(to, ky.ks + (in ? id * ky.ks_str[0] + hk * ky.ks_str[1] + off : 0), in);
-            cp4(to + MAX_BN * 4, ky.vs + (in ? id * ky.vs_str[0] + hk * ky.vs_str[1] + off : 0), in);
+          const int src = one ? 0 : sub[c] & 31, ar = one ? c * 32 + lane : at_row[c];
+          bool in = true;
+          if (!easy) {
+            const int id = __shfl_sync(0xffffffffu, box, src);
+            const int off = __shfl_sync(0xffffffffu, x.row, src) + ar;
+            const int pos = __shfl_sync(0xffffffffu, x.pos, src) + ar;
+            in = id >= 0 && (one || sub[c] < tl.boxes) && off < ps && seen(rg, pos);
+            if (ky.mask && in) in = __ldg(ky.mask + id * ky.mask_stride + off) != 0;
+            const uint32_t word = __ballot_sync(0xffffffffu, in);
+            all &= word;
+            if (lane == c) reinterpret_cast<uint32_t*>(mt + 2 * MAX_BN * 4)[c] = word;
           }
-          const uint32_t word = __ballot_sync(0xffffffffu, in);
-          all &= word;
-          if (lane == c) reinterpret_cast<uint32_t*>(mt + 2 * MAX_BN * 4)[c] = word;
+          if constexpr (KV8) {
+            const int64_t k = __shfl_sync(0xffffffffu, ko, src), v = __shfl_sync(0xffffffffu, vo, src);
+            cp4(to + c * 128, ky.ks + (in ? k + ar : 0), in);
+            cp4(to + MAX_BN * 4 + c * 128, ky.vs + (in ? v + ar : 0), in);
+          }
         }
+        if (easy && lane < KL) reinterpret_cast<uint32_t*>(mt + 2 * MAX_BN * 4)[lane] = 0xFFFFFFFFu;
         if constexpr (KV8) asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(&full[st])) : "memory");
         // BN live keys lie at consecutive positions, whatever the page size
         const bool whole = all == 0xFFFFFFFFu && a.base + BN <= rg.hi_min &&
                            (a.base >= rg.lo_max || a.base + BN <= rg.sink_min);
         if (lane == 4) *reinterpret_cast<uint2*>(mt + 2 * MAX_BN * 4 + 16) = make_uint2(whole, nth_tile(rg, i));
         __syncwarp();
-        auto copy = [&](uint8_t* k, int id) {
-          tma_load_4d(k, &tmK, &full[st], 0, a.row, hk, id);
-          if constexpr (!KV8) tma_load_4d(k + STAGE / 4, &tmK, &full[st], 64, a.row, hk, id);
-          tma_load_4d(k + STAGE / 2, &tmV, &full[st], 0, a.row, hk, id);
-          if constexpr (!KV8) tma_load_4d(k + 3 * STAGE / 4, &tmV, &full[st], 64, a.row, hk, id);
+        auto copy = [&](const CUtensorMap* mk, const CUtensorMap* mv, uint8_t* k, int row, int id) {
+          tma_load_4d(k, mk, &full[st], 0, row, hk, id);
+          if constexpr (!KV8) tma_load_4d(k + STAGE / 4, mk, &full[st], 64, row, hk, id);
+          tma_load_4d(k + STAGE / 2, mv, &full[st], 0, row, hk, id);
+          if constexpr (!KV8) tma_load_4d(k + 3 * STAGE / 4, mv, &full[st], 64, row, hk, id);
         };
-        if (!small) {  // one page: operands in uniform registers
+        if (one) {  // operands in uniform registers
           const int id = __shfl_sync(0xffffffffu, box, 0);
+          const int row = __shfl_sync(0xffffffffu, a.row, 0);
           if (elect_one()) {
             mbar_arrive_expect_tx(&full[st], id >= 0 ? STAGE : 0);
-            if (id >= 0) copy(at, id);
+            if (id >= 0) copy(&tm.k_tile, &tm.v_tile, at, row, id);
           }
         } else {
           const uint32_t boxes = __ballot_sync(0xffffffffu, box >= 0), bytes = (uint32_t)tl.rows * 128;
           if (lane == 0) mbar_arrive_expect_tx(&full[st], __popc(boxes) * bytes * (KV8 ? 2 : 4));
           __syncwarp();
-          if (box >= 0) copy(at + lane * bytes, box);
+          if (box >= 0) copy(&tm.k, &tm.v, at + lane * bytes, x.row, box);
         }
         __syncwarp();
       }
@@ -543,7 +556,7 @@ int64_t parts(const Shape& sh) {
 }
 
 template <int DT>
-static int start(const CUtensorMap& tk, const CUtensorMap& tv, const Keys& ky, const Queries& qr, const Cut& cut, float* part_o, float* part_l, cudaStream_t st) {
+static int start(const PageMaps& tm, const Keys& ky, const Queries& qr, const Cut& cut, float* part_o, float* part_l, cudaStream_t st) {
   static thread_local int configured = -1;
   int dev = 0;
   WFK_CUDA_TRY(cudaGetDevice(&dev));
@@ -561,7 +574,7 @@ static int start(const CUtensorMap& tk, const CUtensorMap& tv, const Keys& ky, c
   at.val.clusterDim = {(unsigned)cut.cluster, 1, 1};
   cfg.attrs = &at;
   cfg.numAttrs = cut.cluster > 1 ? 1 : 0;
-  WFK_CUDA_TRY(cudaLaunchKernelEx(&cfg, rows_kernel<DT>, tk, tv, ky, qr, cut, part_o, part_l));
+  WFK_CUDA_TRY(cudaLaunchKernelEx(&cfg, rows_kernel<DT>, tm, ky, qr, cut, part_o, part_l));
   return WF_OK;
 }
 
@@ -574,12 +587,12 @@ int launch(const Keys& ky, const Queries& qr, const Shape& sh, void* workspace, 
     part_o = static_cast<float*>(workspace);
     part_l = part_o + (int64_t)cut.outer * qr.rows * qr.H * HD;
   }
-  CUtensorMap tk, tv;
+  PageMaps tm;
   int rc;
-  if ((rc = page_maps(&tk, &tv, ky, qr.H / qr.group, cut.tl.rows)) != WF_OK) return rc;
-  rc = ky.dtype == WF_DTYPE_BF16   ? start<WF_DTYPE_BF16>(tk, tv, ky, qr, cut, part_o, part_l, st)
-       : ky.dtype == WF_DTYPE_E4M3 ? start<WF_DTYPE_E4M3>(tk, tv, ky, qr, cut, part_o, part_l, st)
-                                   : start<WF_DTYPE_S8>(tk, tv, ky, qr, cut, part_o, part_l, st);
+  if ((rc = page_maps(&tm, ky, qr.H / qr.group, cut.tl, sh.kv8 ? 128 : 64)) != WF_OK) return rc;
+  rc = ky.dtype == WF_DTYPE_BF16   ? start<WF_DTYPE_BF16>(tm, ky, qr, cut, part_o, part_l, st)
+       : ky.dtype == WF_DTYPE_E4M3 ? start<WF_DTYPE_E4M3>(tm, ky, qr, cut, part_o, part_l, st)
+                                   : start<WF_DTYPE_S8>(tm, ky, qr, cut, part_o, part_l, st);
   if (rc != WF_OK || cut.outer == 1) return rc;
   return join(ky, qr, part_o, part_l, cut.outer, st);
 }

@@ -3,7 +3,7 @@
 // Work item = two sub-tiles of 128 query rows of one K/V head (rows of a
 // sub-tile: TQ = 128 / group tokens x the group's query heads) against a run
 // of 128-key tiles.  K and V tiles are loaded once for both sub-tiles.
-//   warp 0       TMA producer (a lane to a page of a tile)
+//   warp 0       TMA producer (a lane to a box of a tile)
 //   warp 1       MMA issue: S_u = Q_u K_j^T (M=N=K=128), O_u += P_u V_j
 //   warp 2       marks the live keys of each tile, zeroes the V rows of the
 //                others (their P is 0, but 0 * NaN is not), fetches scales
@@ -49,7 +49,7 @@ struct Cfg {
   static constexpr int THREADS = KV8 ? 512 : 384;
   static constexpr int READERS = KV8 ? 15 : 11;  // warps that an item goes to
   static constexpr int NBARS = (3 * NS + 14 + META + 2 * WORKS + 1 + 1) & ~1;  // even: what follows is 16-byte aligned
-  static constexpr int META_BYTES = META * (16 + (KV8 ? 2 * BN * 4 : 0) + 16) + (KV8 ? 4 * BM * 4 : 0);
+  static constexpr int META_BYTES = META * (16 + (KV8 ? 2 * BN * 4 : 0) + 16) + (KV8 ? 4 * BN * 4 + 4 * BM * 4 : 0);
   static constexpr int SMEM = 1024 + 2 * SLOT + NS * SLOT + NBARS * 8 + META_BYTES + 16 + WORKS * WORK_BYTES;
   static_assert(SMEM <= 232448, "shared memory of one CTA");
 };
@@ -267,8 +267,8 @@ __device__ __forceinline__ void expand_q(uint8_t* sub, int row0, int lane, float
 
 template <int DT>
 __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
-    tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Keys ky,
+    tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ PageMaps tm,
+                const __grid_constant__ Keys ky,
                 const __grid_constant__ Queries qr, const __grid_constant__ Tiling tl, float* part_o, float* part_l) {
   constexpr bool KV8 = DT != WF_DTYPE_BF16;
   constexpr int NS = Cfg<KV8>::NS;
@@ -294,7 +294,8 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
   float* kpow = reinterpret_cast<float*>(whole + META);                 // [META] power of two of the K tile
   float* vpow = kpow + META;                                            // [META] and of V up to this tile
   uint32_t* scales = reinterpret_cast<uint32_t*>(vpow + 2 * META);      // [META][2][BN] hi_lo_f16
-  float* qpow = reinterpret_cast<float*>(scales + META * 2 * BN);       // [2][2][BM], by turns of the sub-tile's items
+  float* staged = reinterpret_cast<float*>(scales + META * 2 * BN);     // [2][2][BN] K and V scales as the pages have them, by turns of the tiles
+  float* qpow = staged + 4 * BN;       // [2][2][BM], by turns of the sub-tile's items
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(live) + Cfg<KV8>::META_BYTES);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   Work* works = reinterpret_cast<Work*>(reinterpret_cast<uint8_t*>(tmem_slot) + 16);  // [WORKS]
@@ -378,29 +379,54 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
       uint32_t slot_n = 0;        // ring slots filled
       uint32_t qn[2] = {0, 0};    // Q sub-tiles loaded
       bool ok = true;
-      const int sub = lane;       // a lane to a page of the tile
-      // A lane's page of tile t, as the table has it (-1: not needed); checked when it is used.
-      auto page_for = [&](int t, int& row) -> int {
-        const TileAt a = tile_at<BN>(tl, t);
-        row = a.row;
-        return sub < tl.ppt && needed(w, tl, a.page + sub) ? page_id(ky, w.sp, w.b, a.page + sub) : -1;
+      // The next tile's page ids as the table has them (INT_MIN: not needed),
+      // looked up under the last tile's loads: one, or a lane to a box.
+      int nx_id = INT_MIN, nx_row = 0;
+      bool nx_one = false;
+      auto look = [&](const TileAt& a) {
+        nx_one = one_box<BN>(tl, a);
+        if (nx_one) {
+          nx_row = a.row;
+          nx_id = page_id(ky, w.sp, w.b, a.page);
+        } else {
+          const Box x = box_at<BN>(tl, a, lane);
+          nx_row = x.row;
+          nx_id = lane < tl.boxes && needed(w, x.pos, min(tl.rows, tl.ps - x.row)) ? page_id(ky, w.sp, w.b, x.page) : INT_MIN;
+        }
       };
-      auto load = [&](const CUtensorMap* map, int id, int row) -> bool {
+      // The scales of a tile come with its K: the rows of a page are consecutive.
+      auto copy_scales = [&](uint64_t* bar, int page, int row, int box, int rows) {
+        float* to = staged + (slot_n / 2 & 1) * 2 * BN + box * rows;
+        bulk_load(to, ky.ks + page * ky.ks_str[0] + w.hk * ky.ks_str[1] + row, rows * 4, bar);
+        bulk_load(to + BN, ky.vs + page * ky.vs_str[0] + w.hk * ky.vs_str[1] + row, rows * 4, bar);
+      };
+      auto load = [&](const CUtensorMap* one, const CUtensorMap* box, int id, int row, bool whole) -> bool {
+        const bool with_scales = KV8 && tl.bulk && (slot_n & 1) == 0;
         const uint32_t s = slot_n % NS, n = slot_n / NS;
         if (n > 0 && !warp_wait(&empty[s], n - 1, abort_flag, ST_PAGED_PRODUCER)) return false;
-        uint8_t* dst = ring + s * SLOT;
-        const uint32_t box = (uint32_t)tl.rows * 128;
-        const uint32_t pages = __popc(__ballot_sync(0xffffffffu, id >= 0));
-        if (lane == 0) mbar_arrive_expect_tx(&raw[s], pages * box * (KV8 ? 1 : 2));
-        __syncwarp();
-        if (id >= 0) {
-          if constexpr (KV8) {
-            tma_load_4d(dst + HALF + sub * box, map, &raw[s], 0, row, w.hk, id);
-          } else {
-            tma_load_4d(dst + sub * box, map, &raw[s], 0, row, w.hk, id);
-            tma_load_4d(dst + HALF + sub * box, map, &raw[s], 64, row, w.hk, id);
+        uint8_t* dst = ring + s * SLOT + (KV8 ? HALF : 0);
+        if (whole) {  // one page: operands in uniform registers
+          const int uid = __shfl_sync(0xffffffffu, id, 0), urow = __shfl_sync(0xffffffffu, row, 0);
+          if (elect_one()) {
+            mbar_arrive_expect_tx(&raw[s], uid < 0 ? 0 : (KV8 ? HALF : SLOT) + (with_scales ? 2 * BN * 4 : 0));
+            if (uid >= 0) {
+              tma_load_4d(dst, one, &raw[s], 0, urow, w.hk, uid);
+              if constexpr (!KV8) tma_load_4d(dst + HALF, one, &raw[s], 64, urow, w.hk, uid);
+              if (with_scales) copy_scales(&raw[s], uid, urow, 0, BN);
+            }
+          }
+        } else {
+          const uint32_t bytes = (uint32_t)tl.rows * 128;
+          const uint32_t some = __popc(__ballot_sync(0xffffffffu, id >= 0));
+          if (lane == 0) mbar_arrive_expect_tx(&raw[s], some * (bytes * (KV8 ? 1 : 2) + (with_scales ? tl.rows * 8 : 0)));
+          __syncwarp();
+          if (id >= 0) {
+            tma_load_4d(dst + lane * bytes, box, &raw[s], 0, row, w.hk, id);
+            if constexpr (!KV8) tma_load_4d(dst + HALF + lane * bytes, box, &raw[s], 64, row, w.hk, id);
+            if (with_scales) copy_scales(&raw[s], id, row, lane, tl.rows);
           }
         }
+        __syncwarp();
         ++slot_n;
         return true;
       };
@@ -417,12 +443,16 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
           }
           ++qn[u];
         }
-        int row, next_row = 0, id, next_id = page_for(nth_tile(w, w.t0), next_row);
+        Walk<BN> walk(w, tl, w.t0);
+        look(walk.a);
         for (int i = w.t0; ok && i < w.t1; ++i) {
-          id = next_id >= 0 && next_id < ky.n_pages ? next_id : -1;
-          row = next_row;
-          if (!(ok = load(&tmK, id, row) && load(&tmV, id, row))) break;
-          if (i + 1 < w.t1) next_id = page_for(nth_tile(w, i + 1), next_row);  // looked up under these loads
+          const bool whole = nx_one;
+          const int row = nx_row, id = nx_id >= 0 && nx_id < ky.n_pages ? nx_id : -1;
+          if (!(ok = load(&tm.k_tile, &tm.k, id, row, whole) && load(&tm.v_tile, &tm.v, id, row, whole))) break;
+          if (i + 1 < w.t1) {
+            walk.next();
+            look(walk.a);
+          }
         }
       }
       if (*abort_flag && lane == 0) {
@@ -520,70 +550,131 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
       }
     } else if (warp == 2) {
       // --------------------------------------------------------------- marks
-      // Page ids are fetched a tile ahead, scales and mask bytes before the
-      // wait for the tile's K, so that their latency lies under it.
+      // Page ids are fetched two tiles ahead and a tile marked one ahead, so that
+      // no latency lies between the waits.
       uint32_t slot_n = 0, tiles = 0;
       bool ok = true;
-      int ids[4];
-      auto spot = [&](const TileAt& a, int c, int& j, int& off) -> bool {  // key c * 32 + lane of a tile; seen at all?
-        const int r = c * 32 + lane;
-        off = a.row + r;
-        j = a.page;
-        bool in = off < tl.ps;
-        if (tl.ps < BN) {
-          const int p = r / tl.rows;
-          off = r - p * tl.rows;
-          j += p;
-          in = off < tl.ps && p < tl.ppt;
-        }
-        const int pos = j * tl.ps + off;
-        return in && ((pos < w.hi && pos >= w.lo) || pos < w.sink);
-      };
-      auto fetch_ids = [&](int i) {
-        const TileAt a = tile_at<BN>(tl, nth_tile(w, i));
-        int j, off;
+      TileAt nx_at{};
+      int ids[4];  // pages of keys c * 32 + lane of the tile to fetch next (a one-box tile: all the same)
+      // Pages that divide a tile begin with it: a key's page and row there are fixed.
+      const bool even = tl.dense && BN % tl.ps == 0;
+      int sub[4], sub_row[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) ids[c] = spot(a, c, j, off) ? page_id(ky, w.sp, w.b, j) : INT_MIN;
+      for (int c = 0; c < 4; ++c) {
+        sub[c] = even ? (c * 32 + lane) / tl.ps : 0;
+        sub_row[c] = c * 32 + lane - sub[c] * tl.ps;
+      }
+      // Key r of a tile: page and row, and whether some row of the item sees it.
+      auto key = [&](const TileAt& a, int r, int& page, int& row) -> bool {
+        page = a.page;
+        row = a.row + r;
+        bool in = true;
+        if (tl.dense) {
+          if (row >= tl.ps) {
+            const int j = row / tl.ps;
+            page += j;
+            row -= j * tl.ps;
+          }
+        } else if (tl.ps < BN) {
+          const int j = r / tl.rows;
+          page += j;
+          row = r - j * tl.rows;
+          in = j < tl.boxes;
+        }
+        return in && row < tl.ps && seen(w, page * tl.ps + row);
+      };
+      auto look = [&](const TileAt& a) {
+        nx_at = a;
+        if (one_box<BN>(tl, a)) {
+          ids[0] = page_id(ky, w.sp, w.b, a.page);
+        } else if (even && inside<BN>(w, a)) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) ids[c] = page_id(ky, w.sp, w.b, a.page + sub[c]);
+        } else {
+          int page, row;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) ids[c] = key(a, c * 32 + lane, page, row) ? page_id(ky, w.sp, w.b, page) : INT_MIN;
+        }
+      };
+      // The tile's live keys.
+      auto fetch = [&](uint32_t (&words)[4]) {
+        const TileAt a = nx_at;
+        const bool one = one_box<BN>(tl, a);
+        if (one && ids[0] >= 0 && ids[0] < ky.n_pages && inside<BN>(w, a) && a.row + BN <= tl.ps && !ky.mask) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) words[c] = 0xFFFFFFFFu;
+        } else if (even && !one && inside<BN>(w, a)) {  // (cross attention, which has masks, is one page)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const bool in = ids[c] >= 0 && ids[c] < ky.n_pages;
+            if (!in) status_raise(ST_PAGE_ID);
+            words[c] = __ballot_sync(0xffffffffu, in);
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            int page, row;
+            bool in = key(a, c * 32 + lane, page, row);
+            const int id = one ? ids[0] : ids[c];
+            if (in && (id < 0 || id >= ky.n_pages)) {
+              status_raise(ST_PAGE_ID);
+              in = false;
+            }
+            if (ky.mask && in) in = __ldg(ky.mask + id * ky.mask_stride + row) != 0;
+            words[c] = __ballot_sync(0xffffffffu, in);
+          }
+        }
       };
       for (; ok && take(w); ) {
         float v_top = 0.f;  // power of two of V so far
-        if (w.t0 < w.t1) fetch_ids(w.t0);
-        for (int i = w.t0; ok && i < w.t1; ++i, ++tiles) {
-          const TileAt a = tile_at<BN>(tl, nth_tile(w, i));
-          bool in[4];
-          float sk[KV8 ? 4 : 1], sv[KV8 ? 4 : 1];
+        uint32_t next[4] = {0, 0, 0, 0};
+        if (w.t0 >= w.t1) continue;
+        Walk<BN> walk(w, tl, w.t0);
+        look(walk.a);
+        TileAt a = walk.a, a_next = a;
+        fetch(next);
+        if (w.t0 + 1 < w.t1) {
+          walk.next();
+          look(a_next = walk.a);
+        }
+        for (int i = w.t0; ok && i < w.t1; ++i, ++tiles, a = a_next, a_next = walk.a) {
+          uint32_t words[4];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            int j, off;
-            spot(a, c, j, off);
-            in[c] = ids[c] >= 0 && ids[c] < ky.n_pages;
-            if (!in[c] && ids[c] != INT_MIN) status_raise(ST_PAGE_ID);
-            if constexpr (KV8) {
-              sk[c] = sv[c] = 0.f;
-              if (in[c]) {
-                sk[c] = __ldg(ky.ks + ids[c] * ky.ks_str[0] + w.hk * ky.ks_str[1] + off);
-                sv[c] = __ldg(ky.vs + ids[c] * ky.vs_str[0] + w.hk * ky.vs_str[1] + off);
-              }
-            } else if (ky.mask && in[c]) {
-              in[c] = __ldg(ky.mask + ids[c] * ky.mask_stride + off) != 0;
-            }
+          for (int c = 0; c < 4; ++c) words[c] = next[c];
+          if (i + 1 < w.t1) fetch(next);
+          if (i + 2 < w.t1) {
+            walk.next();
+            look(walk.a);
           }
-          if (i + 1 < w.t1) fetch_ids(i + 1);
           // The marks of tile n - META are dead: its V slot (and with it its
           // P, which was formed with them) has been released before this
           // tile's K could land.
           uint32_t s = slot_n % NS;
           if (!(ok = warp_wait(&raw[s], slot_n / NS, abort_flag, ST_PAGED_MARK))) break;
           const uint32_t m = tiles % META;
-          uint32_t words[4];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) words[c] = __ballot_sync(0xffffffffu, in[c]);
           // 128 live keys lie at consecutive positions, whatever the page size.
           const bool all = (words[0] & words[1] & words[2] & words[3]) == 0xFFFFFFFFu && a.base + BN <= w.hi_min &&
                            (a.base >= w.lo_max || a.base + BN <= w.sink_min);
           if (lane < 4) live[m * 4 + lane] = lane < 2 ? (lane ? words[1] : words[0]) : (lane & 1 ? words[3] : words[2]);
           if (lane == 4) whole[m] = all;
           if constexpr (KV8) {
+            float sk[4], sv[4];  // 0 where no query sees the key
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int r = c * 32 + lane;
+              sk[c] = sv[c] = 0.f;
+              if (!(words[c] >> lane & 1)) continue;
+              if (tl.bulk) {
+                sk[c] = staged[(tiles & 1) * 2 * BN + r];
+                sv[c] = staged[(tiles & 1) * 2 * BN + BN + r];
+              } else {
+                int page, row;
+                key(a, r, page, row);
+                const int id = page_id(ky, w.sp, w.b, page);
+                sk[c] = __ldg(ky.ks + id * ky.ks_str[0] + w.hk * ky.ks_str[1] + row);
+                sv[c] = __ldg(ky.vs + id * ky.vs_str[0] + w.hk * ky.vs_str[1] + row);
+              }
+            }
             // Largest finite scales (non-negative floats order as integers).
             // A row whose V is not finite makes its key's score NaN instead:
             // the queries that see it become NaN, the others never meet it.
@@ -968,7 +1059,7 @@ int64_t parts(const Shape& sh) {
 }
 
 template <int DT>
-static int start(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap& tv, const Keys& ky,
+static int start(const CUtensorMap& tq, const PageMaps& tm, const Keys& ky,
                  const Queries& qr, const Tiling& tl, unsigned grid, float* part_o, float* part_l, cudaStream_t st) {
   using C = Cfg<DT != WF_DTYPE_BF16>;
   static thread_local int configured = -1;
@@ -978,7 +1069,7 @@ static int start(const CUtensorMap& tq, const CUtensorMap& tk, const CUtensorMap
     WFK_CUDA_TRY(cudaFuncSetAttribute(tile_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     configured = dev;
   }
-  tile_kernel<DT><<<grid, C::THREADS, C::SMEM, st>>>(tq, tk, tv, ky, qr, tl, part_o, part_l);
+  tile_kernel<DT><<<grid, C::THREADS, C::SMEM, st>>>(tq, tm, ky, qr, tl, part_o, part_l);
   WFK_CUDA_TRY(cudaGetLastError());
   return WF_OK;
 }
@@ -989,7 +1080,10 @@ int launch(const Keys& ky, const Queries& qr, const Shape& sh, void* workspace, 
   tl.tq = BM / qr.group;
   tl.splits = splits(sh);
   tl.even = dealt(sh);
-  CUtensorMap tq, tk, tv;
+  tl.bulk = tl.dense && ky.dtype != WF_DTYPE_BF16 && aligned16(ky.ks) && aligned16(ky.vs) &&
+            (ky.ks_str[0] | ky.ks_str[1] | ky.vs_str[0] | ky.vs_str[1]) % 4 == 0;
+  CUtensorMap tq;
+  PageMaps tm;
   int rc;
   {
     const uint64_t dim[4] = {HD, (uint64_t)qr.H, (uint64_t)(ky.cross ? qr.Lq : qr.rows),
@@ -1001,7 +1095,7 @@ int launch(const Keys& ky, const Queries& qr, const Shape& sh, void* workspace, 
                            CU_TENSOR_MAP_SWIZZLE_128B)) != WF_OK)
       return rc;
   }
-  if ((rc = page_maps(&tk, &tv, ky, G, tl.rows)) != WF_OK) return rc;
+  if ((rc = page_maps(&tm, ky, G, tl, BN)) != WF_OK) return rc;
   const int64_t items = tiles_bound(sh) * G * tl.splits;
   if (items > INT_MAX / 4) return fail(WF_ERR_INVALID_ARG, "attention: too many query tiles (%lld)", (long long)items);
   // Few key tiles to an item: one CTA per SM walks the items, the next one's
@@ -1011,9 +1105,9 @@ int launch(const Keys& ky, const Queries& qr, const Shape& sh, void* workspace, 
   const int64_t n_parts = parts(sh);
   float* part_o = static_cast<float*>(workspace);
   float* part_l = part_o + n_parts * HD;
-  rc = ky.dtype == WF_DTYPE_BF16   ? start<WF_DTYPE_BF16>(tq, tk, tv, ky, qr, tl, grid, part_o, part_l, st)
-       : ky.dtype == WF_DTYPE_E4M3 ? start<WF_DTYPE_E4M3>(tq, tk, tv, ky, qr, tl, grid, part_o, part_l, st)
-                                   : start<WF_DTYPE_S8>(tq, tk, tv, ky, qr, tl, grid, part_o, part_l, st);
+  rc = ky.dtype == WF_DTYPE_BF16   ? start<WF_DTYPE_BF16>(tq, tm, ky, qr, tl, grid, part_o, part_l, st)
+       : ky.dtype == WF_DTYPE_E4M3 ? start<WF_DTYPE_E4M3>(tq, tm, ky, qr, tl, grid, part_o, part_l, st)
+                                   : start<WF_DTYPE_S8>(tq, tm, ky, qr, tl, grid, part_o, part_l, st);
   if (rc != WF_OK || n_parts == 0) return rc;
   if (tl.even) {
     const int64_t left = items % SMS;  // with rows behind the sequence the device may have others
