@@ -14,7 +14,7 @@ import pytest
 
 from tests.test_attn_protocol import Bar
 
-META, WORKS = 3, 4
+META, WORKS = 4, 4
 
 
 class Sim:
@@ -169,8 +169,11 @@ class Sim:
             i, (nsub, nt) = item
             for j in range(nt):
                 s = n % self.NS
-                yield from self.wait(f"raw{s}", n // self.NS)
-                self.marks[tiles % (1 if self.wrong == "meta" else META)] = (i, j)
+                if not self.kv8:
+                    yield from self.wait(f"raw{s}", n // self.NS)
+                elif tiles > 0:  # the K before
+                    yield from self.wait(f"raw{(n - 2) % self.NS}", (n - 2) // self.NS)
+                self.marks[tiles % (1 if self.wrong == "meta" else META - (self.wrong == "ahead"))] = (i, j)
                 if self.kv8:
                     self.b[f"marked{tiles % META}"].arrive()
                     n += 2
@@ -229,7 +232,7 @@ class Sim:
                 yield from self.wait(f"s{u}", sn)
                 assert self.S[u] == ("S", i, j), (self.S[u], i, j)
                 for _ in range(3):  # the marks are read until P is complete
-                    assert self.marks[tiles % (1 if self.wrong == "meta" else META)] == (i, j), "marks overwritten"
+                    assert self.marks[tiles % (1 if self.wrong == "meta" else META - (self.wrong == "ahead"))] == (i, j), "marks overwritten"
                     yield
                 if self.kv8 and j == 0:
                     assert self.qpow[u][items % (1 if self.wrong == "qpow" else 2)] == i
@@ -316,7 +319,7 @@ def test_protocol(kv8):
         Sim(random_items(random.Random(seed)), kv8, seed).run()
 
 
-@pytest.mark.parametrize("wrong", ["p", "meta", "qpow", "works"])
+@pytest.mark.parametrize("wrong", ["p", "meta", "ahead", "qpow", "works"])
 def test_protocol_errors_are_caught(wrong):
     class Bad(Sim):
         pass
@@ -324,4 +327,4 @@ def test_protocol_errors_are_caught(wrong):
     Bad.wrong = wrong
     with pytest.raises(AssertionError):
         for seed in range(200):
-            Bad([(2, 4), (2, 1), (1, 1), (2, 1), (2, 3), (2, 2), (1, 1)], wrong == "qpow", seed).run()
+            Bad([(2, 4), (2, 1), (1, 1), (2, 1), (2, 3), (2, 2), (1, 1)], wrong in ("qpow", "ahead"), seed).run()

@@ -108,11 +108,10 @@ __device__ __forceinline__ int page_id(const Keys& ky, const Span& s, int b, int
 // box.
 struct Tiling {
   int ps, dense, tpp, boxes, rows;  // page size; tiles per page (large, not dense); boxes of a tile, their rows
-  int tq, splits, even, bulk;       // paged_tile.cu: tokens of a sub-tile, runs of keys, whether items are dealt
-                                    // evenly, whether scales can be fetched by bulk copies
+  int tq, splits, even;             // paged_tile.cu: tokens of a sub-tile, runs of keys, whether items are dealt evenly
 };
-inline Tiling tiling_of(int ps, int bn) {
-  Tiling t{ps, ps % 8 == 0, (ps + bn - 1) / bn, 1, bn, 0, 1, 0, 0};
+inline Tiling tiling_of(int ps, int bn, bool dense = true) {
+  Tiling t{ps, dense && ps % 8 == 0, (ps + bn - 1) / bn, 1, bn, 0, 1, 0};
   if (t.dense)
     while (ps % t.rows) t.rows /= 2;
   else if (ps < bn)
@@ -278,12 +277,6 @@ __device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
 __device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool take) {  // zero when not taken
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(take ? 4 : 0) : "memory");
 }
-// Untiled bulk copy (16-byte aligned, a multiple of 16 bytes) counted on `bar`.
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
-               "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
 // Power of two at or above x (> 0), between 2^-122 and 2^122 (a row scale is below 2^122).
 __device__ __forceinline__ float pow2_above(float x) {
   const uint32_t e = ((__float_as_uint(x) + 0x7FFFFFu) >> 23) << 23;
@@ -299,8 +292,8 @@ struct Shape {
   bool cross, kv8;
 };
 constexpr int SMS = 148;  // B200
-inline int64_t tiles_of_keys(const Shape& sh, int bn) {
-  const Tiling tl = tiling_of(sh.page_size, bn);
+inline int64_t tiles_of_keys(const Shape& sh, int bn, bool dense = true) {
+  const Tiling tl = tiling_of(sh.page_size, bn, dense);
   if (tl.dense) return (sh.keys + bn - 1) / bn;
   const int64_t pages = (sh.keys + sh.page_size - 1) / sh.page_size;
   return sh.page_size >= bn ? pages * tl.tpp : (pages + tl.boxes - 1) / tl.boxes;

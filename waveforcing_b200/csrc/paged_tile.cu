@@ -39,7 +39,7 @@ constexpr int BM = 128;  // rows of a sub-tile
 constexpr int BN = 128;  // keys of a tile
 constexpr int HALF = 16384;       // 128 rows x 64 bf16
 constexpr int SLOT = 2 * HALF;    // a K or V tile, or a Q sub-tile: [d 0-63][d 64-127]
-constexpr int META = 3;           // tiles whose marks (and scales) are kept
+constexpr int META = 4;           // tiles whose marks (and scales) are kept
 constexpr uint32_t COL_S = 0, COL_O = 256;
 
 constexpr int WORK_BYTES = 96, WORKS = 4;  // items found ahead
@@ -49,7 +49,7 @@ struct Cfg {
   static constexpr int THREADS = KV8 ? 512 : 384;
   static constexpr int READERS = KV8 ? 15 : 11;  // warps that an item goes to
   static constexpr int NBARS = (3 * NS + 14 + META + 2 * WORKS + 1 + 1) & ~1;  // even: what follows is 16-byte aligned
-  static constexpr int META_BYTES = META * (16 + (KV8 ? 2 * BN * 4 : 0) + 16) + (KV8 ? 4 * BN * 4 + 4 * BM * 4 : 0);
+  static constexpr int META_BYTES = META * (16 + (KV8 ? 2 * BN * 4 : 0) + 16) + (KV8 ? 4 * BM * 4 : 0);
   static constexpr int SMEM = 1024 + 2 * SLOT + NS * SLOT + NBARS * 8 + META_BYTES + 16 + WORKS * WORK_BYTES;
   static_assert(SMEM <= 232448, "shared memory of one CTA");
 };
@@ -294,8 +294,7 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
   float* kpow = reinterpret_cast<float*>(whole + META);                 // [META] power of two of the K tile
   float* vpow = kpow + META;                                            // [META] and of V up to this tile
   uint32_t* scales = reinterpret_cast<uint32_t*>(vpow + 2 * META);      // [META][2][BN] hi_lo_f16
-  float* staged = reinterpret_cast<float*>(scales + META * 2 * BN);     // [2][2][BN] K and V scales as the pages have them, by turns of the tiles
-  float* qpow = staged + 4 * BN;       // [2][2][BM], by turns of the sub-tile's items
+  float* qpow = reinterpret_cast<float*>(scales + META * 2 * BN);       // [2][2][BM], by turns of the sub-tile's items
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(live) + Cfg<KV8>::META_BYTES);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   Work* works = reinterpret_cast<Work*>(reinterpret_cast<uint8_t*>(tmem_slot) + 16);  // [WORKS]
@@ -394,36 +393,27 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
           nx_id = lane < tl.boxes && needed(w, x.pos, min(tl.rows, tl.ps - x.row)) ? page_id(ky, w.sp, w.b, x.page) : INT_MIN;
         }
       };
-      // The scales of a tile come with its K: the rows of a page are consecutive.
-      auto copy_scales = [&](uint64_t* bar, int page, int row, int box, int rows) {
-        float* to = staged + (slot_n / 2 & 1) * 2 * BN + box * rows;
-        bulk_load(to, ky.ks + page * ky.ks_str[0] + w.hk * ky.ks_str[1] + row, rows * 4, bar);
-        bulk_load(to + BN, ky.vs + page * ky.vs_str[0] + w.hk * ky.vs_str[1] + row, rows * 4, bar);
-      };
       auto load = [&](const CUtensorMap* one, const CUtensorMap* box, int id, int row, bool whole) -> bool {
-        const bool with_scales = KV8 && tl.bulk && (slot_n & 1) == 0;
         const uint32_t s = slot_n % NS, n = slot_n / NS;
         if (n > 0 && !warp_wait(&empty[s], n - 1, abort_flag, ST_PAGED_PRODUCER)) return false;
         uint8_t* dst = ring + s * SLOT + (KV8 ? HALF : 0);
         if (whole) {  // one page: operands in uniform registers
           const int uid = __shfl_sync(0xffffffffu, id, 0), urow = __shfl_sync(0xffffffffu, row, 0);
           if (elect_one()) {
-            mbar_arrive_expect_tx(&raw[s], uid < 0 ? 0 : (KV8 ? HALF : SLOT) + (with_scales ? 2 * BN * 4 : 0));
+            mbar_arrive_expect_tx(&raw[s], uid < 0 ? 0 : KV8 ? HALF : SLOT);
             if (uid >= 0) {
               tma_load_4d(dst, one, &raw[s], 0, urow, w.hk, uid);
               if constexpr (!KV8) tma_load_4d(dst + HALF, one, &raw[s], 64, urow, w.hk, uid);
-              if (with_scales) copy_scales(&raw[s], uid, urow, 0, BN);
             }
           }
         } else {
           const uint32_t bytes = (uint32_t)tl.rows * 128;
           const uint32_t some = __popc(__ballot_sync(0xffffffffu, id >= 0));
-          if (lane == 0) mbar_arrive_expect_tx(&raw[s], some * (bytes * (KV8 ? 1 : 2) + (with_scales ? tl.rows * 8 : 0)));
+          if (lane == 0) mbar_arrive_expect_tx(&raw[s], some * bytes * (KV8 ? 1 : 2));
           __syncwarp();
           if (id >= 0) {
             tma_load_4d(dst + lane * bytes, box, &raw[s], 0, row, w.hk, id);
             if constexpr (!KV8) tma_load_4d(dst + HALF + lane * bytes, box, &raw[s], 64, row, w.hk, id);
-            if (with_scales) copy_scales(&raw[s], id, row, lane, tl.rows);
           }
         }
         __syncwarp();
@@ -548,7 +538,7 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
         umma_commit(bar_fin);
         drain(bar_fin, 0, 200000000ull);
       }
-    } else if (warp == 2) {
+    } else if (warp == 2 && !KV8) {
       // --------------------------------------------------------------- marks
       // Page ids are fetched two tiles ahead and a tile marked one ahead, so that
       // no latency lies between the waits.
@@ -626,7 +616,6 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
         }
       };
       for (; ok && take(w); ) {
-        float v_top = 0.f;  // power of two of V so far
         uint32_t next[4] = {0, 0, 0, 0};
         if (w.t0 >= w.t1) continue;
         Walk<BN> walk(w, tl, w.t0);
@@ -657,69 +646,112 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
                            (a.base >= w.lo_max || a.base + BN <= w.sink_min);
           if (lane < 4) live[m * 4 + lane] = lane < 2 ? (lane ? words[1] : words[0]) : (lane & 1 ? words[3] : words[2]);
           if (lane == 4) whole[m] = all;
-          if constexpr (KV8) {
-            float sk[4], sv[4];  // 0 where no query sees the key
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const int r = c * 32 + lane;
-              sk[c] = sv[c] = 0.f;
-              if (!(words[c] >> lane & 1)) continue;
-              if (tl.bulk) {
-                sk[c] = staged[(tiles & 1) * 2 * BN + r];
-                sv[c] = staged[(tiles & 1) * 2 * BN + BN + r];
-              } else {
-                int page, row;
-                key(a, r, page, row);
-                const int id = page_id(ky, w.sp, w.b, page);
-                sk[c] = __ldg(ky.ks + id * ky.ks_str[0] + w.hk * ky.ks_str[1] + row);
-                sv[c] = __ldg(ky.vs + id * ky.vs_str[0] + w.hk * ky.vs_str[1] + row);
-              }
-            }
-            // Largest finite scales (non-negative floats order as integers).
-            // A row whose V is not finite makes its key's score NaN instead:
-            // the queries that see it become NaN, the others never meet it.
-            float tk = 0.f, tv = 0.f;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              if (!(fabsf(sv[c]) < INFINITY)) sk[c] = __uint_as_float(0x7FC00000u), sv[c] = 0.f;
-              tv = fmaxf(tv, fabsf(sv[c]));
-              tk = fmaxf(tk, fabsf(sk[c]) < INFINITY ? fabsf(sk[c]) : 0.f);
-            }
-            tk = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(tk)));
-            tv = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(tv)));
-            const float kp = pow2_above(tk);
-            if (v_top == 0.f || tv > v_top) v_top = pow2_above(tv) * 8.f;  // room: it should grow rarely
-            const float ik = 1.f / kp, iv = 1.f / v_top;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              scales[m * 2 * BN + c * 32 + lane] = hi_lo_f16(sk[c] * ik);
-              scales[m * 2 * BN + BN + c * 32 + lane] = hi_lo_f16(sv[c] * iv);
-            }
-            if (lane == 5) kpow[m] = kp;
-            if (lane == 6) vpow[m] = v_top;
-          }
           __syncwarp();
-          if (lane == 0) mbar_arrive(KV8 ? &marked[m] : &full[s]);
+          if (lane == 0) mbar_arrive(&full[s]);
           slot_n += 2;
-          if constexpr (!KV8) {
-            s = (slot_n - 1) % NS;
-            if (!(ok = warp_wait(&raw[s], (slot_n - 1) / NS, abort_flag, ST_PAGED_MARK))) break;
-            if ((words[0] & words[1] & words[2] & words[3]) != 0xFFFFFFFFu) {
-              uint8_t* v = ring + s * SLOT + (lane >> 4) * 128 + ((lane >> 3) & 1) * HALF + (lane & 7) * 16;
+          s = (slot_n - 1) % NS;
+          if (!(ok = warp_wait(&raw[s], (slot_n - 1) / NS, abort_flag, ST_PAGED_MARK))) break;
+          if ((words[0] & words[1] & words[2] & words[3]) != 0xFFFFFFFFu) {
+            uint8_t* v = ring + s * SLOT + (lane >> 4) * 128 + ((lane >> 3) & 1) * HALF + (lane & 7) * 16;
 #pragma unroll 1
-              for (int c = 0; c < 4; ++c) {
-                const uint32_t word = c < 2 ? (c ? words[1] : words[0]) : (c & 1 ? words[3] : words[2]);
-                if (word == 0xFFFFFFFFu) continue;
+            for (int c = 0; c < 4; ++c) {
+              const uint32_t word = c < 2 ? (c ? words[1] : words[0]) : (c & 1 ? words[3] : words[2]);
+              if (word == 0xFFFFFFFFu) continue;
 #pragma unroll 1
-                for (int r = lane >> 4; r < 32; r += 2)  // half a warp to a row, 16 bytes a lane
-                  if (!(word >> r & 1))
-                    *reinterpret_cast<uint4*>(v + (c * 32 + r - (lane >> 4)) * 128) = make_uint4(0, 0, 0, 0);
-              }
-              fence_proxy_async_smem();
-              __syncwarp();
+              for (int r = lane >> 4; r < 32; r += 2)  // half a warp to a row, 16 bytes a lane
+                if (!(word >> r & 1))
+                  *reinterpret_cast<uint4*>(v + (c * 32 + r - (lane >> 4)) * 128) = make_uint4(0, 0, 0, 0);
             }
-            if (lane == 0) mbar_arrive(&full[s]);
+            fence_proxy_async_smem();
+            __syncwarp();
           }
+          if (lane == 0) mbar_arrive(&full[s]);
+        }
+      }
+    } else if (warp == 2) {
+      // ---------------------------------------------- marks and scales, 8 bits
+      // A tile is marked when the K before it has landed, so that its expansion
+      // waits for its codes alone; its scales are loaded before that wait and
+      // its page ids a tile earlier.
+      uint32_t slot_n = 0, tiles = 0;
+      bool ok = true;
+      int ids[4], box[4], at_row[4];  // of keys c * 32 + lane: page id, box, row of the box
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        box[c] = tl.ps < BN ? (c * 32 + lane) / tl.rows : 0;
+        at_row[c] = c * 32 + lane - box[c] * tl.rows;
+      }
+      auto key = [&](const TileAt& a, int c, int& page, int& row) -> bool {  // seen by some row of the item?
+        page = a.page + box[c];
+        row = a.row + at_row[c];
+        return box[c] < tl.boxes && row < tl.ps && seen(w, page * tl.ps + row);
+      };
+      auto look = [&](const TileAt& a) {
+        int page, row;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) ids[c] = key(a, c, page, row) ? page_id(ky, w.sp, w.b, page) : INT_MIN;
+      };
+      for (; ok && take(w); ) {
+        float v_top = 0.f;  // power of two of V so far
+        if (w.t0 >= w.t1) continue;
+        Walk<BN> walk(w, tl, w.t0);
+        look(walk.a);
+        for (int i = w.t0; ok && i < w.t1; ++i, ++tiles) {
+          const TileAt a = walk.a;
+          bool in[4];
+          float sk[4], sv[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            in[c] = ids[c] >= 0 && ids[c] < ky.n_pages;
+            if (!in[c] && ids[c] != INT_MIN) status_raise(ST_PAGE_ID);
+            sk[c] = sv[c] = 0.f;
+            if (in[c]) {
+              const int row = a.row + at_row[c];
+              sk[c] = __ldg(ky.ks + ids[c] * ky.ks_str[0] + w.hk * ky.ks_str[1] + row);
+              sv[c] = __ldg(ky.vs + ids[c] * ky.vs_str[0] + w.hk * ky.vs_str[1] + row);
+            }
+          }
+          if (i + 1 < w.t1) {
+            walk.next();
+            look(walk.a);
+          }
+          // The K before has landed: S of three tiles before has been formed, over
+          // the P of the tile whose marks lay here (META tiles before).
+          if (tiles > 0 && !(ok = warp_wait(&raw[(slot_n - 2) % NS], (slot_n - 2) / NS, abort_flag, ST_PAGED_MARK))) break;
+          const uint32_t m = tiles % META;
+          uint32_t words[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) words[c] = __ballot_sync(0xffffffffu, in[c]);
+          // 128 live keys lie at consecutive positions, whatever the page size.
+          const bool all = (words[0] & words[1] & words[2] & words[3]) == 0xFFFFFFFFu && a.base + BN <= w.hi_min &&
+                           (a.base >= w.lo_max || a.base + BN <= w.sink_min);
+          if (lane < 4) live[m * 4 + lane] = lane < 2 ? (lane ? words[1] : words[0]) : (lane & 1 ? words[3] : words[2]);
+          if (lane == 4) whole[m] = all;
+          // Largest finite scales (non-negative floats order as integers).
+          // A row whose V is not finite makes its key's score NaN instead:
+          // the queries that see it become NaN, the others never meet it.
+          float tk = 0.f, tv = 0.f;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            if (!(fabsf(sv[c]) < INFINITY)) sk[c] = __uint_as_float(0x7FC00000u), sv[c] = 0.f;
+            tv = fmaxf(tv, fabsf(sv[c]));
+            tk = fmaxf(tk, fabsf(sk[c]) < INFINITY ? fabsf(sk[c]) : 0.f);
+          }
+          tk = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(tk)));
+          tv = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(tv)));
+          const float kp = pow2_above(tk);
+          if (v_top == 0.f || tv > v_top) v_top = pow2_above(tv) * 8.f;  // room: it should grow rarely
+          const float ik = 1.f / kp, iv = 1.f / v_top;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            scales[m * 2 * BN + c * 32 + lane] = hi_lo_f16(sk[c] * ik);
+            scales[m * 2 * BN + BN + c * 32 + lane] = hi_lo_f16(sv[c] * iv);
+          }
+          if (lane == 5) kpow[m] = kp;
+          if (lane == 6) vpow[m] = v_top;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&marked[m]);
+          slot_n += 2;
         }
       }
     }
@@ -1026,7 +1058,7 @@ static int64_t tiles_bound(const Shape& sh) {
   const int64_t seqs = sh.rows < sh.seqs ? sh.rows : sh.seqs;
   return (sh.rows + seqs * (step - 1)) / step;
 }
-static int64_t key_tiles(const Shape& sh) { return tiles_of_keys(sh, BN); }
+static int64_t key_tiles(const Shape& sh) { return tiles_of_keys(sh, BN, !sh.kv8); }
 
 // Whether the launch is one sequence on a CTA per SM, dealt out as Deal says
 // (should its rows see different keys after all, whole items in turn); worth it
@@ -1076,12 +1108,10 @@ static int start(const CUtensorMap& tq, const PageMaps& tm, const Keys& ky,
 
 int launch(const Keys& ky, const Queries& qr, const Shape& sh, void* workspace, cudaStream_t st) {
   const int G = qr.H / qr.group, ps = ky.page_size;
-  Tiling tl = tiling_of(ps, BN);
+  Tiling tl = tiling_of(ps, BN, !sh.kv8);
   tl.tq = BM / qr.group;
   tl.splits = splits(sh);
   tl.even = dealt(sh);
-  tl.bulk = tl.dense && ky.dtype != WF_DTYPE_BF16 && aligned16(ky.ks) && aligned16(ky.vs) &&
-            (ky.ks_str[0] | ky.ks_str[1] | ky.vs_str[0] | ky.vs_str[1]) % 4 == 0;
   CUtensorMap tq;
   PageMaps tm;
   int rc;
