@@ -19,10 +19,12 @@
 // Read: bf16(code * scale), one rounding.
 //
 // Half a warp holds a row (8 elements a lane): lanes 0-15 take K, 16-31 V.  A
-// block takes 16 packed rows and up to 4 heads; all its loads are in flight
-// before the first use.
+// block takes 16 packed rows and 4 heads at a time, all their loads in flight
+// before the first use, then the next 4 heads, loaded under the stores of the
+// last: the rows' slots are looked up once.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <climits>
 
 #include "host_util.h"
@@ -37,6 +39,7 @@ constexpr int HEADS = 4;            // heads of a block
 constexpr int THREADS = 256;
 constexpr int STEP = THREADS / 32;  // (row, head) pairs a pass over the block covers
 constexpr int NPAIR = RUN * HEADS / STEP;
+constexpr int SMS = 148;  // B200
 
 struct Pool {
   void *k, *v;
@@ -51,9 +54,12 @@ struct Rows {  // packed bf16 rows: read by the write, written by the read
   int64_t k_str[2], v_str[2];  // row, head
 };
 
-// Slot of each of the block's rows: page id (-1: none) and row in the page.
+// Slot of each of the block's rows: page id (-1: none), row in the page (-1:
+// behind the last sequence), and where it lies in K and V pages (-1: nowhere)
+// and their scales, without the head.
 struct Slots {
-  int page[RUN], row[RUN], drop[RUN];
+  int page[RUN], row[RUN];
+  int64_t at[2][RUN], scale[2][RUN];
 };
 
 __device__ __forceinline__ void find_slots(Slots& sl, const Batch& bt, const Pool& pool, int r0) {
@@ -78,9 +84,13 @@ __device__ __forceinline__ void find_slots(Slots& sl, const Batch& bt, const Poo
     } else {
       row = -1;  // behind the last sequence
     }
-    sl.page[threadIdx.x] = page;
-    sl.row[threadIdx.x] = row;
-    sl.drop[threadIdx.x] = 0;
+    const int t = threadIdx.x;
+    sl.page[t] = page;
+    sl.row[t] = row;
+    sl.at[0][t] = page < 0 ? -1 : page * pool.k_str[0] + row * pool.k_str[2];
+    sl.at[1][t] = page < 0 ? -1 : page * pool.v_str[0] + row * pool.v_str[2];
+    sl.scale[0][t] = page * pool.ks_str[0] + row;
+    sl.scale[1][t] = page * pool.vs_str[0] + row;
   }
 }
 
@@ -103,7 +113,7 @@ __device__ __forceinline__ void drop_overwritten(Slots& sl, const Batch& bt, con
       for (int i = 0; i < RUN; ++i) {
         if (id == sl.page[i] && id >= 0) {
           const int pos = j * ps + sl.row[i];
-          if (pos >= base && pos < total && s.first + (pos - base) > r0 + i) sl.drop[i] = 1;
+          if (pos >= base && pos < total && s.first + (pos - base) > r0 + i) sl.at[0][i] = sl.at[1][i] = -1;
         }
       }
     }
@@ -114,131 +124,183 @@ __device__ __forceinline__ float snap18(float y) {
   return __uint_as_float((__float_as_uint(y) + 0x20u) & ~0x3Fu);
 }
 
+// Calls fetch(buffer, h) and put(buffer, h) for h = h0, h0 + HEADS, ... below h1,
+// each fetch before the put that precedes its own (two buffers by turns).
+template <class Buf, class Fetch, class Look, class Put>
+__device__ __forceinline__ void by_heads(int h0, int h1, Fetch fetch, Look look, Put put) {
+  Buf a, b;
+  fetch(a, h0);
+  look();
+  for (int h = h0; h < h1; h += 2 * HEADS) {
+    if (h + HEADS < h1) fetch(b, h + HEADS);
+    put(a, h);
+    if (h + HEADS >= h1) break;
+    if (h + 2 * HEADS < h1) fetch(a, h + 2 * HEADS);
+    put(b, h + HEADS);
+  }
+}
+
 template <int DT>
 __global__ void __launch_bounds__(THREADS) write_kernel(const __grid_constant__ Batch bt,
                                                         const __grid_constant__ Pool pool,
-                                                        const __grid_constant__ Rows src) {
+                                                        const __grid_constant__ Rows src, int heads) {
   __shared__ Slots sl;
-  const int r0 = blockIdx.x * RUN, h0 = blockIdx.y * HEADS;
+  const int r0 = blockIdx.x * RUN, h_lo = blockIdx.y * heads, h_hi = min(h_lo + heads, pool.heads);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane & 15;
+  const int i0 = warp / HEADS, dh = warp % HEADS;  // row i0 + p * STEP / HEADS, head h + dh of pair p
   const bool is_v = lane >= 16;
   const __nv_bfloat16* x = static_cast<const __nv_bfloat16*>(is_v ? src.v : src.k) + c * 8;
   const int64_t* xs = is_v ? src.v_str : src.k_str;
-  uint4 v[NPAIR];
+  struct Buf {
+    uint4 v[NPAIR];
+  };
+  auto fetch = [&](Buf& f, int h) {
+    const __nv_bfloat16* at = x + (int64_t)(r0 + i0) * xs[0] + (h + dh) * xs[1];
 #pragma unroll
-  for (int p = 0; p < NPAIR; ++p) {
-    const int i = (p * STEP + warp) / HEADS, h = h0 + (p * STEP + warp) % HEADS;
-    v[p] = make_uint4(0, 0, 0, 0);
-    if (r0 + i < bt.rows && h < pool.heads)
-      v[p] = __ldg(reinterpret_cast<const uint4*>(x + (r0 + i) * xs[0] + h * xs[1]));
-  }
-  find_slots(sl, bt, pool, r0);
-  __syncthreads();
-  drop_overwritten(sl, bt, pool, r0);
-  __syncthreads();
-  const int64_t* ps = is_v ? pool.v_str : pool.k_str;
-  const int64_t* ss = is_v ? pool.vs_str : pool.ks_str;
+    for (int p = 0; p < NPAIR; ++p) {
+      f.v[p] = make_uint4(0, 0, 0, 0);
+      if (r0 + i0 + p * (STEP / HEADS) < bt.rows && h + dh < h_hi)
+        f.v[p] = __ldg(reinterpret_cast<const uint4*>(at + p * (STEP / HEADS) * xs[0]));
+    }
+  };
+  auto look = [&]() {
+    find_slots(sl, bt, pool, r0);
+    __syncthreads();
+    drop_overwritten(sl, bt, pool, r0);
+    __syncthreads();
+  };
+  const int64_t hs = (is_v ? pool.v_str : pool.k_str)[1], shs = (is_v ? pool.vs_str : pool.ks_str)[1];
   float* scales = is_v ? pool.vs : pool.ks;
   constexpr float Q = DT == WF_DTYPE_E4M3 ? 448.f : 127.f;
+  auto put = [&](const Buf& f, int h4) {
+    const int h = h4 + dh;
+    if (h >= h_hi) return;
+    float inv = 0.f;  // Q / a of pair c / 2's row; 0 where it is not finite
+    if constexpr (DT != WF_DTYPE_BF16) {
+      // Maxima of the 8 rows over the half warp, rows and lanes folded together:
+      // lane c ends with row c / 2's, so that one division serves 8 rows.
+      uint32_t m[NPAIR];
 #pragma unroll
-  for (int p = 0; p < NPAIR; ++p) {
-    const int i = (p * STEP + warp) / HEADS, h = h0 + (p * STEP + warp) % HEADS;
-    const int64_t page = sl.page[i], row = sl.row[i];
-    const bool live = page >= 0 && !sl.drop[i] && h < pool.heads;  // one value for the whole warp
-    if (!live) continue;
-    const int64_t at = page * ps[0] + h * ps[1] + row * ps[2] + c * 8;
-    if constexpr (DT == WF_DTYPE_BF16) {
-      *reinterpret_cast<uint4*>((is_v ? static_cast<__nv_bfloat16*>(pool.v) : static_cast<__nv_bfloat16*>(pool.k)) +
-                                at) = v[p];
-    } else {
-      const uint32_t m2 = quant::amax8_bits(v[p], 0u);
-      uint32_t m = max(m2 & 0xFFFFu, m2 >> 16);
+      for (int p = 0; p < NPAIR; ++p) m[p] = quant::amax8_bits(f.v[p], 0u);
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const bool finite = m < 0x7F80u;
-      const float a = fmaxf(__uint_as_float(m << 16), 0x1p-100f);
-      const float inv = __fdiv_rn(Q, a);
-      const uint32_t w[4] = {v[p].x, v[p].y, v[p].z, v[p].w};
-      uint32_t codes[2] = {0, 0};
+      for (int n = NPAIR / 2, o = 8; n > 0; n /= 2, o /= 2) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float y0 = snap18(__uint_as_float(w[e] << 16) * inv);
-        const float y1 = snap18(__uint_as_float(w[e] & 0xFFFF0000u) * inv);
-        uint32_t two;
-        if constexpr (DT == WF_DTYPE_E4M3)
-          two = quant::e4m3x2_hw(y0, y1);
-        else
-          two = (static_cast<uint32_t>(__float2int_rn(y0)) & 0xFFu) |
-                ((static_cast<uint32_t>(__float2int_rn(y1)) & 0xFFu) << 8);
-        codes[e >> 1] |= two << ((e & 1) * 16);
+        for (int p = 0; p < n; ++p) {
+          const uint32_t give = (c & o) ? m[p] : m[p + n], keep = (c & o) ? m[p + n] : m[p];
+          m[p] = quant::vmax_u16x2(keep, __shfl_xor_sync(0xffffffffu, give, o));
+        }
       }
-      if (!finite) codes[0] = codes[1] = 0;
-      uint8_t* base = static_cast<uint8_t*>(is_v ? pool.v : pool.k);
-      *reinterpret_cast<uint2*>(base + at) = make_uint2(codes[0], codes[1]);
-      if (c == 0) scales[page * ss[0] + h * ss[1] + row] = finite ? __fdiv_rn(a, Q) : __uint_as_float(0x7FC00000u);
+      m[0] = quant::vmax_u16x2(m[0], __shfl_xor_sync(0xffffffffu, m[0], 1));
+      const uint32_t top = max(m[0] & 0xFFFFu, m[0] >> 16);
+      const bool finite = top < 0x7F80u;
+      const float a = fmaxf(__uint_as_float(top << 16), 0x1p-100f);
+      inv = finite ? __fdiv_rn(Q, a) : 0.f;
+      const int i = i0 + (c >> 1) * (STEP / HEADS);
+      if (!(c & 1) && sl.at[is_v][i] >= 0)
+        scales[sl.scale[is_v][i] + h * shs] = finite ? __fdiv_rn(a, Q) : __uint_as_float(0x7FC00000u);
     }
-  }
+    const int64_t to = h * hs + c * 8;
+#pragma unroll
+    for (int p = 0; p < NPAIR; ++p) {
+      const int64_t at = sl.at[is_v][i0 + p * (STEP / HEADS)];
+      if constexpr (DT == WF_DTYPE_BF16) {
+        if (at >= 0)
+          *reinterpret_cast<uint4*>((is_v ? static_cast<__nv_bfloat16*>(pool.v) : static_cast<__nv_bfloat16*>(pool.k)) +
+                                    at + to) = f.v[p];
+      } else {
+        const float mul = __shfl_sync(0xffffffffu, inv, 2 * p, 16);
+        const uint32_t w[4] = {f.v[p].x, f.v[p].y, f.v[p].z, f.v[p].w};
+        uint32_t codes[2] = {0, 0};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float y0 = snap18(__uint_as_float(w[e] << 16) * mul);
+          const float y1 = snap18(__uint_as_float(w[e] & 0xFFFF0000u) * mul);
+          uint32_t two;
+          if constexpr (DT == WF_DTYPE_E4M3)
+            two = quant::e4m3x2_hw(y0, y1);
+          else
+            two = (static_cast<uint32_t>(__float2int_rn(y0)) & 0xFFu) |
+                  ((static_cast<uint32_t>(__float2int_rn(y1)) & 0xFFu) << 8);
+          codes[e >> 1] |= two << ((e & 1) * 16);
+        }
+        if (mul == 0.f) codes[0] = codes[1] = 0;
+        uint8_t* base = static_cast<uint8_t*>(is_v ? pool.v : pool.k);
+        if (at >= 0) *reinterpret_cast<uint2*>(base + at + to) = make_uint2(codes[0], codes[1]);
+      }
+    }
+  };
+  by_heads<Buf>(h_lo, h_hi, fetch, look, put);
 }
 
 template <int DT>
 __global__ void __launch_bounds__(THREADS) read_kernel(const __grid_constant__ Batch bt,
                                                        const __grid_constant__ Pool pool,
-                                                       const __grid_constant__ Rows dst) {
+                                                       const __grid_constant__ Rows dst, int heads) {
   __shared__ Slots sl;
-  const int r0 = blockIdx.x * RUN, h0 = blockIdx.y * HEADS;
+  const int r0 = blockIdx.x * RUN, h_lo = blockIdx.y * heads, h_hi = min(h_lo + heads, pool.heads);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane & 15;
+  const int i0 = warp / HEADS, dh = warp % HEADS;
   const bool is_v = lane >= 16;
   find_slots(sl, bt, pool, r0);
   __syncthreads();
-  const int64_t* ps = is_v ? pool.v_str : pool.k_str;
-  const int64_t* ss = is_v ? pool.vs_str : pool.ks_str;
+  const int64_t hs = (is_v ? pool.v_str : pool.k_str)[1], shs = (is_v ? pool.vs_str : pool.ks_str)[1];
   const float* scales = is_v ? pool.vs : pool.ks;
   constexpr bool WIDE = DT == WF_DTYPE_BF16;
-  uint4 w[WIDE ? NPAIR : 1];
-  uint2 q[WIDE ? 1 : NPAIR];
-  float s[WIDE ? 1 : NPAIR];
+  struct Buf {
+    uint4 w[WIDE ? NPAIR : 1];
+    uint2 q[WIDE ? 1 : NPAIR];
+    float s;  // scale of pair c / 2's row
+  };
+  auto fetch = [&](Buf& f, int h4) {
+    const int h = h4 + dh;
+    if constexpr (!WIDE) {
+      const int i = i0 + (c >> 1) * (STEP / HEADS);
+      f.s = sl.at[is_v][i] >= 0 && h < h_hi ? __ldg(scales + sl.scale[is_v][i] + h * shs) : 0.f;
+    }
+    const int64_t from = h * hs + c * 8;
 #pragma unroll
-  for (int p = 0; p < NPAIR; ++p) {
-    const int i = (p * STEP + warp) / HEADS, h = h0 + (p * STEP + warp) % HEADS;
-    const int64_t page = sl.page[i], row = sl.row[i];
-    const bool live = page >= 0 && h < pool.heads;
-    const int64_t at = live ? page * ps[0] + h * ps[1] + row * ps[2] + c * 8 : 0;
-    if constexpr (WIDE) {
-      w[p] = make_uint4(0, 0, 0, 0);
-      if (live)
-        w[p] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(is_v ? pool.v : pool.k) + at));
-    } else {
-      q[p] = make_uint2(0, 0);
-      s[p] = 0.f;
-      if (live) {
-        q[p] = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(is_v ? pool.v : pool.k) + at));
-        s[p] = __ldg(scales + page * ss[0] + h * ss[1] + row);
+    for (int p = 0; p < NPAIR; ++p) {
+      const int64_t at = sl.at[is_v][i0 + p * (STEP / HEADS)] + from;
+      const bool live = at >= from && h < h_hi;
+      if constexpr (WIDE) {
+        f.w[p] = make_uint4(0, 0, 0, 0);
+        if (live)
+          f.w[p] = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(is_v ? pool.v : pool.k) + at));
+      } else {
+        f.q[p] = make_uint2(0, 0);
+        if (live) f.q[p] = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(is_v ? pool.v : pool.k) + at));
       }
     }
-  }
+  };
   __nv_bfloat16* y = static_cast<__nv_bfloat16*>(is_v ? dst.v : dst.k) + c * 8;
   const int64_t* ys = is_v ? dst.v_str : dst.k_str;
+  auto put = [&](const Buf& f, int h4) {
+    const int h = h4 + dh;
+    if (h >= h_hi) return;
 #pragma unroll
-  for (int p = 0; p < NPAIR; ++p) {
-    const int i = (p * STEP + warp) / HEADS, h = h0 + (p * STEP + warp) % HEADS;
-    if (sl.row[i] < 0 || h >= pool.heads) continue;  // behind the last sequence: left as it was
-    uint4 o;
-    if constexpr (WIDE) {
-      o = w[p];
-    } else if constexpr (DT == WF_DTYPE_E4M3) {
-      o = quant::dequant8(q[p], s[p]);
-    } else {
-      uint32_t u[4];
+    for (int p = 0; p < NPAIR; ++p) {
+      const int i = i0 + p * (STEP / HEADS);
+      const float scale = WIDE ? 1.f : __shfl_sync(0xffffffffu, f.s, 2 * p, 16);
+      if (sl.row[i] < 0) continue;  // behind the last sequence: left as it was
+      uint4 o;
+      if constexpr (WIDE) {
+        o = f.w[p];
+      } else if constexpr (DT == WF_DTYPE_E4M3) {
+        o = quant::dequant8(f.q[p], scale);
+      } else {
+        uint32_t u[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t two = (e < 2 ? q[p].x : q[p].y) >> ((e & 1) * 16);
-        u[e] = pack_bf16x2(static_cast<float>(static_cast<int8_t>(two & 0xFF)) * s[p],
-                           static_cast<float>(static_cast<int8_t>((two >> 8) & 0xFF)) * s[p]);
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t two = (e < 2 ? f.q[p].x : f.q[p].y) >> ((e & 1) * 16);
+          u[e] = pack_bf16x2(static_cast<float>(static_cast<int8_t>(two & 0xFF)) * scale,
+                             static_cast<float>(static_cast<int8_t>((two >> 8) & 0xFF)) * scale);
+        }
+        o = make_uint4(u[0], u[1], u[2], u[3]);
       }
-      o = make_uint4(u[0], u[1], u[2], u[3]);
+      *reinterpret_cast<uint4*>(y + (int64_t)(r0 + i) * ys[0] + h * ys[1]) = o;
     }
-    *reinterpret_cast<uint4*>(y + (r0 + i) * ys[0] + h * ys[1]) = o;
-  }
+  };
+  by_heads<Buf>(h_lo, h_hi, fetch, [] {}, put);
 }
 
 // ------------------------------------------------------------------- host
@@ -302,14 +364,17 @@ static int run(const char* who, const wf_kv_pages* pages, const wf_kv_batch* bat
   const Batch bt = make_batch(batch);
   const Pool pool = make_pool(pages);
   const Rows rows{k, v, {ks[0], ks[1]}, {vs[0], vs[1]}};
-  const dim3 grid((unsigned)((batch->rows + RUN - 1) / RUN), (unsigned)((pages->heads + HEADS - 1) / HEADS));
+  // Heads of a block: as many as leave 8 blocks to an SM.
+  const int64_t runs = (batch->rows + RUN - 1) / RUN, groups = (pages->heads + HEADS - 1) / HEADS;
+  const int heads = HEADS * (int)std::clamp<int64_t>(runs * groups / (8 * SMS), 1, groups);
+  const dim3 grid((unsigned)runs, (unsigned)((pages->heads + heads - 1) / heads));
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto pick = [&](auto bf, auto e4, auto s8) {
     return pages->dtype == WF_DTYPE_BF16 ? bf : pages->dtype == WF_DTYPE_E4M3 ? e4 : s8;
   };
   auto kern = write ? pick(write_kernel<WF_DTYPE_BF16>, write_kernel<WF_DTYPE_E4M3>, write_kernel<WF_DTYPE_S8>)
                     : pick(read_kernel<WF_DTYPE_BF16>, read_kernel<WF_DTYPE_E4M3>, read_kernel<WF_DTYPE_S8>);
-  kern<<<grid, THREADS, 0, st>>>(bt, pool, rows);
+  kern<<<grid, THREADS, 0, st>>>(bt, pool, rows, heads);
   WFK_CUDA_TRY(cudaGetLastError());
   return WF_OK;
 }
