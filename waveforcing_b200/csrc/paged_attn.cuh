@@ -108,10 +108,11 @@ __device__ __forceinline__ int page_id(const Keys& ky, const Span& s, int b, int
 // box.
 struct Tiling {
   int ps, dense, tpp, boxes, rows;  // page size; tiles per page (large, not dense); boxes of a tile, their rows
-  int tq, splits, even;             // paged_tile.cu: tokens of a sub-tile, runs of keys, whether items are dealt evenly
+  int tq, splits, even, wide;       // paged_tile.cu: tokens of a sub-tile, runs of keys, whether items are dealt
+                                    // evenly, whether rows of O begin on 32-byte boundaries
 };
 inline Tiling tiling_of(int ps, int bn, bool dense = true) {
-  Tiling t{ps, dense && ps % 8 == 0, (ps + bn - 1) / bn, 1, bn, 0, 1, 0};
+  Tiling t{ps, dense && ps % 8 == 0, (ps + bn - 1) / bn, 1, bn, 0, 1, 0, 0};
   if (t.dense)
     while (ps % t.rows) t.rows /= 2;
   else if (ps < bn)

@@ -265,6 +265,20 @@ __device__ __forceinline__ void expand_q(uint8_t* sub, int row0, int lane, float
   }
 }
 
+// 32 bytes: a whole sector in one store where the address allows it (a lane
+// writes its own row, so that two halves would be two passes over 32 sectors).
+__device__ __forceinline__ void store32(void* to, const uint32_t* r, bool wide) {
+  if (wide) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(r[0]), "r"(r[1]), "r"(r[2]),
+                 "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+  } else {
+    uint4* d = static_cast<uint4*>(to);
+    d[0] = make_uint4(r[0], r[1], r[2], r[3]);
+    d[1] = make_uint4(r[4], r[5], r[6], r[7]);
+  }
+}
+
 template <int DT>
 __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
     tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ PageMaps tm,
@@ -946,30 +960,28 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
             uint32_t r[32];
             tmem_ld32x32b_x32(tO + c, r);
             if (has_row && !none) {
-              float4* d = reinterpret_cast<float4*>(part_o + at * HD + c);
 #pragma unroll
-              for (int v = 0; v < 8; ++v)
-                d[v] = make_float4(__uint_as_float(r[4 * v]) * inv, __uint_as_float(r[4 * v + 1]) * inv,
-                                   __uint_as_float(r[4 * v + 2]) * inv, __uint_as_float(r[4 * v + 3]) * inv);
+              for (int v = 0; v < 32; ++v) r[v] = __float_as_uint(__uint_as_float(r[v]) * inv);
+#pragma unroll
+              for (int v = 0; v < 32; v += 8) store32(part_o + at * HD + c + v, r + v, tl.wide);
             }
           }
         }
       } else {
         if (has_row && qr.lse) qr.lse[packed] = lse2 * 0.6931471805599453f;
         const int64_t orow = ky.cross ? w.b * qr.o_str[0] + i * qr.o_str[1] : (int64_t)(w.sp.first + i) * qr.o_str[1];
-        uint4* d = reinterpret_cast<uint4*>(qr.o + (has_row ? orow + h * qr.o_str[2] : 0));
+        __nv_bfloat16* d = qr.o + (has_row ? orow + h * qr.o_str[2] : 0);
 #pragma unroll
         for (int c = 0; c < HD; c += 32) {
           uint32_t r[32];
           if (nt > 0) tmem_ld32x32b_x32(tO + c, r);
           if (has_row) {
+            uint32_t o[16];
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-              auto two = [&](int k) {
-                return none ? 0u : pack_bf16x2(__uint_as_float(r[k]) * inv, __uint_as_float(r[k + 1]) * inv);
-              };
-              d[c / 8 + v] = make_uint4(two(8 * v), two(8 * v + 2), two(8 * v + 4), two(8 * v + 6));
-            }
+            for (int k = 0; k < 16; ++k)
+              o[k] = none ? 0u : pack_bf16x2(__uint_as_float(r[2 * k]) * inv, __uint_as_float(r[2 * k + 1]) * inv);
+            store32(d + c, o, tl.wide);
+            store32(d + c + 16, o + 8, tl.wide);
           }
         }
       }
@@ -1112,6 +1124,8 @@ int launch(const Keys& ky, const Queries& qr, const Shape& sh, void* workspace, 
   tl.tq = BM / qr.group;
   tl.splits = splits(sh);
   tl.even = dealt(sh);
+  tl.wide = ((reinterpret_cast<uintptr_t>(qr.o) | reinterpret_cast<uintptr_t>(workspace)) & 31) == 0 &&
+            (qr.o_str[0] | qr.o_str[1] | qr.o_str[2]) % 16 == 0;
   CUtensorMap tq;
   PageMaps tm;
   int rc;
