@@ -92,6 +92,9 @@ __global__ void __launch_bounds__(THREADS, 2)
   const int item = blockIdx.x / cut.cluster;
   const int G = qr.H / qr.group;
   const int rt0 = item % cut.row_tiles, hk = item / cut.row_tiles % G, b = item / cut.row_tiles / G;
+  // The page table's row comes to L2 while the sequence's length is on its way.
+  if (!ky.cross && threadIdx.x * 32 < ky.max_pages)
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(ky.table + b * ky.table_stride + threadIdx.x * 32));
   const Span sp = span_of(ky, qr, b);
   const Tiling& tl = cut.tl;
   const int ps = tl.ps;
@@ -490,12 +493,22 @@ __global__ void __launch_bounds__(THREADS, 2)
       const uint32_t am = smem_u32(base + 16 * O_PITCH + 32 + r), ao = smem_u32(base + r * O_PITCH + dim);
       float m = -INFINITY, l = 0.f, x = 0.f;
       if (cut.cluster > 1) {
-        for (int c = 0; c < cut.cluster; ++c) m = max_nan(m, cluster_load(am, c));
+        float mc[MAX_CLUSTER], lc[MAX_CLUSTER], xc[MAX_CLUSTER];  // all in flight at once
+#pragma unroll
+        for (int c = 0; c < MAX_CLUSTER; ++c) {
+          const int from = min(c, cut.cluster - 1);
+          mc[c] = cluster_load(am, from);
+          lc[c] = cluster_load(am - 64, from);
+          xc[c] = cluster_load(ao, from);
+        }
+#pragma unroll
+        for (int c = 0; c < MAX_CLUSTER; ++c) m = max_nan(m, mc[c]);
         const float mu = m == -INFINITY ? 0.f : m;
-        for (int c = 0; c < cut.cluster; ++c) {
-          const float wt = exp2f(cluster_load(am, c) - mu);
-          l += wt * cluster_load(am - 64, c);
-          x += wt * cluster_load(ao, c);
+#pragma unroll
+        for (int c = 0; c < MAX_CLUSTER; ++c) {
+          const float wt = c < cut.cluster ? exp2f(mc[c] - mu) : 0.f;
+          l += c < cut.cluster ? wt * lc[c] : 0.f;
+          x += c < cut.cluster ? wt * xc[c] : 0.f;
         }
       } else {
         m = base[16 * O_PITCH + 32 + r];
@@ -530,7 +543,7 @@ __global__ void __launch_bounds__(THREADS, 2)
 // waves of CTAs with about six for a CTA's
 // start and end, half of one CTA's again because sequences differ in length,
 // and four for the join of clusters.
-constexpr int PLACES = 2 * SMS;
+static int places(int cluster) { return cluster <= 2 ? 2 * SMS : cluster == 4 ? 284 : 264; }  // CTAs that run at once
 static Cut cut_of(const Shape& sh, bool kv8) {
   const int bn = kv8 ? 128 : 64;
   Cut c{tiling_of(sh.page_size, bn), 1, 1, (int)((sh.max_new * sh.group + 15) / 16)};
@@ -540,10 +553,10 @@ static Cut cut_of(const Shape& sh, bool kv8) {
   const int64_t n = tiles_of_keys(sh, bn);
   double best = 1e30;
   for (int cluster = 1; cluster <= MAX_CLUSTER; cluster *= 2)
-    for (int outer = 1; outer <= 16 && (cluster == MAX_CLUSTER || outer == 1); ++outer) {
+    for (int outer = 1; outer <= 16; ++outer) {
       if (cluster * outer > 1 && n < (int64_t)cluster * outer * 2) break;
       const double rounds = (double)((n + cluster * outer - 1) / (cluster * outer));
-      const double cost = (double)((items * cluster * outer + PLACES - 1) / PLACES) * (rounds + 6) + 0.5 * rounds +
+      const double cost = (double)((items * cluster * outer + places(cluster) - 1) / places(cluster)) * (rounds + 6) + 0.5 * rounds +
                           (outer > 1 ? 4 : 0);
       if (cost < best) best = cost, c.cluster = cluster, c.outer = outer;
     }
