@@ -527,6 +527,9 @@ _PACK_BATCH = struct.Struct("Qq2Q2iq").pack   # wf_kv_batch
 _PACK2, _PACK3 = struct.Struct("2q").pack, struct.Struct("3q").pack
 
 
+_SCALE = 1.0 / math.sqrt(128)
+
+
 def _st2(t: torch.Tensor) -> tuple:
     """The first two strides; a dim of one element, whose stride torch leaves open, gets 16."""
     s, n = t.stride(), t.shape
@@ -553,17 +556,20 @@ class KVPages:
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None,
                  v_scale: torch.Tensor | None = None) -> None:
-        _check(k.dtype in _PAGE_DTYPES and v.dtype == k.dtype, "KVPages: k and v must both be bf16, uint8 (e4m3) or int8")
-        _check(k.dim() == 4 and v.shape == k.shape and v.device == k.device and k.stride(3) == v.stride(3) == 1,
-               "KVPages: k and v must be [pages, kv_heads, page_size, 128] with contiguous rows, on one device")
-        self.kv_dtype = _PAGE_DTYPES[k.dtype]
-        if self.kv_dtype == L.WF_DTYPE_BF16:
-            _check(k_scale is None and v_scale is None, "KVPages: bf16 pages take no scales")
+        dtype, shape, d = k.dtype, k.shape, k.get_device()
+        if not (dtype in _PAGE_DTYPES and v.dtype is dtype):
+            raise ValueError("KVPages: k and v must both be bf16, uint8 (e4m3) or int8")
+        if not (len(shape) == 4 and v.shape == shape and v.get_device() == d and k.stride()[3] == v.stride()[3] == 1):
+            raise ValueError("KVPages: k and v must be [pages, kv_heads, page_size, 128] with contiguous rows, on one device")
+        self.kv_dtype = _PAGE_DTYPES[dtype]
+        if dtype is torch.bfloat16:
+            if k_scale is not None or v_scale is not None:
+                raise ValueError("KVPages: bf16 pages take no scales")
         else:
             for s in (k_scale, v_scale):
-                _check(s is not None and s.dtype == torch.float32 and s.shape == k.shape[:3] and s.device == k.device
-                       and (s.stride(2) == 1 or s.shape[2] == 1),
-                       "KVPages: 8-bit pages need f32 scales [pages, kv_heads, page_size], contiguous in a page")
+                if not (s is not None and s.dtype is torch.float32 and s.shape == shape[:3] and s.get_device() == d
+                        and (s.stride()[2] == 1 or shape[2] == 1)):
+                    raise ValueError("KVPages: 8-bit pages need f32 scales [pages, kv_heads, page_size], contiguous in a page")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
 
     @classmethod
@@ -578,40 +584,55 @@ class KVPages:
     def _desc(self) -> bytes:
         k, v, ks, vs = self.k, self.v, self.k_scale, self.v_scale
         P, G, ps, D = k.shape
+        (k0, k1, k2, _), (v0, v1, v2, _) = k.stride(), v.stride()
+        if P == 1:  # torch leaves the stride of a dim of one element open
+            k0 = v0 = 16
+        if G == 1:
+            k1 = v1 = 16
+        if ps == 1:
+            k2 = v2 = 16
         if ks is None:
-            return _PACK_PAGES(k.data_ptr(), v.data_ptr(), 0, 0, P, ps, G, D, self.kv_dtype, *_st3(k), *_st3(v),
+            return _PACK_PAGES(k.data_ptr(), v.data_ptr(), 0, 0, P, ps, G, D, self.kv_dtype, k0, k1, k2, v0, v1, v2,
                                0, 0, 0, 0)
         return _PACK_PAGES(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), P, ps, G, D, self.kv_dtype,
-                           *_st3(k), *_st3(v), *_st2(ks), *_st2(vs))
+                           k0, k1, k2, v0, v1, v2, *_st2(ks), *_st2(vs))
 
 
+# The wrappers below are called once a layer for single tokens: the checks read
+# each attribute once and format no message before it is needed.
 def _no_grad(what: str, *ts: torch.Tensor) -> None:
-    _check(not (torch.is_grad_enabled() and any(t.requires_grad for t in ts)),
-           f"{what}: no gradient is computed; call it under torch.no_grad()")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+        raise ValueError(f"{what}: no gradient is computed; call it under torch.no_grad()")
 
 
-def _on(dev: torch.device, fn, *args) -> int:
-    """fn(*args, stream) on ``dev``'s current stream, with ``dev`` the current device."""
+def _on(d: int, fn, *args) -> int:
+    """fn(*args, stream) on device d's current stream, with d the current device."""
     LAUNCHES[0] += 1
-    if dev.index == torch.cuda.current_device():
-        return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
-    with torch.cuda.device(dev):
-        return fn(*args, torch._C._cuda_getCurrentRawStream(dev.index))
+    if d == torch.cuda.current_device():
+        return fn(*args, torch._C._cuda_getCurrentRawStream(d))
+    with torch.cuda.device(d):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(d))
 
 
-def _batch_desc(what: str, table: torch.Tensor, cu: torch.Tensor, lens: torch.Tensor, rows: int, dev) -> bytes:
-    B = lens.shape[0]
-    _check(table.dtype == cu.dtype == lens.dtype == torch.int32 and lens.dim() == cu.dim() == 1 and table.dim() == 2
-           and table.shape[0] == B and table.shape[1] >= 1 and cu.shape[0] == B + 1 and lens.is_contiguous()
-           and cu.is_contiguous() and (table.stride(1) == 1 or table.shape[1] == 1),
-           f"{what}: page_table [B, max_pages], cu_new [B + 1] and seq_lens [B] must be int32 with contiguous rows")
-    _check(table.device == cu.device == lens.device == dev, f"{what}: all tensors must be on one device")
-    return _PACK_BATCH(table.data_ptr(), table.stride(0), cu.data_ptr(), lens.data_ptr(), B, table.shape[1], rows)
+def _batch_desc(what: str, table: torch.Tensor, cu: torch.Tensor, lens: torch.Tensor, rows: int, d: int) -> bytes:
+    i32, size, B = torch.int32, table.shape, lens.shape[0] if lens.dim() == 1 else -1
+    if not (table.dtype is i32 and cu.dtype is i32 and lens.dtype is i32 and len(size) == 2 and size[0] == B
+            and size[1] >= 1 and cu.shape == (B + 1,) and lens.is_contiguous() and cu.is_contiguous()
+            and (table.stride()[1] == 1 or size[1] == 1)):
+        raise ValueError(f"{what}: page_table [B, max_pages], cu_new [B + 1] and seq_lens [B] must be int32 with contiguous rows")
+    if not (table.get_device() == cu.get_device() == lens.get_device() == d):
+        raise ValueError(f"{what}: all tensors must be on one device")
+    return _PACK_BATCH(table.data_ptr(), table.stride()[0], cu.data_ptr(), lens.data_ptr(), B, size[1], rows)
 
 
-def _packed(what: str, t: torch.Tensor, heads: int) -> None:
-    _check(t.dim() == 3 and t.shape[1] == heads and t.shape[2] == 128 and t.dtype == torch.bfloat16
-           and t.stride(2) == 1, f"{what}: packed rows must be bf16 [rows, {heads}, 128] with a contiguous last dim")
+def _packed(what: str, t: torch.Tensor, heads: int, d: int) -> tuple:
+    """Rows of the packed bf16 [rows, heads, 128] on device d, and their strides."""
+    size, st = t.shape, t.stride()
+    if not (len(size) == 3 and size[1] == heads and size[2] == 128 and t.dtype is torch.bfloat16 and st[2] == 1):
+        raise ValueError(f"{what}: packed rows must be bf16 [rows, {heads}, 128] with a contiguous last dim")
+    if t.get_device() != d:
+        raise ValueError(f"{what}: all tensors must be on one device")
+    return size[0], _PACK2(st[0] if size[0] != 1 else 16, st[1] if heads != 1 else 16)
 
 
 def paged_kv_write(pages: KVPages, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor, cu_new: torch.Tensor,
@@ -622,16 +643,16 @@ def paged_kv_write(pages: KVPages, k: torch.Tensor, v: torch.Tensor, page_table:
     seq_lens[b] positions, and position p lies in page page_table[b, p //
     page_size].  All three are int32 on the device, so one captured call serves
     every step.  A slot that two rows land in keeps the later row."""
-    _packed("paged_kv_write", k, pages.k.shape[1])
-    _packed("paged_kv_write", v, pages.k.shape[1])
-    _check(k.shape == v.shape, "paged_kv_write: k and v must have the same number of rows")
+    G, d = pages.k.shape[1], pages.k.get_device()
+    rows, k_st = _packed("paged_kv_write", k, G, d)
+    v_rows, v_st = _packed("paged_kv_write", v, G, d)
+    if rows != v_rows:
+        raise ValueError("paged_kv_write: k and v must have the same number of rows")
     _no_grad("paged_kv_write", k, v)
-    dev = pages.k.device
-    _check(k.device == v.device == dev, "paged_kv_write: all tensors must be on one device")
-    batch = _batch_desc("paged_kv_write", page_table, cu_new, seq_lens, k.shape[0], dev)
+    batch = _batch_desc("paged_kv_write", page_table, cu_new, seq_lens, rows, d)
     _need_cuda(k)
-    L.check(_on(dev, L.lib().wf_paged_kv_write, pages._desc(), batch, k.data_ptr(), v.data_ptr(),
-                _PACK2(*_st2(k)), _PACK2(*_st2(v))), "wf_paged_kv_write")
+    L.check(_on(d, L.lib().wf_paged_kv_write, pages._desc(), batch, k.data_ptr(), v.data_ptr(), k_st, v_st),
+            "wf_paged_kv_write")
 
 
 def paged_kv_read(pages: KVPages, page_table: torch.Tensor, cu_new: torch.Tensor, seq_lens: torch.Tensor,
@@ -641,20 +662,22 @@ def paged_kv_read(pages: KVPages, page_table: torch.Tensor, cu_new: torch.Tensor
     kv_heads, 128] (whole sequences when cu_new is the prefix sum of seq_lens).
     ``rows`` (or the outputs' size) is the packed total; rows behind cu_new[-1]
     are not written."""
-    G = pages.k.shape[1]
-    dev = pages.k.device
+    G, d = pages.k.shape[1], pages.k.get_device()
     _check((out_k is None) == (out_v is None), "paged_kv_read: give both outputs or neither")
     if out_k is None:
         _check(rows is not None and rows >= 0, "paged_kv_read: rows is needed without outputs")
-        out_k, out_v = (torch.empty((rows, G, 128), dtype=torch.bfloat16, device=dev) for _ in range(2))
-    _packed("paged_kv_read", out_k, G)
-    _packed("paged_kv_read", out_v, G)
-    _check(out_k.shape == out_v.shape and (rows is None or rows == out_k.shape[0]) and out_k.device == dev
-           and out_v.device == dev, "paged_kv_read: outputs must both hold `rows` rows on the pages' device")
-    batch = _batch_desc("paged_kv_read", page_table, cu_new, seq_lens, out_k.shape[0], dev)
+        out_k = torch.empty((rows, G, 128), dtype=torch.bfloat16, device=pages.k.device)
+        out_v = torch.empty_like(out_k)
+        k_st = v_st = _PACK2(G * 128, 128)
+    else:
+        k_rows, k_st = _packed("paged_kv_read", out_k, G, d)
+        v_rows, v_st = _packed("paged_kv_read", out_v, G, d)
+        _check(k_rows == v_rows and (rows is None or rows == k_rows), "paged_kv_read: outputs must both hold `rows` rows")
+        rows = k_rows
+    batch = _batch_desc("paged_kv_read", page_table, cu_new, seq_lens, rows, d)
     _need_cuda(out_k)
-    L.check(_on(dev, L.lib().wf_paged_kv_read, pages._desc(), batch, out_k.data_ptr(), out_v.data_ptr(),
-                _PACK2(*_st2(out_k)), _PACK2(*_st2(out_v))), "wf_paged_kv_read")
+    L.check(_on(d, L.lib().wf_paged_kv_read, pages._desc(), batch, out_k.data_ptr(), out_v.data_ptr(), k_st, v_st),
+            "wf_paged_kv_read")
     return out_k, out_v
 
 
@@ -674,30 +697,32 @@ def paged_attention(q: torch.Tensor, pages: KVPages, page_table: torch.Tensor, c
     split of the work only.  Rows behind cu_new[-1] are not written.  With
     ``return_lse`` also the f32 log-sum-exp [rows, H]."""
     _check(q.dim() == 3, "paged_attention: q must be packed rows [rows, H, 128]")
-    rows, H = q.shape[:2]
-    _packed("paged_attention", q, H)
+    H, d = q.shape[1], q.get_device()
+    rows, q_st = _packed("paged_attention", q, H, d)
     _no_grad("paged_attention", q)
-    dev = q.device
-    G, ps = pages.k.shape[1:3]
-    _check(pages.k.device == dev, "paged_attention: all tensors must be on one device")
+    _, G, ps, _ = pages.k.shape
+    if pages.k.get_device() != d:
+        raise ValueError("paged_attention: all tensors must be on one device")
     _check(H % G == 0, "paged_attention: query heads must be a multiple of the K/V heads")
-    batch = _batch_desc("paged_attention", page_table, cu_new, seq_lens, rows, dev)
+    batch = _batch_desc("paged_attention", page_table, cu_new, seq_lens, rows, d)
     if out is None:
-        out = torch.empty((rows, H, 128), dtype=torch.bfloat16, device=dev)
-    _packed("paged_attention", out, H)
-    _check(out.shape == q.shape and out.device == dev, "paged_attention: out must match q")
+        out = q.new_empty((rows, H, 128))
+        o_st = _PACK2(H * 128, 128)
+    else:
+        o_rows, o_st = _packed("paged_attention", out, H, d)
+        _check(o_rows == rows, "paged_attention: out must match q")
     _need_cuda(q)
-    lse = torch.empty((rows, H), dtype=torch.float32, device=dev) if return_lse else None
+    lse = q.new_empty((rows, H), dtype=torch.float32) if return_lse else None
     max_new = rows if max_new is None else int(max_new)
     max_len = page_table.shape[1] * ps if max_len is None else int(max_len)
     desc = pages._desc()
     lib = L.lib()
     need = lib.wf_paged_attn_workspace(desc, batch, H, window, sink, max_new, max_len)
-    ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need > 0 else None
-    scale = 1.0 / math.sqrt(128) if softmax_scale is None else float(softmax_scale)
-    L.check(_on(dev, lib.wf_paged_attn, desc, batch, q.data_ptr(), _PACK2(*_st2(q)), out.data_ptr(),
-                _PACK2(*_st2(out)), lse.data_ptr() if lse is not None else None, H, block, window, sink,
-                max_new, max_len, scale, ws.data_ptr() if ws is not None else None, need), "wf_paged_attn")
+    ws = q.new_empty((need,), dtype=torch.uint8) if need > 0 else None
+    scale = _SCALE if softmax_scale is None else float(softmax_scale)
+    L.check(_on(d, lib.wf_paged_attn, desc, batch, q.data_ptr(), q_st, out.data_ptr(), o_st,
+                lse.data_ptr() if lse is not None else None, H, block, window, sink, max_new, max_len, scale,
+                ws.data_ptr() if ws is not None else None, need), "wf_paged_attn")
     return (out, lse) if return_lse else out
 
 
@@ -710,34 +735,36 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, kv_len
     the keys below kv_lens[n] (int32 [N]) that key_mask [N, Lk] (bool) keeps;
     what the other keys hold does not matter.  Queries left without keys give
     zeros.  With ``return_lse`` also the f32 log-sum-exp [B, Lq, H]."""
-    _check(q.dim() == 4 and k.dim() == 4 and v.shape == k.shape
-           and q.dtype == k.dtype == v.dtype == torch.bfloat16 and q.shape[3] == k.shape[3]
-           and q.stride(3) == k.stride(3) == v.stride(3) == 1,
-           "cross_attention: q [B, Lq, H, 128] and k, v [N, Lk, kv_heads, 128] must be bf16 with contiguous last dims")
+    size, bf = k.shape, torch.bfloat16
+    if not (q.dim() == 4 and len(size) == 4 and v.shape == size and q.dtype is bf and k.dtype is bf and v.dtype is bf
+            and q.shape[3] == size[3] and q.stride()[3] == k.stride()[3] == v.stride()[3] == 1):
+        raise ValueError("cross_attention: q [B, Lq, H, 128] and k, v [N, Lk, kv_heads, 128] must be bf16 with contiguous "
+                         "last dims")
     B, Lq, H, D = q.shape
-    N, Lk, G, _ = k.shape
-    dev = q.device
+    N, Lk, G, _ = size
+    d = q.get_device()
     _check(N >= 1 and Lk >= 1 and G >= 1 and H % G == 0,
            "cross_attention: query heads must be a multiple of the K/V heads, states not empty")
-    _check(kv_index is not None or N in (1, B), "cross_attention: N states for B entries need kv_index")
+    _check(kv_index is not None or N == 1 or N == B, "cross_attention: N states for B entries need kv_index")
     for t, n in ((kv_index, B), (kv_lens, N)):
-        _check(t is None or (t.dtype == torch.int32 and t.shape == (n,) and t.is_contiguous() and t.device == dev),
+        _check(t is None or (t.dtype is torch.int32 and t.shape == (n,) and t.is_contiguous() and t.get_device() == d),
                "cross_attention: kv_index [B] and kv_lens [N] must be contiguous int32 on q's device")
-    _check(key_mask is None or (key_mask.dtype == torch.bool and key_mask.shape == (N, Lk) and key_mask.device == dev
-                                and (key_mask.stride(1) == 1 or Lk == 1)),
+    _check(key_mask is None or (key_mask.dtype is torch.bool and key_mask.shape == (N, Lk) and key_mask.get_device() == d
+                                and (key_mask.stride()[1] == 1 or Lk == 1)),
            "cross_attention: key_mask must be bool [N, Lk] with contiguous rows on q's device")
     _no_grad("cross_attention", q, k, v)
     if out is None:
-        out = torch.empty((B, Lq, H, D), dtype=torch.bfloat16, device=dev)
-    _check(out.shape == q.shape and out.dtype == torch.bfloat16 and out.stride(3) == 1 and out.device == dev
-           and k.device == dev and v.device == dev, "cross_attention: out must match q, all tensors on one device")
+        out = q.new_empty((B, Lq, H, D))
+    if not (out.shape == q.shape and out.dtype is bf and out.stride()[3] == 1
+            and out.get_device() == k.get_device() == v.get_device() == d):
+        raise ValueError("cross_attention: out must match q, all tensors on one device")
     _need_cuda(q)
-    lse = torch.empty((B, Lq, H), dtype=torch.float32, device=dev) if return_lse else None
+    lse = q.new_empty((B, Lq, H), dtype=torch.float32) if return_lse else None
     lib = L.lib()
     need = lib.wf_cross_attn_workspace(B, Lq, N, Lk, H, G)
-    ws = torch.empty((need,), dtype=torch.uint8, device=dev) if need > 0 else None
+    ws = q.new_empty((need,), dtype=torch.uint8) if need > 0 else None
     scale = 1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale)
-    L.check(_on(dev, lib.wf_cross_attn, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+    L.check(_on(d, lib.wf_cross_attn, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
                 lse.data_ptr() if lse is not None else None, B, Lq, N, Lk, H, G, D, _PACK3(*_st3(q)),
                 _PACK3(*_st3(k)), _PACK3(*_st3(v)), _PACK3(*_st3(out)),
                 kv_index.data_ptr() if kv_index is not None else None,
