@@ -78,6 +78,24 @@ def sdpa_elsewhere(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.T
     return _torch_sdpa(q, k, v)
 
 
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_index: torch.Tensor,
+                    kv_lens: torch.Tensor | None = None) -> torch.Tensor:
+    """Cross-attention of stages that follow different texts: stage s of q [S, T,
+    H, D] attends to the first kv_lens[n] (int32 [N]; all of them without it) of
+    the states k, v [N, L, H, D] at n = kv_index[s] (int32 [S]).  wf_b200 reads
+    them in place (kernels.cross_attention); torch_sdpa gathers and masks them.
+    A text of no tokens adds nothing: its stages get zeros."""
+    if _WAVE_STATE["attn"] == "wf_b200":
+        return kernels.cross_attention(q.detach(), k, v, kv_lens=kv_lens, kv_index=kv_index)  # inference only
+    at = kv_index.long()
+    mask = None
+    if kv_lens is not None:
+        mask = (torch.arange(k.shape[1], device=q.device) < kv_lens[at][:, None])[:, None, None]
+    o = torch.nn.functional.scaled_dot_product_attention(q.transpose(1, 2), k[at].transpose(1, 2), v[at].transpose(1, 2),
+                                                         attn_mask=mask).transpose(1, 2)
+    return o if kv_lens is None else torch.where((kv_lens[at] > 0)[:, None, None, None], o, o.new_zeros(()))
+
+
 def set_attention_timer(sink: list | None) -> None:
     """When ``sink`` is a list, every dispatched attention appends
     (flops, start_event, end_event, algorithmic_bytes) recorded on the current stream."""

@@ -32,7 +32,7 @@ import torch.nn.functional as F
 
 from waveforcing_b200 import _lib as L
 from waveforcing_b200 import kernels
-from waveforcing_b200.runtime.backend import dispatch_attention, sdpa_elsewhere
+from waveforcing_b200.runtime.backend import cross_attention, dispatch_attention, sdpa_elsewhere
 
 PRESETS = {
     "1.3b": dict(dim=1536, heads=12, layers=30, ffn=8960),
@@ -174,6 +174,7 @@ class StageTask:
     # only the task's per-layer K/V (published through ``exch``) are used, not
     # its flow output (the store stage: the engine keeps its input latent)
     kv_only: bool = False
+    text: int = 0  # which of set_text's texts the chunk follows
 
 
 class WanDiT(nn.Module):
@@ -189,6 +190,8 @@ class WanDiT(nn.Module):
         self.head_norm_mod = nn.Parameter(torch.randn(1, 2, d) / d**0.5)
         self.head = nn.Linear(d, cfg.out_ch * math.prod(cfg.patch))
         self._cross_kv = None
+        self._texts = None  # several texts: (their number, int32 lengths or None)
+        self._text_indices: dict = {}
 
     @classmethod
     def random(cls, cfg: DiTConfig, device, dtype=torch.bfloat16, seed: int = 0) -> "WanDiT":
@@ -204,17 +207,42 @@ class WanDiT(nn.Module):
 
     # ------------------------------------------------------------ conditioning
     @torch.no_grad()
-    def set_text(self, text: torch.Tensor) -> None:
+    def set_text(self, text: torch.Tensor, lens: list[int] | None = None) -> None:
         """Embed [text_len, text_dim] once and cache every layer's cross K/V
-        (the crossattn_cache of causal_model.py / model.py:174-186)."""
+        (the crossattn_cache of causal_model.py / model.py:174-186).
+
+        Several texts [N, text_len, text_dim] may be given, padded to one
+        length, with the ``lens`` of each: a task follows the text that its
+        ``text`` names, and what lies behind a text's length is not attended."""
         cfg = self.cfg
-        ctx = self.text_embedding(text.to(self.patch_embedding.weight.dtype))
+        if text.dim() not in (2, 3) or (text.dim() == 2 and lens is not None):
+            raise ValueError("set_text: one text [text_len, text_dim], or [N, text_len, text_dim] with N lengths")
+        N = 1 if text.dim() == 2 else text.shape[0]
+        if lens is not None and (len(lens) != N or not all(0 <= n <= text.shape[1] for n in lens)):
+            raise ValueError(f"set_text: {N} lengths of 0 to {text.shape[1]} are needed")
+        ctx = self.text_embedding(text.reshape(-1, text.shape[-1]).to(self.patch_embedding.weight.dtype))
         kv = []
         for b in self.blocks:
-            k = b.cross_attn.norm_k(_lin(b.cross_attn.k, ctx)).view(1, -1, cfg.heads, cfg.head_dim)
-            v = _lin(b.cross_attn.v, ctx).view(1, -1, cfg.heads, cfg.head_dim)
+            k = b.cross_attn.norm_k(_lin(b.cross_attn.k, ctx)).view(N, -1, cfg.heads, cfg.head_dim)
+            v = _lin(b.cross_attn.v, ctx).view(N, -1, cfg.heads, cfg.head_dim)
             kv.append((k.contiguous(), v.contiguous()))
         self._cross_kv = kv
+        self._texts = None
+        if text.dim() == 3:
+            self._texts = (N, None if lens is None else torch.tensor(lens, dtype=torch.int32, device=ctx.device))
+
+    def _text_index(self, tasks: list, dev) -> torch.Tensor | None:
+        """The tasks' texts as an int32 device tensor (kept: a run has few
+        different lists); None when there is one text for all."""
+        texts = tuple(t.text for t in tasks)
+        if not all(0 <= n < (self._texts[0] if self._texts else 1) for n in texts):
+            raise ValueError(f"forward_stages: texts {texts} name one that set_text was not given")
+        if self._texts is None:
+            return None
+        got = self._text_indices.get((texts, dev))
+        if got is None:
+            got = self._text_indices[(texts, dev)] = torch.tensor(texts, dtype=torch.int32, device=dev)
+        return got
 
     def time_mod(self, timestep: float, device):
         """Per-stage modulation inputs: e [6, dim] f32 and e_head [2, dim] f32.
@@ -301,6 +329,7 @@ class WanDiT(nn.Module):
         H, D, dim = cfg.heads, cfg.head_dim, cfg.dim
         order = sorted(range(S), key=lambda i: -tasks[i].stage)  # publish before consume
         keep = [i for i in range(S) if not tasks[i].kv_only]  # tasks whose flow output is returned
+        text_index = self._text_index(tasks, dev)
         x = torch.cat([self.patchify(t.latent.to(dt)) for t in tasks], 0)
         x = _lin(self.patch_embedding, x)  # [S*T, dim]
         mods, heads_e = [], []
@@ -437,8 +466,9 @@ class WanDiT(nn.Module):
                                pending[1].index_select(0, rows).contiguous())
                 heads_e = [heads_e[i] for i in keep]
                 S = len(keep)
+                text_index = self._text_index([tasks[i] for i in keep], dev)
             y = _lin(b.self_attn.o, o.view(S * T, dim))
-            # cross-attention: all stages share the text K/V -> one call
+            # cross-attention: one call for all stages, of one text or of several
             if fused and w8a8_channel(b.cross_attn.q):
                 xq, xsc = kernels.gate_residual_then(xs, y, e_all[:, 2], T, quant=True,
                                                      qtype=b.cross_attn.q.qtype)
@@ -449,8 +479,11 @@ class WanDiT(nn.Module):
             qc = (kernels.rms_norm(qc, b.cross_attn.norm_q.weight, eps) if fused
                   else b.cross_attn.norm_q(qc)).view(1, S * T, H, D)
             kc, vc = self._cross_kv[li]
-            oc = sdpa_elsewhere(qc, kc, vc)
-            yc = _lin(b.cross_attn.o, oc.view(S * T, dim))
+            if text_index is None:
+                oc = sdpa_elsewhere(qc, kc, vc)
+            else:
+                oc = cross_attention(qc.view(S, T, H, D), kc, vc, text_index, self._texts[1])
+            yc = _lin(b.cross_attn.o, oc.reshape(S * T, dim))
             fi, fo = b.ffn.fc_in, b.ffn.fc_out
             if fused and w8a8_channel(fi) and getattr(fo, "granularity", None) == "channel" and hasattr(
                     fo, "forward_gelu_input"):

@@ -38,6 +38,7 @@ class EngineConfig:
     context_noise: float = 0.0
     seed: int = 0
     timeout_s: float = 60.0
+    texts: tuple = ()  # which of the model's texts each chunk follows; the last one from then on
 
     @property
     def rf_step(self) -> int:
@@ -46,6 +47,9 @@ class EngineConfig:
     @property
     def num_blocks(self) -> int:
         return self.num_frames // self.npb
+
+    def text_of(self, chunk: int) -> int:
+        return self.texts[min(chunk, len(self.texts) - 1)] if self.texts else 0
 
 
 # Relative attention+linear cost of each stage in steady state (K/V context in
@@ -221,14 +225,16 @@ class WavefrontEngine:
                                                     self._rope, None if slot_sink_given else store_slot,
                                                     rope_tab_fn=self._rope_tab)
                 slot_sink_given = True
-                tasks.append(StageTask(self.inputs[s], self.fm.timestep(cfg.steps[s]), c * cfg.npb, s, exch))
+                tasks.append(StageTask(self.inputs[s], self.fm.timestep(cfg.steps[s]), c * cfg.npb, s, exch,
+                                        text=cfg.text_of(c)))
             elif s == self.store and store_active:
                 c = t - self.store
                 exch = self.xport.make_store_exch(self.clean, store_kv, c, act, t, self._rope,
                                                   rope_tab_fn=self._rope_tab)
                 # the store's flow output is never used (its input chunk is the final latent):
                 # only its K/V are needed, so its last layer stops after the publish
-                tasks.append(StageTask(self.inputs[s], cfg.context_noise, c * cfg.npb, s, exch, kv_only=True))
+                tasks.append(StageTask(self.inputs[s], cfg.context_noise, c * cfg.npb, s, exch, kv_only=True,
+                                        text=cfg.text_of(c)))
         # no publish of this tick may land in a slab generation that a remote
         # consumer is still reading (it read that generation two ticks ago)
         self.xport.acquire_slots(t)
