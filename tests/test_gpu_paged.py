@@ -459,3 +459,129 @@ def test_log_sum_exp_joins_two_halves_of_a_context():
     mag, _, _ = O.paged_attention(q.cpu(), pool.val[0], pool.val[1].abs(), pool.table, cu, pool.lens, 0, 0, 0, SCALE)
     assert ((o - whole.float()).abs().double().cpu() <= (4 * 2 ** -8 + 2 * 5e-4 + 4e-4) * mag).all()
     healthy()
+
+
+LONG = [  # lens, new, H, G, page, block: one sequence's items dealt out in parts, or several sequences' keys split
+    ([2500], [300], 12, 12, 64, 1),      # 24 items: all in parts
+    ([2200], [600], 50, 50, 128, 0),     # 150 items: a round of whole ones, two in parts
+    ([3301], [200], 4, 2, 48, 100),      # pages that do not divide a tile
+    ([5000, 3000], [20, 17], 4, 2, 16, 1),
+    ([4100, 1, 2050], [40, 1, 3], 2, 2, 128, 0),
+    ([3300], [260], 2, 1, 1560, 390),    # tiles across the ends of large pages
+    ([1700], [150], 3, 3, 200, 50),
+]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "e4m3", "s8"])
+@pytest.mark.parametrize("case", LONG, ids=lambda c: f"len{c[0]}new{c[1]}h{c[2]}p{c[4]}")
+def test_attention_in_parts(case, dtype):
+    lens, new, H, G, ps, block = case
+    pool = Pool(dtype, lens, G, ps, seed=len(lens) + H)
+    check_attention(pool, new, H, block, hints=(max(new), max(lens)))
+    check_attention(pool, new, H, block, window=700, sink=130, tail=1)
+    healthy()
+
+
+@pytest.mark.parametrize("dtype", [E4, S8], ids=["e4m3", "s8"])
+def test_scales_with_strides_of_their_own(dtype):
+    pool = Pool(dtype, [400, 90], 2, 64, seed=15)
+    cu, plan = pool.plan([150, 1])
+    p = pool.pages
+    wide = [torch.full((pool.P, 3, 67), float("nan"), device=DEV) for _ in range(2)]
+    for w, s in zip(wide, (p.k_scale, p.v_scale)):
+        w[:, :2, 1:65] = s
+    odd = K().KVPages(p.k, p.v, wide[0][:, :2, 1:65], wide[1][:, :2, 1:65])
+    for rows, block in ((151, 0), (151, 1)):
+        q = torch.randn((rows, 4, 128), device=DEV).to(BF)
+        assert torch.equal(K().paged_attention(q, p, *plan, block=block), K().paged_attention(q, odd, *plan, block=block))
+    cu1, plan1 = pool.plan([1, 1])
+    q = torch.randn((2, 4, 128), device=DEV).to(BF)
+    assert torch.equal(K().paged_attention(q, p, *plan1, max_new=1), K().paged_attention(q, odd, *plan1, max_new=1))
+    k = torch.randn((151, 2, 128), device=DEV).to(BF)
+    for pages in (p, odd):
+        K().paged_kv_write(pages, k, k, *plan)
+    for a, b in zip(K().paged_kv_read(p, *plan, rows=151), K().paged_kv_read(odd, *plan, rows=151)):
+        assert torch.equal(a, b)
+    # what lies beside the scales is left alone
+    assert wide[0][:, 2].isnan().all() and wide[0][:, :, 0].isnan().all() and wide[0][:, :, 65:].isnan().all()
+    healthy()
+
+
+@pytest.mark.parametrize("dtype", [BF, E4], ids=["bf16", "e4m3"])
+def test_pools_of_more_than_2_to_the_31_elements(dtype):
+    """Page offsets in 64 bits: the same rows through the first and the last pages of a large pool."""
+    ps, G = 64, 2
+    P = 2 ** 31 // (ps * G * 128) + 40
+    kv = [torch.empty((P, G, ps, 128), dtype=dtype, device=DEV) for _ in range(2)]
+    pages = K().KVPages(*kv, *([] if dtype == BF else [torch.empty((P, G, ps), device=DEV) for _ in range(2)]))
+    t = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    cu, lens = t([0, 300]), t([300])
+    k, v = (torch.randn((300, G, 128), device=DEV).to(BF) for _ in range(2))
+    q = torch.randn((300, 4, 128), device=DEV).to(BF)
+    got = []
+    for table in ([[0, 1, 2, 3, 4]], [[P - 1, P - 3, P - 5, 2, P - 2]]):
+        K().paged_kv_write(pages, k, v, t(table), cu, lens)
+        got.append([*K().paged_kv_read(pages, t(table), cu, lens, rows=300),
+                    K().paged_attention(q, pages, t(table), cu, lens, block=1),
+                    K().paged_attention(q[-2:], pages, t(table), t([0, 2]), lens, block=1)])
+    for a, b in zip(*got):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
+    healthy()
+
+
+def test_two_graphs_replayed_at_once_keep_their_workspaces():
+    pool = Pool(BF, [4000, 2500], 2, 64, seed=16)
+    cu, plan = pool.plan([1, 1])
+    q = [torch.randn((2, 2, 128), device=DEV).to(BF) for _ in range(2)]
+    q += [torch.randn((40, 2, 128), device=DEV).to(BF) for _ in range(2)]
+    long = pool.plan([20, 20])[1]
+    call = lambda x: K().paged_attention(x, pool.pages, *(plan if len(x) == 2 else long),  # noqa: E731
+                                         max_new=len(x) // 2, max_len=4000, block=1)
+    want = [call(x) for x in q]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for x in q:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(call(x))
+    streams = [torch.cuda.Stream() for _ in q]
+    for _ in range(10):
+        for o in outs:
+            o.zero_()
+        for s, g in zip(streams, graphs):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    healthy()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "e4m3", "s8"])
+def test_write_and_read_of_many_heads(dtype):
+    """Enough rows that a block walks several groups of heads, the last of them not full."""
+    rows, G, ps = 4800, 37, 64
+    pages = K().KVPages.empty(rows // ps + 1, G, ps, dtype, DEV)
+    t = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    plan = (t([list(range(rows // ps, -1, -1))]), t([0, rows]), t([rows + 5]))
+    x = [torch.randn((rows, G, 128), generator=torch.Generator().manual_seed(i)).to(BF) for i in range(2)]
+    K().paged_kv_write(pages, x[0].to(DEV), x[1].to(DEV), *plan)
+    for a, b in zip(K().paged_kv_read(pages, *plan, rows=rows), x):
+        if dtype == BF:
+            assert torch.equal(a.cpu(), b)
+            continue
+        codes, scale = O.quant_rows(b, dtype)
+        want = codes * scale[..., None]
+        assert ((a.double().cpu() - want).abs() <= (2 ** -8 + 2 ** -23) * want.abs()).all()
+    healthy()
+
+
+def test_cross_attention_into_rows_that_are_not_32_byte_aligned():
+    """Outputs whose rows start on 16-byte boundaries only."""
+    q = torch.randn((2, 200, 3, 128), device=DEV).to(BF)
+    k = torch.randn((2, 300, 3, 128), device=DEV).to(BF)
+    want = K().cross_attention(q, k, k)
+    room = torch.full((2, 200, 3, 136), 7.0, device=DEV, dtype=BF)
+    K().cross_attention(q, k, k, out=room[..., 8:])
+    assert torch.equal(room[..., 8:], want) and (room[..., :8] == 7.0).all()
+    healthy()

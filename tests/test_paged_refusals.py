@@ -169,6 +169,17 @@ def test_abi_attention_refusals(args):
     assert rc == L.WF_ERR_INVALID_ARG and L.last_error()
 
 
+@pytest.mark.parametrize("at,short", [(None, 0), (264, 0), (256, 1)], ids=["none", "not aligned", "too small"])
+def test_abi_attention_workspace(at, short):
+    """A call whose keys are split needs the workspace that it asked for."""
+    b = batch(seqs=1, rows=1, max_pages=4096)
+    need = L.lib().wf_paged_attn_workspace(desc(), b, 4, 0, 0, 1, 60000)
+    assert need > 0
+    rc = L.lib().wf_paged_attn(desc(), b, 256, L.i64_array((512, 128)), 256, L.i64_array((512, 128)), None, 4, 0, 0, 0, 1,
+                               60000, 0.1, at, need - short, None)
+    assert rc == L.WF_ERR_INVALID_ARG and "workspace" in L.last_error()
+
+
 @pytest.mark.parametrize("args,code", [
     (dict(q=None), 1), (dict(k=None), 1), (dict(v=264), 1), (dict(o=None), 1), (dict(D=64), 2), (dict(H=5), 1),
     (dict(kv=0), 1), (dict(states=3), 1), (dict(states=0), 1), (dict(Lk=0), 1), (dict(batch=-1), 1),
