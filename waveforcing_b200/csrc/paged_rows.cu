@@ -22,6 +22,7 @@
 // largest power of two so far; Q rows are scaled by powers of two to f16.
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "paged_attn.cuh"
@@ -30,14 +31,17 @@ namespace wfk {
 namespace paged {
 namespace rows {
 
-constexpr int WARPS = 4, THREADS = (WARPS + 1) * 32, ST = 3, MAX_CLUSTER = 8;
+constexpr int WARPS = 4, THREADS = (WARPS + 1) * 32;
 constexpr int STAGE = 32768;               // a tile's K and V rows
 constexpr int MAX_BN = 128;
 constexpr int META = 2 * MAX_BN * 4 + 32;  // scales of K and V, live keys, whether every row sees all, the tile
 constexpr int O_PITCH = 132;               // floats of a row of partial sums, off the banks of the next
-constexpr int PART = 16 * (O_PITCH + 3) * 4;  // a warp's sums: O, m, l, and the CTA's m
-constexpr int SMEM = 1024 + ST * (STAGE + META + 16) + 16;
-static_assert(WARPS * PART <= ST * STAGE, "the sums lie over the ring");
+constexpr int HEAD = 4096;                 // barriers, items and META of up to three stages
+constexpr int smem_of(int stages, int height) {
+  return 1024 + HEAD + stages * STAGE + WARPS * height * (O_PITCH + 2) * 4;
+}
+constexpr int SMEM = 115712;  // two CTAs to an SM
+static_assert(smem_of(3, 5) <= SMEM && smem_of(2, 16) <= SMEM);
 
 // Key of column n of an 8-key score tile.
 __device__ __forceinline__ int key_of(int n) { return n ^ ((n & 1) << 2); }
@@ -63,23 +67,87 @@ __device__ __forceinline__ uint32_t codes_f16(uint32_t two) {
   }
   return r;
 }
-__device__ __forceinline__ float cluster_load(uint32_t saddr, uint32_t rank) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(saddr, rank)) : "memory");
-  return v;
-}
-
+// How the work is shared: all tiles of all items (a sequence's K/V head and
+// `height` of its rows) lie in a line, of which each CTA takes an equal stretch;
+// with `whole` a CTA takes whole items.
 struct Cut {
   Tiling tl;
-  int cluster, outer;  // CTAs of a cluster; clusters to a tile of rows (joined through the workspace)
-  int row_tiles;       // tiles of rows that the grid has to a sequence and K/V head
+  int ctas, height, whole, stages;
 };
+struct Item {
+  int b, hk, rt, n;  // sequence, K/V head, tile of rows; items of the sequence
+  int t, i0, i1;     // its tiles in the line; this CTA's
+  Span sp;
+  Range rg;
+};
+
+template <int BN>
+__device__ __forceinline__ void open_sequence(Item& it, const Keys& ky, const Queries& qr, const Cut& cut, int b) {
+  it.b = b;
+  it.sp = span_of(ky, qr, b);
+  it.n = it.sp.n > 0 ? (it.sp.n * qr.group + cut.height - 1) / cut.height * (qr.H / qr.group) : 0;
+  if (it.n == 0) return;
+  it.rg = range_of<BN>(qr, it.sp, cut.tl, 0, it.sp.n - 1);
+  it.t = cut.whole ? 1 : max(it.rg.n, 1);  // an item without keys still writes its rows
+}
+
+// First place of CTA c's stretch.
+__device__ __forceinline__ long long stretch(long long len, int c, int ctas) { return len * c / ctas; }
+// Where a stretch begins: the line's length, the first place, its sequence and
+// that one's first place; found by each warp for itself.
+struct Spot {
+  long long len, pos, first;
+  int b;
+};
+template <int BN>
+__device__ __forceinline__ Spot find_spot(const Keys& ky, const Queries& qr, const Cut& cut, int cta) {
+  const int lane = threadIdx.x & 31, per = (qr.seqs + 31) / 32, b0 = lane * per, b1 = min(b0 + per, qr.seqs);
+  auto length = [&](int b) -> long long {
+    Item it;
+    open_sequence<BN>(it, ky, qr, cut, b);
+    return it.n > 0 ? (long long)it.t * it.n : 0;
+  };
+  long long mine = 0;
+  for (int b = b0; b < b1; ++b) mine += length(b);
+  long long after = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const long long x = __shfl_up_sync(0xffffffffu, after, o);
+    if (lane >= o) after += x;
+  }
+  Spot s;
+  s.len = __shfl_sync(0xffffffffu, after, 31);
+  s.pos = stretch(s.len, cta, cut.ctas);
+  s.first = after - mine;
+  s.b = b0;
+  const bool here = s.pos >= s.first && s.pos < after;
+  if (here && per > 1)
+    for (long long n; s.pos >= s.first + (n = length(s.b)); ++s.b) s.first += n;
+  const int from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;  // (-1: the line is empty)
+  s.first = __shfl_sync(0xffffffffu, s.first, max(from, 0));
+  s.b = __shfl_sync(0xffffffffu, s.b, max(from, 0));
+  return s;
+}
+
+// What the join has to know of an item whose first part is a CTA's last one.
+struct Split {
+  int b, hk, rt, parts;  // 0 parts: the CTA has none
+};
+
+// Row r of an item's rows (tokens x the heads that share the K/V head), one dim.
+__device__ __forceinline__ void store_row(const Keys& ky, const Queries& qr, int b, int first, int hk, int r, int dim,
+                                          float x, float lse2) {
+  const int i = r / qr.group, h = hk * qr.group + r - i * qr.group;
+  const int64_t orow = ky.cross ? b * qr.o_str[0] + i * qr.o_str[1] : (int64_t)(first + i) * qr.o_str[1];
+  qr.o[orow + h * qr.o_str[2] + dim] = __float2bfloat16_rn(x);
+  if (qr.lse && dim == 0) qr.lse[(int64_t)(first + i) * qr.H + h] = lse2 * 0.6931471805599453f;
+}
 
 template <int DT>
 __global__ void __launch_bounds__(THREADS, 2)
     rows_kernel(const __grid_constant__ PageMaps tm,
                 const __grid_constant__ Keys ky, const __grid_constant__ Queries qr, const __grid_constant__ Cut cut,
-                float* part_o, float* part_l) {
+                float* part_o, float* part_l, Split* split) {
   constexpr bool KV8 = DT != WF_DTYPE_BF16;
   constexpr int BN = KV8 ? 128 : 64;       // keys of a tile
   constexpr int KC = BN / WARPS;           // keys of a warp
@@ -88,21 +156,18 @@ __global__ void __launch_bounds__(THREADS, 2)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const uint32_t rank = cut.cluster > 1 ? cluster_ctarank() : 0;
-  const int item = blockIdx.x / cut.cluster;
-  const int G = qr.H / qr.group;
-  const int rt0 = item % cut.row_tiles, hk = item / cut.row_tiles % G, b = item / cut.row_tiles / G;
-  // The page table's row comes to L2 while the sequence's length is on its way.
-  if (!ky.cross && threadIdx.x * 32 < ky.max_pages)
-    asm volatile("prefetch.global.L2 [%0];" ::"l"(ky.table + b * ky.table_stride + threadIdx.x * 32));
-  const Span sp = span_of(ky, qr, b);
   const Tiling& tl = cut.tl;
-  const int ps = tl.ps;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + ST * (STAGE + META));
-  uint64_t* empty = full + ST;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + ST);
+  const int ps = tl.ps, G = qr.H / qr.group;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem);
+  uint64_t* empty = full + 3;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(empty + 3);
+  Item& it = reinterpret_cast<Item*>(smem + 64)[warp];  // the warp's; registers are short
+  static_assert(64 + (WARPS + 1) * sizeof(Item) <= HEAD - 3 * META);
+  uint8_t* meta = smem + HEAD - 3 * META;
+  uint8_t* ring = smem + HEAD;
+  float* sums = reinterpret_cast<float*>(ring + cut.stages * STAGE);  // [WARPS] of O [height][O_PITCH], m [height], l [height]
   if (threadIdx.x == 0) {
-    for (int k = 0; k < ST; ++k) {
+    for (int k = 0; k < cut.stages; ++k) {
       mbar_init(&full[k], KV8 ? 33 : 1);
       mbar_init(&empty[k], WARPS);
     }
@@ -111,38 +176,78 @@ __global__ void __launch_bounds__(THREADS, 2)
     tma_prefetch_desc(&tm.k_tile);
     tma_prefetch_desc(&tm.v_tile);
   }
+  const int cta = blockIdx.x;
+  const Spot spot = find_spot<BN>(ky, qr, cut, cta);
+  const long long len = spot.len;
+  long long left = stretch(len, cta + 1, cut.ctas) - stretch(len, cta, cut.ctas);
   __syncthreads();
-  uint32_t done = 0;  // tiles through the ring
-
-  for (int rt = rt0; rt * 16 < sp.n * qr.group; rt += cut.row_tiles) {
-    const int i0 = rt * 16 / qr.group, i1 = min((rt * 16 + 15) / qr.group, sp.n - 1);
-    const Range rg = range_of<BN>(qr, sp, tl, i0, i1);
-    const int n_rows = min(16, sp.n * qr.group - rt * 16);
-    const int parts = cut.cluster * cut.outer, part = blockIdx.y * cut.cluster + rank;
-    const int p0 = (int)((long long)rg.n * part / parts), p1 = (int)((long long)rg.n * (part + 1) / parts);
-    if (warp == WARPS) {
-      // ---------------------------------------------------------- producer
-      // A tile's page ids (a lane to a box) are fetched a tile ahead; scales go
-      // to shared memory by cp.async: no latency lies between the waits.
-      constexpr int KL = BN / 32;
-      int sub[KL], at_row[KL];  // of key c * 32 + lane: its box, and the row in it
+  asm volatile("griddepcontrol.launch_dependents;\n" ::: "memory");  // the join may take its place (it waits for the end)
+  if (left == 0) {  // (the whole CTA)
+    if (!cut.whole && threadIdx.x < 16) part_l[cta * 32 + threadIdx.x] = -INFINITY;
+    if (!cut.whole && threadIdx.x == 0) split[cta].parts = 0;
+    return;
+  }
+  int st = 0;             // the ring's stage, and how often it has come round
+  uint32_t turn = 0;
+  auto next_stage = [&]() {
+    if (++st == cut.stages) st = 0, ++turn;
+  };
+  // The CTA's items in turn, each with the tiles that it has to do.
+  int item, i;
+  {
+    open_sequence<BN>(it, ky, qr, cut, spot.b);
+    const long long off = spot.pos - spot.first;
+    item = (int)(off / it.t);
+    i = (int)(off - (long long)item * it.t);
+  }
+  auto open_item = [&]() {
+    it.rt = item / G;
+    it.hk = item - it.rt * G;
+    const int n = (int)min((long long)(it.t - i), left);
+    it.i0 = i, it.i1 = i + n;
+    left -= n;
+    __syncwarp();
+  };
+  auto next_item = [&]() -> bool {
+    if (left == 0) return false;
+    __syncwarp();  // (all lanes write the item, the same)
+    i = 0;
+    if (++item == it.n) {
+      item = 0;
+      do open_sequence<BN>(it, ky, qr, cut, it.b + 1);
+      while (it.n == 0);
+    }
+    return true;
+  };
+  if (warp == WARPS) {
+    // ---------------------------------------------------------- producer
+    // A tile's page ids (a lane to a box) are fetched a tile ahead; scales go
+    // to shared memory by cp.async: no latency lies between the waits.
+    constexpr int KL = BN / 32;
+    int sub[KL], at_row[KL];  // of key c * 32 + lane: its box, and the row in it
 #pragma unroll
-      for (int c = 0; c < KL; ++c) {
-        const int r = c * 32 + lane;
-        sub[c] = min(r / tl.rows, tl.boxes);  // behind the last box: a hole
-        at_row[c] = r - sub[c] * tl.rows;
-      }
+    for (int c = 0; c < KL; ++c) {
+      const int r = c * 32 + lane;
+      sub[c] = min(r / tl.rows, tl.boxes);  // behind the last box: a hole
+      at_row[c] = r - sub[c] * tl.rows;
+    }
+    bool ok = true;
+    do {
+      open_item();
+      const Item w = it;
+      const int p0 = cut.whole ? 0 : w.i0, p1 = cut.whole ? w.rg.n : min(w.i1, w.rg.n);
+      if (p0 >= p1) continue;
       Box nx{};             // the next tile, or this lane's box of it
       int nx_id = INT_MIN;  // and its page, as the table has it (INT_MIN: not needed)
       auto look = [&](const TileAt& a) {
         const bool one = one_box<BN>(tl, a);
         nx = one ? Box{a.page, a.row, a.base} : box_at<BN>(tl, a, lane);
-        nx_id = one || (lane < tl.boxes && needed(rg, nx.pos, min(tl.rows, ps - nx.row))) ? page_id(ky, sp, b, nx.page)
+        nx_id = one || (lane < tl.boxes && needed(w.rg, nx.pos, min(tl.rows, ps - nx.row))) ? page_id(ky, w.sp, w.b, nx.page)
                                                                                           : INT_MIN;
       };
-      Walk<BN> walk(rg, tl, min(p0, max(p1 - 1, 0)));
-      if (p0 < p1) look(walk.a);
-      for (int i = p0; i < p1; ++i, ++done) {
+      Walk<BN> walk(w.rg, tl, p0);
+      look(walk.a);
+      for (int i = p0; ok && i < p1; ++i) {
         const TileAt a = walk.a;
         const bool bad = nx_id != INT_MIN && (nx_id < 0 || nx_id >= ky.n_pages), one = one_box<BN>(tl, a);
         if (bad) status_raise(ST_PAGE_ID);
@@ -152,14 +257,13 @@ __global__ void __launch_bounds__(THREADS, 2)
           walk.next();
           look(walk.a);
         }
-        const uint32_t st = done % ST, turn = done / ST;
-        if (turn > 0 && !warp_wait(&empty[st], turn - 1, abort_flag, ST_PAGED_ROWS)) break;
-        uint8_t *at = smem + st * STAGE, *mt = smem + ST * STAGE + st * META;
+        if (turn > 0 && !(ok = warp_wait(&empty[st], turn - 1, abort_flag, ST_PAGED_ROWS))) break;
+        uint8_t *at = ring + st * STAGE, *mt = meta + st * META;
         const uint32_t to = smem_u32(mt) + lane * 4;
         uint32_t all = 0xFFFFFFFFu;
-        const int64_t ko = KV8 ? box * ky.ks_str[0] + hk * ky.ks_str[1] + x.row : 0;
-        const int64_t vo = KV8 ? box * ky.vs_str[0] + hk * ky.vs_str[1] + x.row : 0;
-        const bool easy = __all_sync(0xffffffffu, (one || lane < tl.boxes) ? box >= 0 : true) && inside<BN>(rg, a) &&
+        const int64_t ko = KV8 ? box * ky.ks_str[0] + w.hk * ky.ks_str[1] + x.row : 0;
+        const int64_t vo = KV8 ? box * ky.vs_str[0] + w.hk * ky.vs_str[1] + x.row : 0;
+        const bool easy = __all_sync(0xffffffffu, (one || lane < tl.boxes) ? box >= 0 : true) && inside<BN>(w.rg, a) &&
                           !ky.mask && (tl.dense || (one && x.row + BN <= ps));  // every key of the tile
 #pragma unroll
         for (int c = 0; c < KL; ++c) {
@@ -169,7 +273,7 @@ __global__ void __launch_bounds__(THREADS, 2)
             const int id = __shfl_sync(0xffffffffu, box, src);
             const int off = __shfl_sync(0xffffffffu, x.row, src) + ar;
             const int pos = __shfl_sync(0xffffffffu, x.pos, src) + ar;
-            in = id >= 0 && (one || sub[c] < tl.boxes) && off < ps && seen(rg, pos);
+            in = id >= 0 && (one || sub[c] < tl.boxes) && off < ps && seen(w.rg, pos);
             if (ky.mask && in) in = __ldg(ky.mask + id * ky.mask_stride + off) != 0;
             const uint32_t word = __ballot_sync(0xffffffffu, in);
             all &= word;
@@ -184,15 +288,15 @@ __global__ void __launch_bounds__(THREADS, 2)
         if (easy && lane < KL) reinterpret_cast<uint32_t*>(mt + 2 * MAX_BN * 4)[lane] = 0xFFFFFFFFu;
         if constexpr (KV8) asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(&full[st])) : "memory");
         // BN live keys lie at consecutive positions, whatever the page size
-        const bool whole = all == 0xFFFFFFFFu && a.base + BN <= rg.hi_min &&
-                           (a.base >= rg.lo_max || a.base + BN <= rg.sink_min);
-        if (lane == 4) *reinterpret_cast<uint2*>(mt + 2 * MAX_BN * 4 + 16) = make_uint2(whole, nth_tile(rg, i));
+        const bool whole = all == 0xFFFFFFFFu && a.base + BN <= w.rg.hi_min &&
+                           (a.base >= w.rg.lo_max || a.base + BN <= w.rg.sink_min);
+        if (lane == 4) *reinterpret_cast<uint2*>(mt + 2 * MAX_BN * 4 + 16) = make_uint2(whole, nth_tile(w.rg, i));
         __syncwarp();
         auto copy = [&](const CUtensorMap* mk, const CUtensorMap* mv, uint8_t* k, int row, int id) {
-          tma_load_4d(k, mk, &full[st], 0, row, hk, id);
-          if constexpr (!KV8) tma_load_4d(k + STAGE / 4, mk, &full[st], 64, row, hk, id);
-          tma_load_4d(k + STAGE / 2, mv, &full[st], 0, row, hk, id);
-          if constexpr (!KV8) tma_load_4d(k + 3 * STAGE / 4, mv, &full[st], 64, row, hk, id);
+          tma_load_4d(k, mk, &full[st], 0, row, w.hk, id);
+          if constexpr (!KV8) tma_load_4d(k + STAGE / 4, mk, &full[st], 64, row, w.hk, id);
+          tma_load_4d(k + STAGE / 2, mv, &full[st], 0, row, w.hk, id);
+          if constexpr (!KV8) tma_load_4d(k + 3 * STAGE / 4, mv, &full[st], 64, row, w.hk, id);
         };
         if (one) {  // operands in uniform registers
           const int id = __shfl_sync(0xffffffffu, box, 0);
@@ -208,27 +312,37 @@ __global__ void __launch_bounds__(THREADS, 2)
           if (box >= 0) copy(&tm.k, &tm.v, at + lane * bytes, x.row, box);
         }
         __syncwarp();
+        next_stage();
       }
-      if (*abort_flag && lane == 0) {  // let the loads in flight land before their place is used again
-        const uint64_t t0 = globaltimer_ns();
-        for (uint32_t k = done > ST ? done - ST : 0; k < done; ++k)
-          while (!mbar_try_wait(&full[k % ST], (k / ST) & 1) && globaltimer_ns() - t0 < 200000000ull) {
-          }
+    } while (ok && next_item());
+    if (*abort_flag && lane == 0) {  // let the loads in flight land before the CTA exits
+      const uint64_t t0 = globaltimer_ns();
+      for (int k = 0; k < cut.stages; ++k) {  // stage k's last load: its turn, or the one before
+        const int64_t n = (int64_t)turn - (k >= st);
+        while (n >= 0 && !mbar_try_wait(&full[k], n & 1) && globaltimer_ns() - t0 < 200000000ull) {
+        }
       }
-      __syncwarp();
-    } else {
+    }
+    __syncwarp();
+    return;
+  }
+  // ------------------------------------------------------------ consumers
+  do {
+    open_item();
+    const int p0 = cut.whole ? 0 : it.i0, p1 = cut.whole ? it.rg.n : min(it.i1, it.rg.n);
+    const int n_rows = min(cut.height, it.sp.n * qr.group - it.rt * cut.height);
     // This thread's two rows, g and g + 8.
     int tok[2], head[2];
     bool has[2];
     Sees se[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int r = rt * 16 + g + e * 8;
+      const int r = it.rt * cut.height + min(g + e * 8, cut.height);
       tok[e] = r / qr.group;
-      head[e] = hk * qr.group + r - tok[e] * qr.group;
-      has[e] = tok[e] < sp.n;
-      if (!has[e]) tok[e] = sp.n - 1;
-      se[e] = sees(qr, sp, tok[e]);
+      head[e] = it.hk * qr.group + r - tok[e] * qr.group;
+      has[e] = g + e * 8 < cut.height && tok[e] < it.sp.n;
+      if (!has[e]) tok[e] = it.sp.n - 1;
+      se[e] = sees(qr, it.sp, tok[e]);
     }
     // Q fragments, dims in the order in which K is read.
     uint32_t a[8][4];
@@ -238,8 +352,8 @@ __global__ void __launch_bounds__(THREADS, 2)
       float top[2] = {0.f, 0.f};
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int64_t at = ky.cross ? b * qr.q_str[0] + tok[e] * qr.q_str[1] : (int64_t)(sp.first + tok[e]) * qr.q_str[1];
-        const __nv_bfloat16* q = qr.q + at + (has[e] ? head[e] : hk * qr.group) * qr.q_str[2];
+        const int64_t at = ky.cross ? it.b * qr.q_str[0] + tok[e] * qr.q_str[1] : (int64_t)(it.sp.first + tok[e]) * qr.q_str[1];
+        const __nv_bfloat16* q = qr.q + at + (has[e] ? head[e] : it.hk * qr.group) * qr.q_str[2];
 #pragma unroll
         for (int s = 0; s < 8; ++s) {
           const int d = KV8 ? (s >> 2) * 64 + t * 16 + (s & 3) * 4 : (t + 4 * (s >> 1)) * 8 + (s & 1) * 4;
@@ -277,12 +391,11 @@ __global__ void __launch_bounds__(THREADS, 2)
       for (int e = 0; e < 4; ++e) o[k][e] = 0.f;
     float m_run[2] = {-INFINITY, -INFINITY}, m_use[2] = {0.f, 0.f}, l_run[2] = {0.f, 0.f}, v_top = 0.f;
 
-    for (int i = p0; i < p1; ++i, ++done) {
-      const uint32_t st = done % ST;
-      if (!warp_wait(&full[st], done / ST, abort_flag, ST_PAGED_ROWS)) break;
-      uint8_t* K = smem + st * STAGE + warp * KC * 128;
+    for (int i = p0; i < p1; ++i) {
+      if (!warp_wait(&full[st], turn, abort_flag, ST_PAGED_ROWS)) break;
+      uint8_t* K = ring + st * STAGE + warp * KC * 128;
       uint8_t* V = K + STAGE / 2;
-      const uint8_t* mt = smem + ST * STAGE + st * META;
+      const uint8_t* mt = meta + st * META;
       const float* scale = reinterpret_cast<const float*>(mt) + warp * KC;
       const uint2 mark = *reinterpret_cast<const uint2*>(mt + 2 * MAX_BN * 4 + 16);
       const bool whole = mark.x != 0;
@@ -405,11 +518,12 @@ __global__ void __launch_bounds__(THREADS, 2)
             w[e] = *reinterpret_cast<const uint4*>(V + r * 128 + ((g ^ (r & 7)) << 4));
           }
 #pragma unroll
-          for (int k = 0; k < 16; ++k) {
+          for (int k = 0; k < 16; k += 2) {  // bytes k, k + 1 of each key: the columns' codes of two output tiles
             auto word = [&](const uint4& x) { return k < 4 ? x.x : k < 8 ? x.y : k < 12 ? x.z : x.w; };
-            const uint32_t sel = (k & 3) | ((4 + (k & 3)) << 4);
-            mma_f16(o[k], p[k16], codes_f16<DT>(__byte_perm(word(w[0]), word(w[1]), sel) & 0xFFFFu),
-                    codes_f16<DT>(__byte_perm(word(w[2]), word(w[3]), sel) & 0xFFFFu));
+            const uint32_t sel = k & 2 ? 0x7362 : 0x5140;
+            const uint32_t lo = __byte_perm(word(w[0]), word(w[1]), sel), hi = __byte_perm(word(w[2]), word(w[3]), sel);
+            mma_f16(o[k], p[k16], codes_f16<DT>(lo & 0xFFFFu), codes_f16<DT>(hi & 0xFFFFu));
+            mma_f16(o[k + 1], p[k16], codes_f16<DT>(lo >> 16), codes_f16<DT>(hi >> 16));
           }
         } else {
           const int mat = lane >> 3, r = key_of(lane & 7) + (mat & 1) * 8;
@@ -428,148 +542,126 @@ __global__ void __launch_bounds__(THREADS, 2)
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[st]);
+      next_stage();
     }
-    named_bar_sync(1, WARPS * 32);  // the sums lie over the ring: every warp is past it
-    // ---- the warps' sums: O [16][O_PITCH], then m[16], l[16], over the ring
-    float* mine = reinterpret_cast<float*>(smem + warp * PART);
+    // The warps' sums, and from them the item's (or this CTA's part of them), a
+    // thread to a dim.
+    float* mine = sums + warp * cut.height * (O_PITCH + 2);
     if (KV8 && v_top == 0.f) v_top = 1.f;
+    named_bar_sync(1, WARPS * 32);  // the last item's have been read
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 1);
       l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 2);
-      if (g + e * 8 >= n_rows) continue;
+      const int r = g + e * 8;
+      if (r >= n_rows) continue;
       if (t == 0) {
-        mine[16 * O_PITCH + g + e * 8] = m_run[e];
-        mine[16 * O_PITCH + 16 + g + e * 8] = l_run[e];
+        mine[cut.height * O_PITCH + r] = m_run[e];
+        mine[cut.height * (O_PITCH + 1) + r] = l_run[e];
       }
 #pragma unroll
       for (int k = 0; k < 16; ++k)
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
           const int d = KV8 ? (2 * t + f) * 16 + k : k * 8 + 2 * t + f;
-          mine[(g + e * 8) * O_PITCH + d] = KV8 ? o[k][2 * e + f] * v_top : o[k][2 * e + f];
+          mine[r * O_PITCH + d] = KV8 ? o[k][2 * e + f] * v_top : o[k][2 * e + f];
         }
     }
-    }
-    __syncthreads();
-    // The CTA's sums, into warp 0's place: first each row's maximum, l and the
-    // warps' weights (in place of their maxima), then thread x dim x of the rows.
-    constexpr int PITCH_W = PART / 4;
-    float* base = reinterpret_cast<float*>(smem);
+    named_bar_sync(1, WARPS * 32);
     const int dim = threadIdx.x;
-    if (dim < n_rows) {
-      float* at = base + 16 * O_PITCH + dim;
-      float m = -INFINITY, l = 0.f;
+    const bool complete = it.i1 - it.i0 == it.t;
+    const int64_t slot = 2 * cta + (it.i0 == 0);  // of a part: the stretch's first or last
+#pragma unroll 2
+    for (int r = 0; r < n_rows; ++r) {
+      const float* at = sums + cut.height * O_PITCH + r;
+      const int pitch = cut.height * (O_PITCH + 2);
+      float m = -INFINITY, l = 0.f, x = 0.f;
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) m = max_nan(m, at[w * PITCH_W]);
+      for (int w = 0; w < WARPS; ++w) m = max_nan(m, at[w * pitch]);
       const float mu = m == -INFINITY ? 0.f : m;
 #pragma unroll
       for (int w = 0; w < WARPS; ++w) {
-        const float wt = exp2f(at[w * PITCH_W] - mu);
-        l += wt * at[w * PITCH_W + 16];
-        at[w * PITCH_W] = wt;
-      }
-      at[16] = l;
-      at[32] = m;
-    }
-    __syncthreads();
-    if (dim < HD)
-#pragma unroll 2
-    for (int r = 0; r < n_rows; ++r) {
-      float x = 0.f;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w)
-        x += base[w * PITCH_W + 16 * O_PITCH + r] * base[w * PITCH_W + r * O_PITCH + dim];
-      base[r * O_PITCH + dim] = x;
-    }
-    if (cut.cluster > 1)
-      cluster_sync();
-    else
-      __syncthreads();
-    // CTA `rank` finishes rows rank, rank + cluster, ...: the CTAs' sums joined.
-    for (int r = rank; r < n_rows && dim < HD; r += cut.cluster) {
-      const int row = rt * 16 + r, i = row / qr.group;
-      const int h = hk * qr.group + row - i * qr.group;
-      const uint32_t am = smem_u32(base + 16 * O_PITCH + 32 + r), ao = smem_u32(base + r * O_PITCH + dim);
-      float m = -INFINITY, l = 0.f, x = 0.f;
-      if (cut.cluster > 1) {
-        float mc[MAX_CLUSTER], lc[MAX_CLUSTER], xc[MAX_CLUSTER];  // all in flight at once
-#pragma unroll
-        for (int c = 0; c < MAX_CLUSTER; ++c) {
-          const int from = min(c, cut.cluster - 1);
-          mc[c] = cluster_load(am, from);
-          lc[c] = cluster_load(am - 64, from);
-          xc[c] = cluster_load(ao, from);
-        }
-#pragma unroll
-        for (int c = 0; c < MAX_CLUSTER; ++c) m = max_nan(m, mc[c]);
-        const float mu = m == -INFINITY ? 0.f : m;
-#pragma unroll
-        for (int c = 0; c < MAX_CLUSTER; ++c) {
-          const float wt = c < cut.cluster ? exp2f(mc[c] - mu) : 0.f;
-          l += c < cut.cluster ? wt * lc[c] : 0.f;
-          x += c < cut.cluster ? wt * xc[c] : 0.f;
-        }
-      } else {
-        m = base[16 * O_PITCH + 32 + r];
-        l = base[16 * O_PITCH + 16 + r];
-        x = base[r * O_PITCH + dim];
+        const float wt = exp2f(at[w * pitch] - mu);
+        l += wt * at[w * pitch + cut.height];
+        x += wt * sums[w * pitch + r * O_PITCH + dim];
       }
       const bool none = m == -INFINITY;
       const float inv = none ? 0.f : m != m ? m : 1.f / l;
       const float lse2 = none ? -INFINITY : m + log2f(l);
-      const int64_t packed = (int64_t)(sp.first + i) * qr.H + h;
-      if (cut.outer > 1) {
-        const int64_t at = (int64_t)blockIdx.y * qr.rows * qr.H + packed;
-        part_o[at * HD + dim] = x * inv;
-        if (dim == 0) part_l[at] = lse2;
+      if (complete) {
+        store_row(ky, qr, it.b, it.sp.first, it.hk, r + it.rt * cut.height, dim, none ? 0.f : x * inv, lse2);
       } else {
-        const int64_t orow = ky.cross ? b * qr.o_str[0] + i * qr.o_str[1] : (int64_t)(sp.first + i) * qr.o_str[1];
-        qr.o[orow + h * qr.o_str[2] + dim] = __float2bfloat16_rn(none ? 0.f : x * inv);
-        if (qr.lse && dim == 0) qr.lse[packed] = lse2 * 0.6931471805599453f;
+        part_o[(slot * 16 + r) * HD + dim] = x * inv;
+        if (dim == 0) part_l[slot * 16 + r] = lse2;
       }
     }
-    // the others may still read this CTA's sums; the next rows' TMA comes after
-    fence_proxy_async_smem();
-    if (cut.cluster > 1)
-      cluster_sync();
-    else
-      __syncthreads();
+  } while (next_item());
+  if (!cut.whole && threadIdx.x == 0) {
+    // CTA j's stretch begins before the item's end if j * len < end * ctas
+    const long long end = stretch(len, cta + 1, cut.ctas) - it.i1 + it.t;
+    const bool tail = it.i0 == 0 && it.i1 < it.t;
+    split[cta] = Split{it.b, it.hk, it.rt, tail ? (int)((end * cut.ctas + len - 1) / len) - cta : 0};
   }
 }
 
+// Joins items that CTAs hold in parts: block (c, r) row r of the one whose first
+// part is CTA c's last.
+__global__ void __launch_bounds__(HD) join_line_kernel(const __grid_constant__ Keys ky, const __grid_constant__ Queries qr,
+                                                       const __grid_constant__ Cut cut, const float* part_o,
+                                                       const float* part_l, const Split* split) {
+  __shared__ float weight[2 * SMS], tops[HD / 32];
+  const int c = blockIdx.x, r = blockIdx.y, dim = threadIdx.x;
+  asm volatile("griddepcontrol.wait;\n" ::: "memory");
+  const Split it = split[c];
+  if (it.parts == 0) return;
+  const Span sp = span_of(ky, qr, it.b);
+  if (it.rt * cut.height + r >= sp.n * qr.group) return;
+  auto at = [&](int j) { return (int64_t)(2 * (c + j) + (j == 0)) * 16 + r; };
+  float m = -INFINITY;
+  for (int j = dim; j < it.parts; j += HD) m = max_nan(m, weight[j] = part_l[at(j)]);
+#pragma unroll
+  for (int o = 16; o > 0; o /= 2) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if (dim % 32 == 0) tops[dim / 32] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < HD / 32; ++w) m = max_nan(m, tops[w]);
+  for (int j = dim; j < it.parts; j += HD) weight[j] = weight[j] == -INFINITY ? 0.f : exp2f(weight[j] - m);
+  __syncthreads();
+  float l = 0.f, x = 0.f;
+#pragma unroll 8
+  for (int j = 0; j < it.parts; ++j) {
+    const float w = weight[j], v = part_o[at(j) * HD + dim];
+    l += w;
+    x += w == 0.f ? 0.f : w * v;  // (what a part without keys holds does not matter)
+  }
+  store_row(ky, qr, it.b, sp.first, it.hk, r + it.rt * cut.height, dim, m == -INFINITY ? 0.f : x / l,
+            m == -INFINITY ? m : m + log2f(l));
+}
+
 // --------------------------------------------------------------------- host
-// The cut of the keys with the least estimated time, in tiles: those of all
-// waves of CTAs with about six for a CTA's
-// start and end, half of one CTA's again because sequences differ in length,
-// and four for the join of clusters.
-static int places(int cluster) { return cluster <= 2 ? 2 * SMS : cluster == 4 ? 284 : 264; }  // CTAs that run at once
-static Cut cut_of(const Shape& sh, bool kv8) {
-  const int bn = kv8 ? 128 : 64;
-  Cut c{tiling_of(sh.page_size, bn), 1, 1, (int)((sh.max_new * sh.group + 15) / 16)};
-  if (c.row_tiles < 1) c.row_tiles = 1;
-  const int64_t seqs = sh.seqs < sh.rows ? sh.seqs : sh.rows;
-  const int64_t items = seqs * (sh.H / sh.group) * c.row_tiles;
-  const int64_t n = tiles_of_keys(sh, bn);
-  double best = 1e30;
-  for (int cluster = 1; cluster <= MAX_CLUSTER; cluster *= 2)
-    for (int outer = 1; outer <= 16; ++outer) {
-      if (cluster * outer > 1 && n < (int64_t)cluster * outer * 2) break;
-      const double rounds = (double)((n + cluster * outer - 1) / (cluster * outer));
-      const double cost = (double)((items * cluster * outer + places(cluster) - 1) / places(cluster)) * (rounds + 6) + 0.5 * rounds +
-                          (outer > 1 ? 4 : 0);
-      if (cost < best) best = cost, c.cluster = cluster, c.outer = outer;
-    }
+// Whole items where that costs no more tiles of a CTA's time than equal
+// stretches and their join, about eight tiles.
+static Cut cut_of(const Shape& sh) {
+  const int bn = sh.kv8 ? 128 : 64;
+  Cut c{tiling_of(sh.page_size, bn), 1, (int)std::min<int64_t>(std::max<int64_t>(sh.max_new * sh.group, 1), 16), 1, 2};
+  const int64_t seqs = std::min<int64_t>(sh.seqs, sh.rows);
+  const int64_t items = seqs * (sh.H / sh.group) * ((sh.max_new * sh.group + c.height - 1) / c.height);
+  const int64_t n = std::max<int64_t>(tiles_of_keys(sh, bn), 1);
+  const double places = 2 * SMS;
+  c.whole = std::ceil((double)items / places) * (double)n <= items * n / places + 8;
+  c.ctas = (int)std::max<int64_t>(std::min<int64_t>(2 * SMS, c.whole ? items : items * n), 1);
+  c.stages = c.height <= 5 ? 3 : 2;
   return c;
 }
 
 int64_t parts(const Shape& sh) {
-  const int outer = cut_of(sh, sh.kv8).outer;
-  return outer > 1 ? (int64_t)outer * sh.rows * sh.H : 0;
+  const Cut c = cut_of(sh);
+  return c.whole ? 0 : (2 * 16 + 1) * c.ctas;  // 16 rows of two parts, and the splits
 }
 
 template <int DT>
-static int start(const PageMaps& tm, const Keys& ky, const Queries& qr, const Cut& cut, float* part_o, float* part_l, cudaStream_t st) {
+static int start(const PageMaps& tm, const Keys& ky, const Queries& qr, const Cut& cut, float* part_o, float* part_l,
+                 cudaStream_t st) {
   static thread_local int configured = -1;
   int dev = 0;
   WFK_CUDA_TRY(cudaGetDevice(&dev));
@@ -577,37 +669,34 @@ static int start(const PageMaps& tm, const Keys& ky, const Queries& qr, const Cu
     WFK_CUDA_TRY(cudaFuncSetAttribute(rows_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
     configured = dev;
   }
+  Split* split = reinterpret_cast<Split*>(part_l + 32 * cut.ctas);
+  rows_kernel<DT><<<(unsigned)cut.ctas, THREADS, smem_of(cut.stages, cut.height), st>>>(tm, ky, qr, cut, part_o, part_l, split);
+  WFK_CUDA_TRY(cudaGetLastError());
+  if (cut.whole) return WF_OK;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((int64_t)qr.seqs * (qr.H / qr.group) * cut.row_tiles * cut.cluster), (unsigned)cut.outer);
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = SMEM;
+  cfg.gridDim = dim3((unsigned)cut.ctas, (unsigned)cut.height);
+  cfg.blockDim = dim3(HD);
   cfg.stream = st;
   cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim = {(unsigned)cut.cluster, 1, 1};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
-  cfg.numAttrs = cut.cluster > 1 ? 1 : 0;
-  WFK_CUDA_TRY(cudaLaunchKernelEx(&cfg, rows_kernel<DT>, tm, ky, qr, cut, part_o, part_l));
+  cfg.numAttrs = 1;
+  WFK_CUDA_TRY(cudaLaunchKernelEx(&cfg, join_line_kernel, ky, qr, cut, (const float*)part_o, (const float*)part_l,
+                                  (const Split*)split));
   return WF_OK;
 }
 
 int launch(const Keys& ky, const Queries& qr, const Shape& sh, void* workspace, cudaStream_t st) {
-  const Cut cut = cut_of(sh, sh.kv8);
-  if ((int64_t)qr.seqs * (qr.H / qr.group) * cut.row_tiles * cut.cluster > INT_MAX)
-    return fail(WF_ERR_INVALID_ARG, "attention: too many rows");
-  float *part_o = nullptr, *part_l = nullptr;
-  if (cut.outer > 1) {
-    part_o = static_cast<float*>(workspace);
-    part_l = part_o + (int64_t)cut.outer * qr.rows * qr.H * HD;
-  }
+  const Cut cut = cut_of(sh);
+  float* part_o = static_cast<float*>(workspace);
+  float* part_l = part_o + 32 * cut.ctas * HD;
   PageMaps tm;
   int rc;
   if ((rc = page_maps(&tm, ky, qr.H / qr.group, cut.tl, sh.kv8 ? 128 : 64)) != WF_OK) return rc;
-  rc = ky.dtype == WF_DTYPE_BF16   ? start<WF_DTYPE_BF16>(tm, ky, qr, cut, part_o, part_l, st)
-       : ky.dtype == WF_DTYPE_E4M3 ? start<WF_DTYPE_E4M3>(tm, ky, qr, cut, part_o, part_l, st)
-                                   : start<WF_DTYPE_S8>(tm, ky, qr, cut, part_o, part_l, st);
-  if (rc != WF_OK || cut.outer == 1) return rc;
-  return join(ky, qr, part_o, part_l, cut.outer, st);
+  return ky.dtype == WF_DTYPE_BF16   ? start<WF_DTYPE_BF16>(tm, ky, qr, cut, part_o, part_l, st)
+         : ky.dtype == WF_DTYPE_E4M3 ? start<WF_DTYPE_E4M3>(tm, ky, qr, cut, part_o, part_l, st)
+                                     : start<WF_DTYPE_S8>(tm, ky, qr, cut, part_o, part_l, st);
 }
 
 }  // namespace rows
