@@ -87,7 +87,7 @@ __device__ __forceinline__ Sees sees(const Queries& qr, const Span& s, int i) {
   const int p = s.pos0 + i;
   Sees v;
   v.hi = s.len;
-  if (qr.block > 0) v.hi = (int)min((long long)s.len, ((long long)p / qr.block + 1) * qr.block);
+  if (qr.block > 0 && p >= 0) v.hi = (int)min((long long)s.len, (p / qr.block + 1ll) * qr.block);
   if (p < 0) v.hi = 0;
   v.lo = qr.window > 0 ? max(v.hi - qr.window, 0) : 0;
   v.sink = min(qr.sink, v.lo);
@@ -107,23 +107,27 @@ __device__ __forceinline__ int page_id(const Keys& ky, const Span& s, int b, int
 // give ceil(page_size / BN) tiles each, smaller ones share a tile, a page to a
 // box.
 struct Tiling {
+  uint32_t mul, shift;              // x / ps = x * mul >> shift for 0 <= x < 2^31
   int ps, dense, tpp, boxes, rows;  // page size; tiles per page (large, not dense); boxes of a tile, their rows
   int tq, splits, even, wide;       // paged_tile.cu: tokens of a sub-tile, runs of keys, whether items are dealt
                                     // evenly, whether rows of O begin on 32-byte boundaries
 };
 inline Tiling tiling_of(int ps, int bn, bool dense = true) {
-  Tiling t{ps, dense && ps % 8 == 0, (ps + bn - 1) / bn, 1, bn, 0, 1, 0, 0};
+  Tiling t{0, 31, ps, dense && ps % 8 == 0, (ps + bn - 1) / bn, 1, bn, 0, 1, 0, 0};
   if (t.dense)
     while (ps % t.rows) t.rows /= 2;
   else if (ps < bn)
     t.rows = (ps + 7) & ~7;
   t.boxes = bn / t.rows;
+  while ((1ll << (t.shift - 31)) < ps) ++t.shift;  // mul = ceil(2^shift / ps): off by less than x / 2^shift < 1 / ps
+  t.mul = (uint32_t)(((1ull << t.shift) + ps - 1) / ps);
   return t;
 }
+__device__ __forceinline__ int page_of(const Tiling& tl, int pos) { return (int)((uint64_t)pos * tl.mul >> tl.shift); }
 template <int BN>
 __device__ __forceinline__ int tile_of(const Tiling& tl, int pos) {
   if (tl.dense) return pos / BN;
-  const int j = pos / tl.ps;
+  const int j = page_of(tl, pos);
   return tl.ps < BN ? j / tl.boxes : j * tl.tpp + (pos - j * tl.ps) / BN;
 }
 struct TileAt {
@@ -134,7 +138,7 @@ __device__ __forceinline__ TileAt tile_at(const Tiling& tl, int t) {
   TileAt a;
   if (tl.dense) {
     a.base = t * BN;
-    a.page = a.base / tl.ps;
+    a.page = page_of(tl, a.base);
     a.row = a.base - a.page * tl.ps;
     return a;
   }
@@ -155,7 +159,7 @@ __device__ __forceinline__ int rows_below(const Tiling& tl, const TileAt& a, int
   if (d <= 0) return 0;
   if (tl.dense) return min(d, BN);
   if (tl.ps >= BN) return min(d, min(BN, tl.ps - a.row));
-  const int j = d / tl.ps;
+  const int j = page_of(tl, d);
   return min(j, tl.boxes) * tl.rows + (j < tl.boxes ? d - j * tl.ps : 0);
 }
 // The tile after a (of consecutive tiles).
@@ -188,7 +192,7 @@ __device__ __forceinline__ Box box_at(const Tiling& tl, const TileAt& a, int i) 
   Box x{a.page, a.row, a.base};
   if (tl.dense) {
     x.pos += i * tl.rows;
-    x.page = x.pos / tl.ps;
+    x.page = page_of(tl, x.pos);
     x.row = x.pos - x.page * tl.ps;
   } else if (tl.ps < BN) {
     x.page += i;
@@ -274,9 +278,6 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
 __device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
-}
-__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {  // without an arrival
-  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool take) {  // zero when not taken
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(take ? 4 : 0) : "memory");

@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
         bool in = true;
         if (tl.dense) {
           if (row >= tl.ps) {
-            const int j = row / tl.ps;
+            const int j = page_of(tl, row);
             page += j;
             row -= j * tl.ps;
           }
