@@ -21,7 +21,13 @@
 // Half a warp holds a row (8 elements a lane): lanes 0-15 take K, 16-31 V.  A
 // block takes 16 packed rows and 4 heads at a time, all their loads in flight
 // before the first use, then the next 4 heads, loaded under the stores of the
-// last: the rows' slots are looked up once.
+// last: the rows' slots are looked up once (28080 rows of 40 heads, e4m3: 320 us
+// with a block to every 4 heads).  The maxima of a half warp's 8 rows are folded
+// together so that two divisions serve all of them; with two divisions and four
+// shuffles a row the write took 301 us, bound by instructions.
+//
+// Measured: that write 195 us, 4.5 TB/s or 0.69 of the HBM copy rate; 23400
+// rows of 12 heads read back in 45 us, 4.8 TB/s.
 #include <cuda_runtime.h>
 
 #include <algorithm>

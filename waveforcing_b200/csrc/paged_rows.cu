@@ -2,14 +2,29 @@
 // runs of them): bound by reading K and V once from HBM.
 //
 // Rows of one K/V head (tokens x the query heads that share it) come in tiles
-// of 16, the height of mma.sync's A operand, which here only has to keep up
-// with the loads: 32 instructions to 8 KB of K and V.  A cluster of up to 8
-// CTAs takes one tile of rows, each CTA a share of the key tiles.  Warp 4 loads
-// tiles by TMA into a ring of three (64 KB in flight, two CTAs to an SM); warps
+// of up to 16, the height of mma.sync's A operand, which here only has to keep
+// up with the loads: 32 instructions to 8 KB of K and V.  An item of work is one
+// tile of rows against its key tiles.  All items' key tiles lie in a line, cut
+// into an equal stretch for each of two CTAs an SM, so that ragged lengths
+// leave no SM idle; the parts of an item that lies in several stretches (each
+// CTA has at most two) are joined by a second launch, whose blocks are in place
+// before the first one ends.  Where whole items fill the SMs evenly they are not
+// cut.  Warp 4 walks the stretch and loads tiles by TMA into a ring of two or
+// three (64 KB in flight), on into the next item while the last one ends; warps
 // 0-3 take a quarter of a tile's keys each, multiply them straight from shared
-// memory and keep sums of their own, which are joined through (distributed)
-// shared memory at the end.  (With every warp loading its own chunks, issuing
-// four TMA copies cost 600 of 1700 clocks a chunk.)
+// memory and keep sums of their own, joined through shared memory at an item's
+// end.  (With every warp loading its own chunks, issuing four TMA copies cost
+// 600 of 1700 clocks a chunk.  With a cluster of CTAs to an item, joined through
+// distributed shared memory, the ragged batch below took 94 us and the masked
+// cross attention 53.)
+//
+// Measured: 32 ragged sequences of up to 8192 tokens, 40 heads on 8, e4m3: 77 us,
+// 0.54 of the HBM copy rate; 8 x 8192 tokens, 32 heads on 8, bf16: 57 us, 4.7
+// TB/s; 32768 tokens, 12 heads, bf16: 46 us, 4.4 TB/s; 24 x 40 single rows over
+// 257 masked keys: 44 us.  Bound by the start (12,000 clocks to the first data:
+// lengths, page table and pages are loads that wait for each other) and, over
+// 8-bit pages, by each warp's chain of load, expansion and product: 3300 clocks a
+// tile of 128 keys against 1350 for 64 keys of bf16.
 //
 // A contraction does not mind in which order its dimension is taken, so a
 // thread loads 16 consecutive bytes of a K row and feeds them to the k indices

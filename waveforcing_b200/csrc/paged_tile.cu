@@ -5,8 +5,9 @@
 // of 128-key tiles.  K and V tiles are loaded once for both sub-tiles.
 //   warp 0       TMA producer (a lane to a box of a tile)
 //   warp 1       MMA issue: S_u = Q_u K_j^T (M=N=K=128), O_u += P_u V_j
-//   warp 2       marks the live keys of each tile, zeroes the V rows of the
-//                others (their P is 0, but 0 * NaN is not), fetches scales
+//   warp 2       marks the live keys of each tile; bf16: zeroes the V rows of
+//                the others (their P is 0, but 0 * NaN is not); 8 bits: fetches
+//                scales, a tile ahead of the codes
 //   warp 3       finds the CTA's items ahead of the other roles
 //   warps 4-11   softmax; warpgroup u owns sub-tile u, a thread a row
 //   warps 12-15  (8-bit pages) expand codes to f16
@@ -25,6 +26,15 @@
 // scale per key applied to S and P instead costs two shared-memory reads of
 // 512 bytes a row and tile: 525 against 398 us without at 9472 x 16384 x 4
 // heads, where the rows' reads and the operands' share shared memory.
+//
+// Measured at that size: bf16 248 us, 1285 TFLOP/s (0.77 of the cuBLAS burst
+// rate), e4m3 335-360 us; 4680 x 37440 x 12 heads: bf16 903 us over 128-row
+// pages and 1010 over 1560-row ones, e4m3 1325 us.  A tile takes about 3600 clocks
+// where its products take 2048: a warp's chain from S to P (load, maximum,
+// exponentials, store) is as long as the other sub-tile's products cover.  8-bit
+// pages: the expansion's shared-memory traffic, and the roles' code, which
+// exceeds what the instruction caches hold (stalls for instructions 1.2 an issue
+// against 0.5).
 #include <cuda_fp16.h>
 
 #include <cmath>
