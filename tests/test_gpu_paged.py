@@ -482,6 +482,16 @@ def test_attention_in_parts(case, dtype):
     healthy()
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "e4m3", "s8"])
+@pytest.mark.parametrize("block,window,sink", [(1, 0, 0), (64, 500, 40)])
+def test_attention_of_ragged_prompts(dtype, block, window, sink):
+    """More items than run at once, taken from the longest to the shortest; one sequence has no new
+    rows, one is shorter than its new rows, and rows lie behind the last."""
+    pool = Pool(dtype, [1500, 40, 300, 7, 900, 2000], 6, 16, seed=17)
+    check_attention(pool, [700, 40, 0, 9, 300, 900], 24, block, window, sink, hints=(900, 2000), tail=3)
+    healthy()
+
+
 @pytest.mark.parametrize("dtype", [E4, S8], ids=["e4m3", "s8"])
 def test_scales_with_strides_of_their_own(dtype):
     pool = Pool(dtype, [400, 90], 2, 64, seed=15)

@@ -137,6 +137,8 @@ def header_symbols() -> list[str]:
 def lib() -> C.CDLL:
     """Load libwfk.so once; raise if it is absent (no CPU fallback exists)."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is None:
             if not os.path.exists(LIB_PATH):

@@ -38,6 +38,7 @@
 #include <cuda_fp16.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "paged_attn.cuh"
 
@@ -87,6 +88,77 @@ __device__ __forceinline__ int count_tiles(const Keys& ky, const Queries& qr, co
 // Run p of s of n tiles starts here.
 __device__ __forceinline__ int run_start(int n, int p, int s) { return n / s * p + n % s * p / s; }
 
+// The item of query tile `tile` of sequence w.b (w.sp) and head w.hk, with all of its key tiles.
+__device__ __forceinline__ void fill_work(Work& w, const Queries& qr, const Tiling& tl, int tile) {
+  w.i0 = tile * 2 * tl.tq;
+  const int i1 = min(w.i0 + 2 * tl.tq, w.sp.n) - 1;  // last token
+  w.nsub = i1 >= w.i0 + tl.tq ? 2 : 1;
+  static_cast<Range&>(w) = range_of<BN>(qr, w.sp, tl, w.i0, i1);
+  w.t0 = 0;
+  w.t1 = w.n;
+  w.slot = -1;
+}
+
+// Item `it` of a launch whose items are taken from the longest to the shortest,
+// all K/V heads of a query tile in turn (one warp, at most 32 sequences and MANY
+// query tiles): a lane finds the lengths of up to MANY / 32 query tiles, and
+// the one that it / G others are longer than is taken.
+constexpr int MANY = 128;
+__device__ __forceinline__ bool nth_longest(Work& w, const Keys& ky, const Queries& qr, const Tiling& tl, int n_tiles,
+                                            int G, unsigned it, int lane) {
+  if (it >= (unsigned)n_tiles * G) return false;
+  Span mine{};
+  if (lane < qr.seqs) mine = span_of(ky, qr, lane);
+  const int nq = (mine.n + 2 * tl.tq - 1) / (2 * tl.tq);
+  int before = nq;  // query tiles of the sequences before this lane's
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += x;
+  }
+  before -= nq;
+  int key[MANY / 32], longer[MANY / 32];
+#pragma unroll
+  for (int k = 0; k < MANY / 32; ++k) {
+    key[k] = -1;
+    longer[k] = 0;
+    if (k * 32 >= n_tiles) continue;
+    const int q = k * 32 + lane;
+    int b = 0;
+#pragma unroll 1
+    for (int x = 1; x < qr.seqs; ++x) b = __shfl_sync(0xffffffffu, before, x) <= q ? x : b;
+    w.sp.first = __shfl_sync(0xffffffffu, mine.first, b);
+    w.sp.n = __shfl_sync(0xffffffffu, mine.n, b);
+    w.sp.len = __shfl_sync(0xffffffffu, mine.len, b);
+    w.sp.pos0 = __shfl_sync(0xffffffffu, mine.pos0, b);
+    const int tile = q - __shfl_sync(0xffffffffu, before, b);
+    if (q >= n_tiles) continue;
+    fill_work(w, qr, tl, tile);
+    key[k] = min(w.n, 1 << 23) * MANY + MANY - 1 - q;  // no two alike
+  }
+#pragma unroll
+  for (int k = 0; k < MANY / 32; ++k) {
+    if (k * 32 >= n_tiles) continue;
+#pragma unroll 1
+    for (int x = 0; x < 32; ++x) {
+      const int other = __shfl_sync(0xffffffffu, key[k], x);
+#pragma unroll
+      for (int y = 0; y < MANY / 32; ++y) longer[y] += other > key[y];
+    }
+  }
+  int q = 0;
+#pragma unroll
+  for (int k = 0; k < MANY / 32; ++k) {
+    const uint32_t here = __ballot_sync(0xffffffffu, key[k] >= 0 && longer[k] == (int)(it / (unsigned)G));
+    if (here) q = k * 32 + __ffs(here) - 1;
+  }
+  w.b = 31 - __clz(__ballot_sync(0xffffffffu, lane < qr.seqs && before <= q));
+  w.hk = it % (unsigned)G;
+  w.sp = span_of(ky, qr, w.b);
+  fill_work(w, qr, tl, q - __shfl_sync(0xffffffffu, before, w.b));
+  return true;
+}
+
 // Item `it` of the launch (one warp, same result in every lane).
 __device__ __forceinline__ bool find_work(Work& w, const Keys& ky, const Queries& qr, const Tiling& tl, int n_tiles,
                                           int G, unsigned it, int lane) {
@@ -124,15 +196,8 @@ __device__ __forceinline__ bool find_work(Work& w, const Keys& ky, const Queries
       tile -= __shfl_sync(0xffffffffu, sum, 31);
     }
   }
-  tile = nq - 1 - tile;  // a causal sequence's longest rows first
   w.sp = span_of(ky, qr, w.b);
-  w.i0 = tile * 2 * tl.tq;
-  const int i1 = min(w.i0 + 2 * tl.tq, w.sp.n) - 1;  // last token
-  w.nsub = i1 >= w.i0 + tl.tq ? 2 : 1;
-  static_cast<Range&>(w) = range_of<BN>(qr, w.sp, tl, w.i0, i1);
-  w.t0 = 0;
-  w.t1 = w.n;
-  w.slot = -1;
+  fill_work(w, qr, tl, nq - 1 - tile);  // a causal sequence's longest rows first
   if (tl.splits > 1) {  // at most 32 of them
     w.t0 = run_start(w.n, w.split, tl.splits);
     w.t1 = run_start(w.n, w.split + 1, tl.splits);
@@ -289,7 +354,7 @@ __device__ __forceinline__ void store32(void* to, const uint32_t* r, bool wide) 
   }
 }
 
-template <int DT>
+template <int DT, bool SORTED>
 __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
     tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ PageMaps tm,
                 const __grid_constant__ Keys ky,
@@ -795,7 +860,8 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
         ++work_n;
       };
       const unsigned whole = d.even ? d.full : 0xFFFFFFFFu;
-      for (unsigned it = c; ok && it < whole && find_work(w, ky, qr, tl, n_tiles, G, it, lane); it += ctas) give();
+      for (unsigned it = c; ok && it < whole && (SORTED ? nth_longest(w, ky, qr, tl, n_tiles, G, it, lane) : find_work(w, ky, qr, tl, n_tiles, G, it, lane)); it += ctas)
+        give();
       for (int v = c; ok && d.even && v < d.left * d.parts; v += ctas) {
         const int p = v / d.left, r = v - p * d.left;
         find_work(w, ky, qr, tl, n_tiles, G, d.full + r, lane);
@@ -1103,6 +1169,14 @@ static int splits(const Shape& sh) {
   }
   return best;
 }
+// Whether items are taken from the longest to the shortest (see nth_longest): more
+// of them than run at once, of sequences of different lengths, whose K and V stay
+// in L2 whatever the order.
+static bool sorted(const Shape& sh) {
+  const int64_t G = sh.H / sh.group, tiles = tiles_bound(sh);
+  return !sh.cross && sh.seqs > 1 && sh.seqs <= 32 && tiles <= MANY && tiles * G > SMS && key_tiles(sh) >= 8 &&
+         splits(sh) == 1 && sh.seqs * sh.keys * G * (sh.kv8 ? 2 * (HD + 4) : 4 * HD) <= (64 << 20);
+}
 int64_t parts(const Shape& sh) {
   if (dealt(sh)) {  // rows that turn out fewer leave other items
     const int64_t items = tiles_bound(sh) * (sh.H / sh.group);
@@ -1112,7 +1186,7 @@ int64_t parts(const Shape& sh) {
   return s > 1 ? (int64_t)s * sh.rows * sh.H : 0;
 }
 
-template <int DT>
+template <int DT, bool SORTED>
 static int start(const CUtensorMap& tq, const PageMaps& tm, const Keys& ky,
                  const Queries& qr, const Tiling& tl, unsigned grid, float* part_o, float* part_l, cudaStream_t st) {
   using C = Cfg<DT != WF_DTYPE_BF16>;
@@ -1120,10 +1194,10 @@ static int start(const CUtensorMap& tq, const PageMaps& tm, const Keys& ky,
   int dev = 0;
   WFK_CUDA_TRY(cudaGetDevice(&dev));
   if (configured != dev) {
-    WFK_CUDA_TRY(cudaFuncSetAttribute(tile_kernel<DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    WFK_CUDA_TRY(cudaFuncSetAttribute(tile_kernel<DT, SORTED>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     configured = dev;
   }
-  tile_kernel<DT><<<grid, C::THREADS, C::SMEM, st>>>(tq, tm, ky, qr, tl, part_o, part_l);
+  tile_kernel<DT, SORTED><<<grid, C::THREADS, C::SMEM, st>>>(tq, tm, ky, qr, tl, part_o, part_l);
   WFK_CUDA_TRY(cudaGetLastError());
   return WF_OK;
 }
@@ -1159,9 +1233,13 @@ int launch(const Keys& ky, const Queries& qr, const Shape& sh, void* workspace, 
   const int64_t n_parts = parts(sh);
   float* part_o = static_cast<float*>(workspace);
   float* part_l = part_o + n_parts * HD;
-  rc = ky.dtype == WF_DTYPE_BF16   ? start<WF_DTYPE_BF16>(tq, tm, ky, qr, tl, grid, part_o, part_l, st)
-       : ky.dtype == WF_DTYPE_E4M3 ? start<WF_DTYPE_E4M3>(tq, tm, ky, qr, tl, grid, part_o, part_l, st)
-                                   : start<WF_DTYPE_S8>(tq, tm, ky, qr, tl, grid, part_o, part_l, st);
+  auto pick = [&](auto x) {
+    constexpr bool S = decltype(x)::value;
+    return ky.dtype == WF_DTYPE_BF16   ? start<WF_DTYPE_BF16, S>(tq, tm, ky, qr, tl, grid, part_o, part_l, st)
+           : ky.dtype == WF_DTYPE_E4M3 ? start<WF_DTYPE_E4M3, S>(tq, tm, ky, qr, tl, grid, part_o, part_l, st)
+                                       : start<WF_DTYPE_S8, S>(tq, tm, ky, qr, tl, grid, part_o, part_l, st);
+  };
+  rc = sorted(sh) ? pick(std::true_type{}) : pick(std::false_type{});
   if (rc != WF_OK || n_parts == 0) return rc;
   if (tl.even) {
     const int64_t left = items % SMS;  // with rows behind the sequence the device may have others

@@ -608,7 +608,7 @@ def _no_grad(what: str, *ts: torch.Tensor) -> None:
 def _on(d: int, fn, *args) -> int:
     """fn(*args, stream) on device d's current stream, with d the current device."""
     LAUNCHES[0] += 1
-    if d == torch.cuda.current_device():
+    if d == torch._C._cuda_getDevice():  # (a CUDA tensor is there: CUDA has been initialised)
         return fn(*args, torch._C._cuda_getCurrentRawStream(d))
     with torch.cuda.device(d):
         return fn(*args, torch._C._cuda_getCurrentRawStream(d))
