@@ -20,7 +20,8 @@ META, WORKS = 4, 4
 class Sim:
     wrong = None
 
-    def __init__(self, items, kv8, seed):
+    def __init__(self, items, kv8, seed, slow=None):
+        self.slow = slow  # a role that seldom runs: phases that pass it by unseen show
         self.items, self.kv8, self.rnd = items, kv8, random.Random(seed)  # items: (sub-tiles, key tiles)
         self.NS = 4 if kv8 else 5
         B = {}
@@ -28,6 +29,7 @@ class Sim:
             B[f"raw{s}"], B[f"full{s}"], B[f"empty{s}"] = Bar(1), Bar(1), Bar(1)
         for m in range(META):
             B[f"marked{m}"] = Bar(1)
+            B[f"unmarked{m}"] = Bar(1)
         for u in range(2):
             for n in ("q_raw", "q_full", "q_empty", "s", "p0", "p1", "o_full"):
                 B[f"{n}{u}"] = Bar(1)
@@ -105,7 +107,7 @@ class Sim:
         self.pipe.append(("commit", f"s{u}"))
 
     def mma(self):
-        n, items, pn, work_n = 0, [0, 0], [0, 0], 0
+        n, items, pn, work_n, tiles = 0, [0, 0], [0, 0], 0, 0
         while True:
             item = yield from self.take(work_n)
             work_n += 1
@@ -138,6 +140,8 @@ class Sim:
                     pn[u] += 1
                     if u == nsub - 1:
                         self.pipe.append(("commit", f"empty{s}"))
+                        if self.kv8:
+                            self.pipe.append(("commit", f"unmarked{tiles % META}"))
                     if not more:
                         self.pipe.append(("commit", f"o_full{u}"))
                     yield
@@ -151,6 +155,7 @@ class Sim:
                             self.pipe.append(("commit", f"empty{sk % self.NS}"))
                         yield
                 n += 2 if more else 1
+                tiles += 1
             for u in range(nsub):
                 items[u] += 1
 
@@ -171,8 +176,11 @@ class Sim:
                 s = n % self.NS
                 if not self.kv8:
                     yield from self.wait(f"raw{s}", n // self.NS)
-                elif tiles > 0:  # the K before
-                    yield from self.wait(f"raw{(n - 2) % self.NS}", (n - 2) // self.NS)
+                elif self.wrong == "stale":  # the K before, whose barrier may be a phase further
+                    if tiles > 0:
+                        yield from self.wait(f"raw{(n - 2) % self.NS}", (n - 2) // self.NS)
+                elif tiles >= META:
+                    yield from self.wait(f"unmarked{tiles % META}", tiles // META - 1)
                 self.marks[tiles % (1 if self.wrong == "meta" else META - (self.wrong == "ahead"))] = (i, j)
                 if self.kv8:
                     self.b[f"marked{tiles % META}"].arrive()
@@ -291,9 +299,11 @@ class Sim:
         roles = [self.finder(), self.producer(), self.mma(), self.mark(), self.softmax(0), self.softmax(1)]
         if self.kv8:
             roles.append(self.expand())
-        idle = 0
+        idle, slow = 0, roles[self.slow % len(roles)] if self.slow is not None else None
         while roles or self.pipe or self.tma:
             k = self.rnd.randrange(len(roles) + 2)
+            if self.slow is not None and k < len(roles) and roles[k] is slow and self.rnd.random() < 0.98:
+                continue  # the others run far ahead of it
             before = (len(self.tma), len(self.pipe), len(roles), tuple(b.phase * 1000 + b.pend for b in self.b.values()))
             if k < len(roles):
                 try:
@@ -306,7 +316,7 @@ class Sim:
                 self.step_pipe()
             after = (len(self.tma), len(self.pipe), len(roles), tuple(b.phase * 1000 + b.pend for b in self.b.values()))
             idle = idle + 1 if before == after else 0
-            assert idle < 5000, "deadlock"
+            assert idle < (5000 if slow is None else 60000), "deadlock"
 
 
 def random_items(rnd):
@@ -317,6 +327,22 @@ def random_items(rnd):
 def test_protocol(kv8):
     for seed in range(150):
         Sim(random_items(random.Random(seed)), kv8, seed).run()
+
+
+@pytest.mark.parametrize("kv8", [False, True])
+@pytest.mark.parametrize("slow", range(7))
+def test_protocol_with_a_slow_role(kv8, slow):
+    for seed in range(20):
+        Sim(random_items(random.Random(seed)), kv8, seed, slow).run()
+
+
+def test_a_phase_that_passes_unseen_is_caught():
+    class Bad(Sim):
+        wrong = "stale"
+
+    with pytest.raises(AssertionError, match="deadlock"):
+        for seed in range(40):
+            Bad(random_items(random.Random(seed)), True, seed, 3).run()
 
 
 @pytest.mark.parametrize("wrong", ["p", "meta", "ahead", "qpow", "works"])

@@ -59,7 +59,7 @@ struct Cfg {
   static constexpr int NS = KV8 ? 4 : 5;  // ring slots
   static constexpr int THREADS = KV8 ? 512 : 384;
   static constexpr int READERS = KV8 ? 15 : 11;  // warps that an item goes to
-  static constexpr int NBARS = (3 * NS + 14 + META + 2 * WORKS + 1 + 1) & ~1;  // even: what follows is 16-byte aligned
+  static constexpr int NBARS = (3 * NS + 14 + 2 * META + 2 * WORKS + 1 + 1) & ~1;  // even: what follows is 16-byte aligned
   static constexpr int META_BYTES = META * (16 + (KV8 ? 2 * BN * 4 : 0) + 16) + (KV8 ? 4 * BM * 4 : 0);
   static constexpr int SMEM = 1024 + 2 * SLOT + NS * SLOT + NBARS * 8 + META_BYTES + 16 + WORKS * WORK_BYTES;
   static_assert(SMEM <= 232448, "shared memory of one CTA");
@@ -376,7 +376,8 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
   uint64_t* bar_fin = o_full + 2;
   uint64_t* q_raw = bar_fin + 1;     // [2] 8-bit pages: Q_u landed (q_full: as f16)
   uint64_t* marked = q_raw + 2;      // [META] 8-bit pages: a tile's scales are there
-  uint64_t* work_full = marked + META;     // [WORKS] an item is there
+  uint64_t* unmarked = marked + META;  // [META] and have been used: P V of the tile is done
+  uint64_t* work_full = unmarked + META;  // [WORKS] an item is there
   uint64_t* work_empty = work_full + WORKS;
   uint32_t* live = reinterpret_cast<uint32_t*>(raw + Cfg<KV8>::NBARS);  // [META][4] live keys of a tile
   int* whole = reinterpret_cast<int*>(live + META * 4);                 // [META] every row sees all of it
@@ -409,7 +410,10 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
       mbar_init(&bar_p[2 * u + 1], 128);
       mbar_init(&o_full[u], 1);
     }
-    for (int m = 0; m < META; ++m) mbar_init(&marked[m], 1);
+    for (int m = 0; m < META; ++m) {
+      mbar_init(&marked[m], 1);
+      mbar_init(&unmarked[m], 1);
+    }
     for (int k = 0; k < WORKS; ++k) {
       mbar_init(&work_full[k], 1);
       mbar_init(&work_empty[k], Cfg<KV8>::READERS);
@@ -545,7 +549,7 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
       constexpr uint32_t FMT = KV8 ? FMT_F16 : FMT_BF16;
       constexpr uint32_t idesc_qk = make_idesc(1, FMT, FMT, 0, BM, BN);
       constexpr uint32_t idesc_pv = make_idesc(1, FMT, FMT, 1, BM, HD);
-      uint32_t slot_n = 0, items[2] = {0, 0}, pn[2] = {0, 0};
+      uint32_t slot_n = 0, items[2] = {0, 0}, pn[2] = {0, 0}, tiles = 0;
       bool ok = true;
       auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
         ok = ok && warp_wait(bar, parity, abort_flag, ST_PAGED_MMA);
@@ -605,6 +609,7 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
             ++pn[u];
             if (elect_one()) {
               if (u == last_u) umma_commit(&empty[sv % NS]);
+              if (KV8 && u == last_u) umma_commit(&unmarked[tiles % META]);
               if (!more) umma_commit(&o_full[u]);
             }
             __syncwarp();
@@ -619,6 +624,7 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
             }
           }
           slot_n += more ? 2 : 1;
+          ++tiles;
         }
         for (int u = 0; u < nsub; ++u) ++items[u];
       }
@@ -759,10 +765,10 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
       }
     } else if (warp == 2) {
       // ---------------------------------------------- marks and scales, 8 bits
-      // A tile is marked when the K before it has landed, so that its expansion
-      // waits for its codes alone; its scales are loaded before that wait and
-      // its page ids a tile earlier.
-      uint32_t slot_n = 0, tiles = 0;
+      // A tile is marked as soon as the marks of tile n - META are done with, so
+      // that its expansion waits for its codes alone; its scales are loaded before
+      // that wait and its page ids a tile earlier.
+      uint32_t tiles = 0;
       bool ok = true;
       int ids[4], box[4], at_row[4];  // of keys c * 32 + lane: page id, box, row of the box
 #pragma unroll
@@ -804,9 +810,9 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
             walk.next();
             look(walk.a);
           }
-          // The K before has landed: S of three tiles before has been formed, over
-          // the P of the tile whose marks lay here (META tiles before).
-          if (tiles > 0 && !(ok = warp_wait(&raw[(slot_n - 2) % NS], (slot_n - 2) / NS, abort_flag, ST_PAGED_MARK))) break;
+          // (a barrier of the ring could pass this phase and the next before the
+          // warp looks; unmarked[m] goes no further than the tile that waits)
+          if (tiles >= META && !(ok = warp_wait(&unmarked[tiles % META], tiles / META - 1, abort_flag, ST_PAGED_MARK))) break;
           const uint32_t m = tiles % META;
           uint32_t words[4];
 #pragma unroll
@@ -840,7 +846,6 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
           if (lane == 6) vpow[m] = v_top;
           __syncwarp();
           if (lane == 0) mbar_arrive(&marked[m]);
-          slot_n += 2;
         }
       }
     }
