@@ -969,13 +969,26 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
           if (KV8) alpha *= v_run / v_new;
           v_run = v_new;
           if (j > 0) {
+            // (written for the registers that S leaves: unrolled, the wide form's
+            // pieces spill S for 8-bit pages, rolled it costs bf16 4 % of cross attention)
+            if constexpr (KV8) {
+#pragma unroll 1
+              for (int c = 0; c < HD; c += 32) {
+                uint32_t r[32];
+                tmem_ld32x32b_x32(tO + c, r);
 #pragma unroll
-            for (int c = 0; c < HD; c += 32) {
-              uint32_t r[32];
-              tmem_ld32x32b_x32(tO + c, r);
+                for (int k = 0; k < 32; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * alpha);
+                tmem_st32x32b_x32(tO + c, r);
+              }
+            } else {
 #pragma unroll
-              for (int k = 0; k < 32; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * alpha);
-              tmem_st32x32b_x32(tO + c, r);
+              for (int c = 0; c < HD; c += 16) {
+                uint32_t r[16];
+                tmem_ld32x32b_x16(tO + c, r);
+#pragma unroll
+                for (int k = 0; k < 16; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * alpha);
+                tmem_st32x32b_x16(tO + c, r);
+              }
             }
           }
         }
