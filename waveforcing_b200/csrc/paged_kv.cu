@@ -370,9 +370,9 @@ static int run(const char* who, const wf_kv_pages* pages, const wf_kv_batch* bat
   const Batch bt = make_batch(batch);
   const Pool pool = make_pool(pages);
   const Rows rows{k, v, {ks[0], ks[1]}, {vs[0], vs[1]}};
-  // Heads of a block: as many as leave 8 blocks to an SM.
+  // Heads of a block: as many as leave the blocks that run at once, two to an SM.
   const int64_t runs = (batch->rows + RUN - 1) / RUN, groups = (pages->heads + HEADS - 1) / HEADS;
-  const int heads = HEADS * (int)std::clamp<int64_t>(runs * groups / (8 * SMS), 1, groups);
+  const int heads = HEADS * (int)std::clamp<int64_t>((runs * groups + 2 * SMS - 1) / (2 * SMS), 1, groups);
   const dim3 grid((unsigned)runs, (unsigned)((pages->heads + heads - 1) / heads));
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto pick = [&](auto bf, auto e4, auto s8) {
