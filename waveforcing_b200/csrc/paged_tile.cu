@@ -27,9 +27,10 @@
 // 512 bytes a row and tile: 525 against 398 us without at 9472 x 16384 x 4
 // heads, where the rows' reads and the operands' share shared memory.
 //
-// Measured at that size: bf16 248 us, 1285 TFLOP/s (0.77 of the cuBLAS burst
-// rate), e4m3 335-360 us; 4680 x 37440 x 12 heads: bf16 903 us over 128-row
-// pages and 1010 over 1560-row ones, e4m3 1325 us.  A tile takes about 3600 clocks
+// Measured at that size: bf16 247 us, 1288 TFLOP/s (0.77 of the cuBLAS burst
+// rate), e4m3 341 us; 4680 x 37440 x 12 heads: bf16 904 us over 128-row pages
+// and 1000 over 1560-row ones, e4m3 1307 us; 6 x 4680 rows over 512 states and
+// 12 heads 123 us.  A tile takes about 3600 clocks
 // where its products take 2048: a warp's chain from S to P (load, maximum,
 // exponentials, store) is as long as the other sub-tile's products cover.  8-bit
 // pages: the expansion's shared-memory traffic, and the roles' code, which
