@@ -595,3 +595,19 @@ def test_cross_attention_into_rows_that_are_not_32_byte_aligned():
     K().cross_attention(q, k, k, out=room[..., 8:])
     assert torch.equal(room[..., 8:], want) and (room[..., :8] == 7.0).all()
     healthy()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "e4m3", "s8"])
+def test_single_tokens_of_many_sequences(dtype):
+    """Each CTA of the few-row kernel walks several sequences, over runs of such as have no new token."""
+    g = torch.Generator().manual_seed(21)
+    lens = torch.randint(0, 200, (700,), generator=g).tolist()
+    new = (torch.rand(700, generator=g) < 0.7).int().tolist()
+    new[100:150] = [0] * 50
+    pool = Pool(dtype, lens, 2, 16, seed=22)
+    check_attention(pool, new, 4, block=1, hints=(1, 200))
+    lens = torch.randint(1, 3000, (40,), generator=g).tolist()  # cut into equal stretches
+    new = (torch.rand(40, generator=g) < 0.7).int().tolist()
+    pool = Pool(dtype, lens, 2, 64, seed=23)
+    check_attention(pool, new, 4, block=1, hints=(1, 3000))
+    healthy()

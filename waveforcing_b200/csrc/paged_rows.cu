@@ -207,30 +207,36 @@ __global__ void __launch_bounds__(THREADS, 2)
   auto next_stage = [&]() {
     if (++st == cut.stages) st = 0, ++turn;
   };
-  // The CTA's items in turn, each with the tiles that it has to do.
+  // The CTA's items in turn, each with the tiles that it has to do.  A warp's
+  // lanes share `it`: lane 0 writes it, after all of them have read what it held.
   int item, i;
+  auto open_from = [&](int b) {  // the first sequence with items from b on
+    Item x;
+    do open_sequence<BN>(x, ky, qr, cut, b++);
+    while (x.n == 0);
+    __syncwarp();
+    if (lane == 0) it = x;
+    __syncwarp();
+  };
   {
-    open_sequence<BN>(it, ky, qr, cut, spot.b);
+    open_from(spot.b);
     const long long off = spot.pos - spot.first;
     item = (int)(off / it.t);
     i = (int)(off - (long long)item * it.t);
   }
   auto open_item = [&]() {
-    it.rt = item / G;
-    it.hk = item - it.rt * G;
-    const int n = (int)min((long long)(it.t - i), left);
-    it.i0 = i, it.i1 = i + n;
+    const int rt = item / G, n = (int)min((long long)(it.t - i), left);
     left -= n;
+    __syncwarp();
+    if (lane == 0) it.rt = rt, it.hk = item - rt * G, it.i0 = i, it.i1 = i + n;
     __syncwarp();
   };
   auto next_item = [&]() -> bool {
     if (left == 0) return false;
-    __syncwarp();  // (all lanes write the item, the same)
     i = 0;
     if (++item == it.n) {
       item = 0;
-      do open_sequence<BN>(it, ky, qr, cut, it.b + 1);
-      while (it.n == 0);
+      open_from(it.b + 1);
     }
     return true;
   };
