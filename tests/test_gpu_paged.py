@@ -611,3 +611,69 @@ def test_single_tokens_of_many_sequences(dtype):
     pool = Pool(dtype, lens, 2, 64, seed=23)
     check_attention(pool, new, 4, block=1, hints=(1, 3000))
     healthy()
+
+
+def set_keys(pool, rows):
+    """Gives the first len(rows) positions of the only sequence (all heads) the K rows `rows` [n, 128] f64,
+    quantised as the write does; rows of zeros by turns as written (scale 2^-100 / Q) and as never written."""
+    for p, x in enumerate(rows):
+        page, row = pool.table[0][p // pool.ps], p % pool.ps
+        if pool.dtype == BF:
+            pool.pages.k[page, :, row] = x.to(BF).to(DEV)
+            pool.val[0][page, :, row] = x.to(BF).double()
+            continue
+        codes, scale = O.quant_rows(x.to(BF), pool.dtype)
+        scale = scale.float() * (0.0 if p % 2 and not x.any() else 1.0)
+        stored = codes.float().to(torch.float8_e4m3fn).view(torch.uint8) if pool.dtype == E4 else codes.to(S8)
+        pool.pages.k[page, :, row], pool.pages.k_scale[page, :, row] = stored.to(DEV), scale.to(DEV)
+        pool.val[0][page, :, row] = codes * scale.double()
+
+
+# new tokens: the few-row and the many-row kernel, one and two sub-tiles
+NEW = [3, 100, 150]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "e4m3", "s8"])
+@pytest.mark.parametrize("new", NEW)
+@pytest.mark.parametrize("block", [0, 1])
+def test_queries_and_keys_of_zeros(dtype, new, block):
+    """Scores of 0 in tiles that end inside and that rows see in part: the mean of V, not NaN."""
+    for tiny in (0.0, 2.0 ** -120):
+        q = torch.full((new, 2, 128), tiny).to(BF)
+        q[::3] = torch.randn((len(q[::3]), 2, 128), generator=torch.Generator().manual_seed(30)).to(BF)
+        pool = Pool(dtype, [300], 2, 64, seed=31)
+        check_attention(pool, [new], 2, block, q=q)  # zero queries over ordinary keys
+        check_attention(pool, [new], 2, block, window=130, sink=3, q=q)
+        set_keys(pool, torch.zeros(300, 128, dtype=torch.float64))
+        check_attention(pool, [new], 2, block, q=q)
+        check_attention(pool, [new], 2, block, window=130, sink=3, q=q)
+    healthy()
+
+
+@pytest.mark.parametrize("dtype", [E4, S8], ids=["e4m3", "s8"])
+def test_an_empty_pool_gives_zeros(dtype):
+    """As a warm-up calls it: zero queries over pages that were never written."""
+    pages = K().KVPages.empty(8, 2, 64, dtype, DEV)
+    t = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    for new in NEW:
+        q = torch.zeros((new, 4, 128), dtype=BF, device=DEV)
+        o, lse = K().paged_attention(q, pages, t([list(range(8))]), t([0, new]), t([300]), return_lse=True)
+        assert (o == 0).all() and (lse - math.log(300)).abs().max() <= 2e-4 + 1e-6 * math.log(300)
+    healthy()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "e4m3", "s8"])
+@pytest.mark.parametrize("ps", [16, 48, 128])
+def test_bad_page_ids_over_every_type(dtype, ps):
+    """Whole tiles and parts of them out of the pool; zero query rows among the others."""
+    from waveforcing_b200 import _lib
+
+    for new in NEW:
+        pool = Pool(dtype, [700], 2, ps, seed=32)
+        for j in [0, 1, *range(256 // ps, 384 // ps), -1]:
+            pool.table[0][j] = -5 if j % 2 else 10 ** 6
+        q = torch.randn((new, 4, 128), generator=torch.Generator().manual_seed(33)).to(BF)
+        q[::2] = 0
+        for block in (0, 1):
+            check_attention(pool, [new], 4, block, q=q)
+            assert _lib.status_take() == 1 << 9
