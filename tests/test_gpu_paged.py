@@ -677,3 +677,23 @@ def test_bad_page_ids_over_every_type(dtype, ps):
         for block in (0, 1):
             check_attention(pool, [new], 4, block, q=q)
             assert _lib.status_take() == 1 << 9
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "e4m3", "s8"])
+@pytest.mark.parametrize("new", NEW)
+def test_products_beyond_f32(dtype, new):
+    """|q| |k| above f32's range where q.k is 0 (a score of 0) or far below 0 (no weight)."""
+    keys = torch.randn((300, 128), generator=torch.Generator().manual_seed(34)).double()
+    keys[:, :2] = 0
+    keys[5], keys[200] = 0.0, 0.0
+    keys[5, 1], keys[200, 0] = 2.0 ** 100, -(2.0 ** 100)
+    q = torch.zeros((new, 2, 128))
+    q[..., 0] = 2.0 ** 100
+    pool = Pool(dtype, [300], 2, 64, seed=35)
+    set_keys(pool, keys)
+    cu, plan = pool.plan([new])
+    got, lse = K().paged_attention(q.to(BF).to(DEV), pool.pages, *plan, return_lse=True)
+    ref, ref_lse, _ = O.paged_attention(q.to(BF), *pool.val, pool.table, cu, pool.lens, 0, 0, 0, SCALE)
+    mag, _, _ = O.paged_attention(q.to(BF), pool.val[0], pool.val[1].abs(), pool.table, cu, pool.lens, 0, 0, 0, SCALE)
+    close(got, lse, ref, ref_lse, mag, 0.0 if dtype == BF else 2 ** -11)  # every score is 0 or has no weight: none moves
+    healthy()

@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(THREADS, 2)
           }
         }
     }
-    const float q_scale[2] = {q_pow[0] * qr.scale_log2, q_pow[1] * qr.scale_log2};
+    const float q_scale[2] = {fmaxf(q_pow[0] * qr.scale_log2, 0x1p-126f), fmaxf(q_pow[1] * qr.scale_log2, 0x1p-126f)};
 
     float o[16][4];
 #pragma unroll
@@ -460,14 +460,16 @@ __global__ void __launch_bounds__(THREADS, 2)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[nt][e] = c0[e] + c1[e];
       }
-      // Scores in log2 units, -inf where the row does not see the key.
+      // Scores short of q_scale (together with a key's scale it may pass f32's
+      // range, and its product with a score of 0 be NaN), -inf where the row does
+      // not see the key; maxima in log2 units.
       float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int k = nt * 8 + key_of(2 * t + (e & 1));
-          s[nt][e] *= KV8 ? q_scale[e >> 1] * scale[k] : qr.scale_log2;
+          if (KV8) s[nt][e] *= scale[k];
           if (!whole && !(keep[e >> 1] >> k & 1)) s[nt][e] = -INFINITY;
           mx[e >> 1] = max_nan(mx[e >> 1], s[nt][e]);
         }
@@ -476,7 +478,7 @@ __global__ void __launch_bounds__(THREADS, 2)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         mx[e] = max_nan(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
-        mx[e] = max_nan(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
+        mx[e] = max_nan(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2)) * q_scale[e];
         grow |= !(mx[e] <= m_run[e] + 8.f);
       }
       float v_new = v_top;
@@ -515,7 +517,7 @@ __global__ void __launch_bounds__(THREADS, 2)
         float x[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          x[e] = ex2_approx(s[nt][e] - m_use[e >> 1]);
+          x[e] = ex2_approx(fmaf(s[nt][e], q_scale[e >> 1], -m_use[e >> 1]));
           l_run[e >> 1] += x[e];
         }
         if constexpr (KV8) {

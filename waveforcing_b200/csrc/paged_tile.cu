@@ -952,8 +952,9 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
             for (int c = 0; c < 4; ++c) mc[c] = max3_nan(mc[c], s[k + c], s[k + 4 + c]);
           mx = max3_nan(max3_nan(mc[0], mc[1], mc[2]), mc[3], mc[3]);
         }
-        // (rows of zeros have powers whose product is 0 in f32, and -inf * 0 is NaN)
-        const float scale = KV8 ? fmaxf(q_scale * kpow[m], 0x1p-126f) : qr.scale_log2;
+        // (rows of zeros have powers whose product is 0 in f32, huge ones infinity: times
+        // -inf and times a score of 0 that would be NaN)
+        const float scale = KV8 ? fminf(fmaxf(q_scale * kpow[m], 0x1p-126f), 3.402823466e38f) : qr.scale_log2;
         const float mx2 = mx * scale;
         // O is rescaled only when the maximum grows by more than 2^8; l and O
         // use the same stale maximum, so the quotient does not change.  A NaN
