@@ -697,3 +697,22 @@ def test_products_beyond_f32(dtype, new):
     mag, _, _ = O.paged_attention(q.to(BF), pool.val[0], pool.val[1].abs(), pool.table, cu, pool.lens, 0, 0, 0, SCALE)
     close(got, lse, ref, ref_lse, mag, 0.0 if dtype == BF else 2 ** -11)  # every score is 0 or has no weight: none moves
     healthy()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "e4m3", "s8"])
+def test_scores_beyond_2_to_the_28(dtype):
+    """Few rows with scores of about 2^34, where f32 has steps of 2^10: the largest takes all."""
+    g = torch.Generator().manual_seed(36)
+    keys = (torch.randn((300, 128), generator=g) * 2.0 ** 16).double()
+    q = (torch.randn((3, 2, 128), generator=g) * 2.0 ** 18).to(BF)
+    pool = Pool(dtype, [300], 2, 64, seed=37)
+    set_keys(pool, keys)
+    cu, plan = pool.plan([3])
+    got = K().paged_attention(q.to(DEV), pool.pages, *plan).double().cpu()
+    k, v = (torch.cat([pool.val[i][page] for page in pool.table[0]], 1)[:, :300] for i in range(2))  # [heads, keys, 128]
+    s = torch.einsum("rhd,hkd->rhk", q.double(), k) * SCALE
+    top = s.topk(2, -1)
+    assert (top.values[..., 0] - top.values[..., 1]).min() > 2.0 ** 20  # far above f32's steps of the sum
+    want = torch.stack([v[h][top.indices[:, h, 0]] for h in range(2)], 1)
+    assert ((got - want).abs() <= (2 ** -8 + (0 if dtype == BF else 2 ** -11)) * want.abs()).all()
+    healthy()

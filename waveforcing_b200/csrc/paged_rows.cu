@@ -403,7 +403,7 @@ __global__ void __launch_bounds__(THREADS, 2)
           }
         }
     }
-    const float q_scale[2] = {fmaxf(q_pow[0] * qr.scale_log2, 0x1p-126f), fmaxf(q_pow[1] * qr.scale_log2, 0x1p-126f)};
+    const float q_scale[2] = {q_pow[0] * qr.scale_log2, q_pow[1] * qr.scale_log2};
 
     float o[16][4];
 #pragma unroll
@@ -460,16 +460,17 @@ __global__ void __launch_bounds__(THREADS, 2)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[nt][e] = c0[e] + c1[e];
       }
-      // Scores short of q_scale (together with a key's scale it may pass f32's
-      // range, and its product with a score of 0 be NaN), -inf where the row does
-      // not see the key; maxima in log2 units.
+      // Scores in log2 units, -inf where the row does not see the key.  One factor
+      // at a time: the product of both may pass f32's range, and then make NaN of a
+      // score of 0.  The maximum is subtracted from rounded scores: in one
+      // multiply-add the largest of a row of scores above 2^28 would not become 0.
       float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int k = nt * 8 + key_of(2 * t + (e & 1));
-          if (KV8) s[nt][e] *= scale[k];
+          s[nt][e] = KV8 ? s[nt][e] * scale[k] * q_scale[e >> 1] : s[nt][e] * qr.scale_log2;
           if (!whole && !(keep[e >> 1] >> k & 1)) s[nt][e] = -INFINITY;
           mx[e >> 1] = max_nan(mx[e >> 1], s[nt][e]);
         }
@@ -478,7 +479,7 @@ __global__ void __launch_bounds__(THREADS, 2)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         mx[e] = max_nan(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
-        mx[e] = max_nan(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2)) * q_scale[e];
+        mx[e] = max_nan(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
         grow |= !(mx[e] <= m_run[e] + 8.f);
       }
       float v_new = v_top;
@@ -517,7 +518,7 @@ __global__ void __launch_bounds__(THREADS, 2)
         float x[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          x[e] = ex2_approx(fmaf(s[nt][e], q_scale[e >> 1], -m_use[e >> 1]));
+          x[e] = ex2_approx(s[nt][e] - m_use[e >> 1]);
           l_run[e >> 1] += x[e];
         }
         if constexpr (KV8) {
