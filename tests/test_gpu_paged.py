@@ -716,3 +716,56 @@ def test_scores_beyond_2_to_the_28(dtype):
     want = torch.stack([v[h][top.indices[:, h, 0]] for h in range(2)], 1)
     assert ((got - want).abs() <= (2 ** -8 + (0 if dtype == BF else 2 ** -11)) * want.abs()).all()
     healthy()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "e4m3", "s8"])
+@pytest.mark.parametrize("new,H,G,L,sink_at", [
+    (3, 1, 1, 4200, 0), (3, 1, 1, 4200, 2050), (3, 1, 1, 4200, 4199), (3, 1, 1, 32768, 0),  # few rows
+    (150, 1, 1, 4200, 0), (150, 1, 1, 32768, 0),                                            # in parts
+    (400, 128, 2, 1900, 0), (400, 128, 2, 1900, 1030), (400, 128, 2, 1900, 1899)])          # whole items
+@pytest.mark.parametrize("sink", ["empty", "tiny", "like"])
+def test_weights_far_below_the_largest(dtype, new, H, G, L, sink_at, sink):
+    """One key takes nearly all weight, as an attention sink does, and has no V, little or as much as the
+    others, whose weights are e^-8 to e^-16 of its own.
+
+    The scores are exact (one product of powers of two, or 0) so that d is 0.  Over 8-bit pages weights
+    are f16 with the largest at least 2^7 (many rows) or 2^13 times V's scale over a power of two that is at
+    most 4 times the largest scale (few rows): half of f16's smallest step is 2^-25, so each key may lose
+    2^-25 / 2^7 of the largest weight times its |v|, or 2^-25 / 2^13 * 4 times the largest |v|."""
+    g = torch.Generator().manual_seed(40)
+    k = torch.zeros((L, G, 128))
+    k[sink_at, :, 0] = 16.0
+    v = torch.randn((L, G, 128), generator=g) + 0.5
+    if sink == "like":
+        v[:] = v[1]
+    else:
+        v[sink_at] = 0.0 if sink == "empty" else 2.0 ** -20
+    k, v = k.to(BF), v.to(BF)
+    q = torch.zeros((4, 128))
+    q[:, 0] = torch.tensor([12.0, 14.0, 16.0, 8.0]) / (16 * SCALE)
+    q = q.to(BF)
+    kind = torch.arange(new) % 4
+    ps = 64
+    pages = K().KVPages.empty(L // ps + 1, G, ps, dtype, DEV)
+    t = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    table = t([list(range(L // ps, -1, -1))])
+    K().paged_kv_write(pages, k.to(DEV), v.to(DEV), table, t([0, L]), t([L]))
+    o, lse = K().paged_attention(q[kind][:, None].expand(new, H, 128).contiguous().to(DEV), pages, table, t([0, new]), t([L]),
+                                 return_lse=True)
+    o, lse = o.double().cpu().view(new, G, H // G, 128), lse.double().cpu().view(new, G, H // G)
+    if dtype == BF:
+        kk, vv, lost = k.double(), v.double(), 0.0
+    else:
+        kk, vv = ((c * s.float().double()[..., None]) for c, s in (O.quant_rows(x, dtype) for x in (k, v)))
+        lost = 2 ** -38 * 4 if new == 3 else 2 ** -32
+    keep = torch.ones((4, L), dtype=torch.bool)
+    for h in range(G):
+        ref, ref_lse = O.softmax_rows(q, kk[:, h], vv[:, h], keep, SCALE)
+        mag, _ = O.softmax_rows(q, kk[:, h], vv[:, h].abs(), keep, SCALE)
+        # (the sum of weights over the largest is at least 1; of A this is 2e-3 at most, at e^-16)
+        small = L * lost * (float(vv.abs().max()) if new == 3 else vv[:, h].abs().mean(0))
+        tol = (2 ** -8 + 5e-4 + (2 ** -11 if dtype != BF else 0.0)) * mag + 2 ** -8 * ref.abs() + small
+        err = (o[:, h] - ref[kind][:, None]).abs() / tol[kind][:, None]
+        assert (err <= 1).all(), float(err.max())
+        assert ((lse[:, h] - ref_lse[kind][:, None]).abs() <= 2e-4 + 1e-6 * ref_lse.abs().max()).all()
+    healthy()

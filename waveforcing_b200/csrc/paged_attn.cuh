@@ -275,6 +275,12 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+// Over 8-bit pages P is rounded to f16, which ends at 2^-24 where weights do not: with
+// P of 1 for a row's largest score, keys 17 nats below it were lost, all there is where
+// the largest belongs to a sink without V.  So P is 2^(s - m + bias), up to 2^15; the
+// sum l holds the same power, which leaves the quotient as it was.  Maxima beyond 2^16
+// take none: there m - bias would round.
+__device__ __forceinline__ float p_base(float m, float bias) { return fabsf(m) < 0x1p16f ? m - bias : m; }
 __device__ __forceinline__ uint32_t f16x2(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);

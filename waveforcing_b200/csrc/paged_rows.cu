@@ -168,6 +168,12 @@ __global__ void __launch_bounds__(THREADS, 2)
   constexpr int KC = BN / WARPS;           // keys of a warp
   constexpr int ROWB = KV8 ? 128 : 256;    // bytes of a row
   constexpr int NT = KC / 8;               // score tiles of a warp
+  // Sums are rescaled when a row's maximum grows by more than 2^SLACK, or V's largest
+  // scale beyond the power of two in use, taken with a factor of ROOM.  Both limit P, which
+  // f16 holds as 2^(s - m + 15 - SLACK) * (scale / V's power <= 1): the less they leave, the
+  // smaller the weights that count (4 and 2, 8 and 8 measured the same: 61 us for 32
+  // single tokens).
+  constexpr float SLACK = KV8 ? 2.f : 8.f, ROOM = 2.f;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -480,27 +486,28 @@ __global__ void __launch_bounds__(THREADS, 2)
       for (int e = 0; e < 2; ++e) {
         mx[e] = max_nan(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
         mx[e] = max_nan(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
-        grow |= !(mx[e] <= m_run[e] + 8.f);
+        grow |= !(mx[e] <= m_run[e] + SLACK);
       }
       float v_new = v_top;
       if constexpr (KV8) {
         float top = fabsf(scale[MAX_BN + lane]);  // 0 where a key is not seen at all
         if (!(top < INFINITY)) top = 0.f;
         top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-        if (v_top == 0.f || top > v_top) v_new = pow2_above(top) * 8.f;
+        if (v_top == 0.f || top > v_top) v_new = pow2_above(top) * ROOM;
       }
-      // Sums are rescaled only when a row's maximum grows by more than 2^8, or
-      // V's largest scale does; a NaN or +inf score makes its row NaN.
+      // A NaN or +inf score makes its row NaN.
       if (__any_sync(0xffffffffu, grow) || v_new != v_top) {
         float al[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           al[e] = 1.f;
-          if (!(mx[e] <= m_run[e] + 8.f)) {
+          if (!(mx[e] <= m_run[e] + SLACK)) {
             const float m_new = mx[e] < INFINITY ? mx[e] : __uint_as_float(0x7FC00000u);
-            al[e] = exp2f(m_run[e] - m_new);
+            const float m_old = m_run[e] == -INFINITY ? -INFINITY : m_use[e];
+            m_run[e] = m_new;
+            m_use[e] = KV8 ? p_base(m_new, 15.f - SLACK) : m_new;
+            al[e] = exp2f(m_old - m_use[e]);
             l_run[e] *= al[e];
-            m_run[e] = m_use[e] = m_new;
           }
           if (KV8) al[e] *= v_top / v_new;
         }
@@ -571,7 +578,8 @@ __global__ void __launch_bounds__(THREADS, 2)
     // The warps' sums, and from them the item's (or this CTA's part of them), a
     // thread to a dim.
     float* mine = sums + warp * cut.height * (O_PITCH + 2);
-    if (KV8 && v_top == 0.f) v_top = 1.f;
+    constexpr float P_TOP = KV8 ? 0x1p15f : 1.f;  // taken out of O here: l * V may pass f32's range
+    const float v_back = KV8 ? (v_top == 0.f ? 1.f : v_top / P_TOP) : 1.f;
     named_bar_sync(1, WARPS * 32);  // the last item's have been read
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -580,7 +588,7 @@ __global__ void __launch_bounds__(THREADS, 2)
       const int r = g + e * 8;
       if (r >= n_rows) continue;
       if (t == 0) {
-        mine[cut.height * O_PITCH + r] = m_run[e];
+        mine[cut.height * O_PITCH + r] = m_run[e] == -INFINITY ? -INFINITY : m_use[e];
         mine[cut.height * (O_PITCH + 1) + r] = l_run[e];
       }
 #pragma unroll
@@ -588,7 +596,7 @@ __global__ void __launch_bounds__(THREADS, 2)
 #pragma unroll
         for (int f = 0; f < 2; ++f) {
           const int d = KV8 ? (2 * t + f) * 16 + k : k * 8 + 2 * t + f;
-          mine[r * O_PITCH + d] = KV8 ? o[k][2 * e + f] * v_top : o[k][2 * e + f];
+          mine[r * O_PITCH + d] = o[k][2 * e + f] * v_back;
         }
     }
     named_bar_sync(1, WARPS * 32);
@@ -610,7 +618,7 @@ __global__ void __launch_bounds__(THREADS, 2)
         x += wt * sums[w * pitch + r * O_PITCH + dim];
       }
       const bool none = m == -INFINITY;
-      const float inv = none ? 0.f : m != m ? m : 1.f / l;
+      const float inv = none ? 0.f : m != m ? m : P_TOP / l;
       const float lse2 = none ? -INFINITY : m + log2f(l);
       if (complete) {
         store_row(ky, qr, it.b, it.sp.first, it.hk, r + it.rt * cut.height, dim, none ? 0.f : x * inv, lse2);

@@ -53,6 +53,10 @@ constexpr int HALF = 16384;       // 128 rows x 64 bf16
 constexpr int SLOT = 2 * HALF;    // a K or V tile, or a Q sub-tile: [d 0-63][d 64-127]
 constexpr int META = 4;           // tiles whose marks (and scales) are kept
 constexpr uint32_t COL_S = 0, COL_O = 256;
+// O is rescaled only when a row's maximum grows by more than 2^SLACK (4680 x 14040 x 12
+// heads over e4m3, scores of deviation 1: 550 us; with 4, which would leave P over 8-bit
+// pages more of f16's range, 601).
+constexpr float SLACK = 8.f;
 
 constexpr int WORK_BYTES = 96, WORKS = 4;  // items found ahead
 template <bool KV8>
@@ -907,7 +911,9 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
       const int i = w.i0 + u * tl.tq + row / qr.group, h = w.hk * qr.group + row % qr.group;
       const bool has_row = row < tl.tq * qr.group && i < w.sp.n;
       const Sees se = sees(qr, w.sp, min(i, w.sp.n - 1));
-      float m_run = -INFINITY, m_use = 0.f;  // the maximum in use; 0 while nothing has been seen
+      // The maximum in use, -inf while nothing has been seen, and what P's exponents
+      // are taken from (0 then).
+      float m_run = -INFINITY, m_use = 0.f;
       float l_run = 0.f, v_run = 1.f, q_scale = 0.f;
       for (int j = 0; j < nt; ++j, ++sn, ++tiles) {
         ok = warp_wait(&bar_s[u], sn, abort_flag, ST_PAGED_SOFTMAX);
@@ -956,17 +962,18 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
         // -inf and times a score of 0 that would be NaN)
         const float scale = KV8 ? fminf(fmaxf(q_scale * kpow[m], 0x1p-126f), 3.402823466e38f) : qr.scale_log2;
         const float mx2 = mx * scale;
-        // O is rescaled only when the maximum grows by more than 2^8; l and O
-        // use the same stale maximum, so the quotient does not change.  A NaN
-        // or +inf score makes the row NaN from here on.
-        const bool grow = !(mx2 <= m_run + 8.f);
+        // l and O use the same stale maximum, so the quotient does not change.  A
+        // NaN or +inf score makes the row NaN from here on.
+        const bool grow = !(mx2 <= m_run + SLACK);
         const float v_new = KV8 ? vpow[m] : 1.f;
         if (__any_sync(0xffffffffu, grow) || (KV8 && v_new != v_run)) {
           float alpha = 1.f;
           if (grow) {
             const float m_new = mx2 < INFINITY ? mx2 : __uint_as_float(0x7FC00000u);
-            alpha = ex2_approx(m_run - m_new);
-            m_run = m_use = m_new;
+            const float m_old = m_run == -INFINITY ? -INFINITY : m_use;
+            m_run = m_new;
+            m_use = KV8 ? p_base(m_new, 15.f - SLACK) : m_new;
+            alpha = ex2_approx(m_old - m_use);
             l_run *= alpha;
           }
           if (KV8) alpha *= v_run / v_new;
@@ -1046,7 +1053,7 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
       const bool none = m_run == -INFINITY;
       const float inv = none ? 0.f : m_run != m_run ? m_run : v_run / l_run;
       const int64_t packed = (int64_t)(w.sp.first + i) * qr.H + h;
-      const float lse2 = none ? -INFINITY : m_run + log2f(l_run);
+      const float lse2 = none ? -INFINITY : m_use + log2f(l_run);
       if (tl.splits > 1 || w.slot >= 0) {
         const int64_t at = w.slot >= 0 ? (int64_t)w.slot * (2 * BM) + u * BM + row
                                        : (int64_t)w.split * qr.rows * qr.H + packed;
