@@ -769,3 +769,14 @@ def test_weights_far_below_the_largest(dtype, new, H, G, L, sink_at, sink):
         assert (err <= 1).all(), float(err.max())
         assert ((lse[:, h] - ref_lse[kind][:, None]).abs() <= 2e-4 + 1e-6 * ref_lse.abs().max()).all()
     healthy()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=["bf16", "e4m3", "s8"])
+def test_what_an_earlier_call_left_on_the_chip_does_not_matter(dtype):
+    """Groups that do not divide 128 leave rows of a Q tile without a token."""
+    pool = Pool(dtype, [2500], 4, 64, seed=50)
+    nan = torch.full((1200, 4, 128), float("nan"), dtype=BF, device=DEV)
+    for H in (12, 20, 24):
+        K().paged_attention(nan, pool.pages, *pool.plan([1200])[1])
+        check_attention(pool, [130], H, block=1)
+    healthy()
