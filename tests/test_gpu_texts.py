@@ -63,3 +63,17 @@ def test_engine_changes_texts_along_the_chunks():
     assert torch.isfinite(a).all() and _cos(a, b) >= 0.999
     # one text of several is that text alone
     assert _cos(_run("wf_b200", True, (0,)), _run("wf_b200", False)) >= 0.999
+
+
+def test_a_new_list_of_texts_does_not_wait_for_the_device():
+    from waveforcing_b200.wavefront.dit import StageTask
+
+    model, dev = _model(True, [16, 5, 0])
+    tasks = [[StageTask(None, 600.0, 0, 0, text=n) for n in texts] for texts in ([0, 1], [2, 2, 1], [1])]
+    torch.cuda.synchronize()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        got = [model._text_index(t) for t in tasks]
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    assert [g.tolist() for g in got] == [[0, 1], [2, 2, 1], [1]] and all(g.dtype == torch.int32 for g in got)

@@ -80,3 +80,14 @@ def test_engine_chunks_follow_the_last_text_from_then_on():
     cfg = EngineConfig(texts=(0, 0, 2, 1))
     assert [cfg.text_of(c) for c in range(6)] == [0, 0, 2, 1, 1, 1]
     assert EngineConfig().text_of(5) == 0
+
+
+def test_lists_of_texts_leave_nothing_behind(model):
+    """A text per chunk gives a new list every tick."""
+    model.set_text(model._test_texts)
+    kept = lambda: {k: len(v) for k, v in vars(model).items() if hasattr(v, "__len__")}  # noqa: E731
+    model.forward_stages(_tasks(model, [0, 0, 0]), fused=False)
+    before = kept()
+    for n in range(27):
+        model.forward_stages(_tasks(model, [n // 9, n // 3 % 3, n % 3]), fused=False)
+    assert kept() == before

@@ -190,8 +190,7 @@ class WanDiT(nn.Module):
         self.head_norm_mod = nn.Parameter(torch.randn(1, 2, d) / d**0.5)
         self.head = nn.Linear(d, cfg.out_ch * math.prod(cfg.patch))
         self._cross_kv = None
-        self._texts = None  # several texts: (their number, int32 lengths or None)
-        self._text_indices: dict = {}
+        self._texts = None  # several texts: (0 .. N - 1 in int32, int32 lengths or None)
 
     @classmethod
     def random(cls, cfg: DiTConfig, device, dtype=torch.bfloat16, seed: int = 0) -> "WanDiT":
@@ -229,20 +228,17 @@ class WanDiT(nn.Module):
         self._cross_kv = kv
         self._texts = None
         if text.dim() == 3:
-            self._texts = (N, None if lens is None else torch.tensor(lens, dtype=torch.int32, device=ctx.device))
+            self._texts = (torch.arange(N, dtype=torch.int32, device=ctx.device),
+                           None if lens is None else torch.tensor(lens, dtype=torch.int32, device=ctx.device))
 
-    def _text_index(self, tasks: list, dev) -> torch.Tensor | None:
-        """The tasks' texts as an int32 device tensor (kept: a run has few
-        different lists); None when there is one text for all."""
-        texts = tuple(t.text for t in tasks)
-        if not all(0 <= n < (self._texts[0] if self._texts else 1) for n in texts):
-            raise ValueError(f"forward_stages: texts {texts} name one that set_text was not given")
-        if self._texts is None:
-            return None
-        got = self._text_indices.get((texts, dev))
-        if got is None:
-            got = self._text_indices[(texts, dev)] = torch.tensor(texts, dtype=torch.int32, device=dev)
-        return got
+    def _text_index(self, tasks: list) -> torch.Tensor | None:
+        """The tasks' texts as an int32 device tensor, put together on the device
+        (a copy of new host data would wait for it); None when there is one text
+        for all."""
+        texts = [t.text for t in tasks]
+        if not all(0 <= n < (len(self._texts[0]) if self._texts else 1) for n in texts):
+            raise ValueError(f"forward_stages: texts {tuple(texts)} name one that set_text was not given")
+        return torch.cat([self._texts[0][n:n + 1] for n in texts]) if self._texts else None
 
     def time_mod(self, timestep: float, device):
         """Per-stage modulation inputs: e [6, dim] f32 and e_head [2, dim] f32.
@@ -329,7 +325,7 @@ class WanDiT(nn.Module):
         H, D, dim = cfg.heads, cfg.head_dim, cfg.dim
         order = sorted(range(S), key=lambda i: -tasks[i].stage)  # publish before consume
         keep = [i for i in range(S) if not tasks[i].kv_only]  # tasks whose flow output is returned
-        text_index = self._text_index(tasks, dev)
+        text_index = self._text_index(tasks)
         x = torch.cat([self.patchify(t.latent.to(dt)) for t in tasks], 0)
         x = _lin(self.patch_embedding, x)  # [S*T, dim]
         mods, heads_e = [], []
@@ -466,7 +462,7 @@ class WanDiT(nn.Module):
                                pending[1].index_select(0, rows).contiguous())
                 heads_e = [heads_e[i] for i in keep]
                 S = len(keep)
-                text_index = self._text_index([tasks[i] for i in keep], dev)
+                text_index = self._text_index([tasks[i] for i in keep])
             y = _lin(b.self_attn.o, o.view(S * T, dim))
             # cross-attention: one call for all stages, of one text or of several
             if fused and w8a8_channel(b.cross_attn.q):
