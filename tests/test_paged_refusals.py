@@ -83,6 +83,15 @@ def test_attention():
         _passes(K.paged_attention, q.clone().requires_grad_(), p, table, cu, lens)
 
 
+def test_attention_ranges():
+    """Beyond 32 bits ctypes would pass on what is left of a number."""
+    p, (table, cu, lens) = pages(), plan()
+    q = torch.zeros(5, 4, 128, dtype=bf)
+    _passes(K.paged_attention, q, p, table, cu, lens, block=2**31 - 1, window=2**31 - 1, sink=2**31 - 1)
+    for bad in [dict(block=2**32 + 1), dict(window=2**32 + 5), dict(window=3, sink=2**32), dict(block=-1), dict(window=-(2**32) + 1)]:
+        _rejects(K.paged_attention, q, p, table, cu, lens, **bad)
+
+
 def test_cross_attention():
     q, k = torch.zeros(2, 5, 4, 128, dtype=bf), torch.zeros(2, 7, 2, 128, dtype=bf)
     idx = torch.zeros(2, dtype=i32)

@@ -528,6 +528,7 @@ _PACK2, _PACK3 = struct.Struct("2q").pack, struct.Struct("3q").pack
 
 
 _SCALE = 1.0 / math.sqrt(128)
+_I32 = 2**31 - 1
 
 
 def _st2(t: torch.Tensor) -> tuple:
@@ -704,6 +705,8 @@ def paged_attention(q: torch.Tensor, pages: KVPages, page_table: torch.Tensor, c
     if pages.k.get_device() != d:
         raise ValueError("paged_attention: all tensors must be on one device")
     _check(H % G == 0, "paged_attention: query heads must be a multiple of the K/V heads")
+    if not (0 <= block <= _I32 and 0 <= window <= _I32 and 0 <= sink <= _I32):  # ctypes would cut them off
+        raise ValueError("paged_attention: block, window and sink must be 0 to 2^31 - 1")
     batch = _batch_desc("paged_attention", page_table, cu_new, seq_lens, rows, d)
     if out is None:
         out = q.new_empty((rows, H, 128))
