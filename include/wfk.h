@@ -243,10 +243,12 @@ int wf_paged_kv_read(const wf_kv_pages* pages, const wf_kv_batch* batch, void* k
  * read where they lie instead of from an assembled buffer (paged.py:191-255).
  * A row that sees nothing gives zeros.  lse (f32 [rows, H] dense, or NULL)
  * receives the natural log of the sum of exponentials, -inf for such rows.
- * Keys that no row of the call sees may hold anything, NaN included; a
- * non-finite V row that some query sees can also reach other queries that do
- * not.  Over 8-bit pages weights are held in f16: below 2^-21 of a row's largest
- * they lose bits, and below 2^-32 they no longer count.  max_new and max_len are upper bounds of the sequences' packed rows and
+ * Keys that a row does not see may hold anything, NaN included: what is not
+ * finite in bf16 rows, or a scale that is not, reaches the rows that see it and
+ * no others (8-bit codes are taken as finite, as the write makes them: an e4m3
+ * NaN code can reach all rows).  Over 8-bit pages weights are held in f16: below
+ * 2^-21 of a row's largest they lose bits, and below 2^-32 they no longer count.
+ * max_new and max_len are upper bounds of the sequences' packed rows and
  * lengths: they choose how the work is cut, never what is computed.
  * workspace: wf_paged_attn_workspace bytes of device memory, 16-byte aligned,
  * used by this call alone until it has run (NULL when that is 0). */

@@ -780,3 +780,43 @@ def test_what_an_earlier_call_left_on_the_chip_does_not_matter(dtype):
         K().paged_attention(nan, pool.pages, *pool.plan([1200])[1])
         check_attention(pool, [130], H, block=1)
     healthy()
+
+
+@pytest.mark.parametrize("lens,new,ps,block,window,sink", [
+    ([300], [3], 64, 1, 0, 0), ([300, 40], [7, 7], 16, 1, 50, 3), ([130], [8], 24, 1, 20, 5),    # few rows
+    ([300], [100], 64, 1, 0, 0), ([300, 90], [150, 70], 48, 1, 0, 0), ([500], [260], 16, 1, 60, 5),
+    ([900], [300], 100, 64, 200, 90), ([2500], [300], 390, 195, 0, 0), ([2500], [200], 128, 1, 700, 130)])
+def test_values_that_are_not_finite_reach_only_rows_that_see_them(lens, new, ps, block, window, sink):
+    """bf16 pages, where single elements of V may be NaN or infinite: each reaches its own dim of the rows
+    that see its key, and no other."""
+    pool = Pool(BF, lens, 2, ps, seed=60)
+    cu, plan = pool.plan(new)
+    g = torch.Generator().manual_seed(61)
+    q = torch.randn((cu[-1], 4, 128), generator=g).to(BF)
+    odd = torch.zeros_like(pool.val[1])  # what is not finite, by slot
+    for b, n in enumerate(lens):
+        at = [n - 1, n - 2, n - new[b] // 2, n - new[b], max(n - new[b] - 1, 0), 0, 4, max(n - window - 2, 0), n - n // 3]
+        for i, p in enumerate(at):
+            page, row, head = pool.table[b][p // ps], p % ps, i % 2
+            bad = [float("nan"), float("inf"), -float("inf")][i % 3]
+            dims = slice(0, 128) if i == 3 else torch.randint(0, 128, (3,), generator=g)
+            odd[page, head, row, dims] = bad
+    is_odd = odd != 0
+    pool.pages.v[is_odd.to(DEV)] = odd[is_odd].to(BF).to(DEV)
+    pool.val[1][is_odd] = 0.0  # the oracle sums what is finite
+    got = K().paged_attention(q.to(DEV), pool.pages, *plan, block=block, window=window, sink=sink)
+    args = (pool.table, cu, pool.lens, block, window, sink, SCALE)
+    ref, _, _ = O.paged_attention(q, *pool.val, *args)
+    mag, _, _ = O.paged_attention(q, pool.val[0], pool.val[1].abs(), *args)
+    for b, n in enumerate(lens):
+        v = torch.cat([odd[page] for page in pool.table[b]], 1)[:, :n]  # [heads, keys, 128]
+        for i in range(new[b]):
+            keep = O.visible(n - new[b] + i, n, block, window, sink)
+            for h in range(4):
+                ref[cu[b] + i, h] += v[h // 2][keep].sum(0)
+    o, fin = got.double().cpu(), torch.isfinite(ref)
+    assert 0 < (~fin).sum() < fin.numel()
+    assert torch.equal(torch.isfinite(o), fin)
+    assert torch.equal(torch.isnan(o), torch.isnan(ref)) and torch.equal(o[torch.isinf(ref)], ref[torch.isinf(ref)])
+    assert ((o - ref).abs()[fin] <= tolerance(ref, mag)[fin]).all()
+    healthy()

@@ -261,6 +261,24 @@ __device__ __forceinline__ bool inside(const Range& r, const TileAt& a) {
 }
 __device__ __forceinline__ bool seen(const Range& r, int pos) { return (pos < r.hi && pos >= r.lo) || pos < r.sink; }
 
+// Whether some tokens see a key of the tile that others do not.  There a V row of
+// bf16 pages may hold a NaN or an infinity that its P of 0 would hand to the others:
+// such elements are taken out and given to the rows that see them.
+template <int BN>
+__device__ __forceinline__ bool mixed(const Range& r, const TileAt& a) {
+  return (r.hi != r.hi_min || r.lo != r.lo_max || r.sink != r.sink_min) &&
+         !(a.base + BN <= r.hi_min && (a.base >= r.lo_max || a.base + BN <= r.sink_min));
+}
+__device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+// Bits 15 and 31: which of two bf16 are not finite.
+__device__ __forceinline__ uint32_t not_finite2(uint32_t w) { return ((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u; }
+// The pair with what is not finite made 0.
+__device__ __forceinline__ uint32_t finite2(uint32_t w) { return w & ~((not_finite2(w) >> 15) * 0xFFFFu); }
+
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, uint32_t code) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity & 1, abort, code));
 }

@@ -518,6 +518,34 @@ __global__ void __launch_bounds__(THREADS, 2)
           o[k][2] *= al[1], o[k][3] *= al[1];
         }
       }
+      if constexpr (!KV8) {
+        if (!whole && mixed<BN>(it.rg, tile_at<BN>(tl, mark.y))) {
+          uint32_t odd = 0;  // rows of V that are not finite: half a warp to a row
+#pragma unroll
+          for (int r = lane >> 4; r < KC; r += 2) {
+            const uint4 x = *reinterpret_cast<const uint4*>(V + ((lane >> 3) & 1) * (STAGE / 4) + r * 128 + (lane & 7) * 16);
+            if (not_finite2(x.x) | not_finite2(x.y) | not_finite2(x.z) | not_finite2(x.w)) odd |= 1u << r;
+          }
+          for (odd = __reduce_or_sync(0xffffffffu, odd); odd; odd &= odd - 1) {
+            const int r = __ffs(odd) - 1;
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              uint32_t* at = reinterpret_cast<uint32_t*>(V + (k >> 3) * (STAGE / 4) + r * 128 + (((k & 7) ^ (r & 7)) << 4)) + t;
+              const uint32_t w = *at, bad = w & ~finite2(w);
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if (bad && (keep[e] >> r & 1)) {
+                  o[k][2 * e] += __uint_as_float(bad << 16);
+                  o[k][2 * e + 1] += __uint_as_float(bad & 0xFFFF0000u);
+                }
+              __syncwarp();
+              if (g == 0) *at = finite2(w);
+            }
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+      }
       const float v_inv = KV8 ? 1.f / v_top : 1.f;
       uint32_t p[NT / 2][4];  // as the A operand of P V: [rows g | g + 8][keys 2t | 2t + 8]
 #pragma unroll

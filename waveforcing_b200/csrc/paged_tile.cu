@@ -6,8 +6,10 @@
 //   warp 0       TMA producer (a lane to a box of a tile)
 //   warp 1       MMA issue: S_u = Q_u K_j^T (M=N=K=128), O_u += P_u V_j
 //   warp 2       marks the live keys of each tile; bf16: zeroes the V rows of
-//                the others (their P is 0, but 0 * NaN is not); 8 bits: fetches
-//                scales, a tile ahead of the codes
+//                the others (their P is 0, but 0 * NaN is not), and what is not
+//                finite in tiles that some rows see and others do not (the rows
+//                that do get it back at their end); 8 bits: fetches scales, a
+//                tile ahead of the codes
 //   warp 3       finds the CTA's items ahead of the other roles
 //   warps 4-11   softmax; warpgroup u owns sub-tile u, a thread a row
 //   warps 12-15  (8-bit pages) expand codes to f16
@@ -77,7 +79,27 @@ struct Work : Range {
   int t0, t1;        // this item's share of the tile list
   int slot;          // its partial rows' place in the workspace, -1: none (see Deal)
 };
-static_assert(sizeof(Work) <= WORK_BYTES, "room for an item");
+static_assert(sizeof(Work) + 4 <= WORK_BYTES, "room for an item");
+
+// Page (of the sequence) and row of key r of a tile; false: a hole.
+template <int N>
+__device__ __forceinline__ bool place(const Tiling& tl, const TileAt& a, int r, int& page, int& row) {
+  page = a.page;
+  row = a.row + r;
+  if (tl.dense) {
+    if (row >= tl.ps) {
+      const int j = page_of(tl, row);
+      page += j;
+      row -= j * tl.ps;
+    }
+  } else if (tl.ps < N) {
+    const int j = r / tl.rows;
+    page += j;
+    row = r - j * tl.rows;
+    if (j >= tl.boxes) return false;
+  }
+  return row < tl.ps;
+}
 
 // Query tiles of the launch over all sequences (one warp).
 __device__ __forceinline__ int count_tiles(const Keys& ky, const Queries& qr, const Tiling& tl, int lane) {
@@ -359,6 +381,30 @@ __device__ __forceinline__ void store32(void* to, const uint32_t* r, bool wide) 
   }
 }
 
+// Makes the bf16 V tile at v finite; whether it was not (a warp).  Not inlined: in the
+// marks' loop it slowed every call, mixed tiles or none (4680 x 37440 x 12 heads: 1010 us,
+// 907 so, 896 without).
+__device__ __noinline__ bool make_finite(uint8_t* v, int lane) {
+  v += (lane >> 4) * 128 + ((lane >> 3) & 1) * HALF + (lane & 7) * 16;  // half a warp to a row, 16 bytes a lane
+  uint32_t odd[4] = {0, 0, 0, 0};  // sums of 0 * x: 0 or NaN
+#pragma unroll 4
+  for (int r = 0; r < BN; r += 2) {
+    const uint4 x = *reinterpret_cast<const uint4*>(v + r * 128);
+    odd[0] = fma_bf16x2(x.x, 0u, odd[0]), odd[1] = fma_bf16x2(x.y, 0u, odd[1]);
+    odd[2] = fma_bf16x2(x.z, 0u, odd[2]), odd[3] = fma_bf16x2(x.w, 0u, odd[3]);
+  }
+  if (!__any_sync(0xffffffffu, ((odd[0] | odd[1] | odd[2] | odd[3]) & 0x7FFF7FFFu) != 0)) return false;
+#pragma unroll 1
+  for (int r = 0; r < BN; r += 2) {
+    uint4* at = reinterpret_cast<uint4*>(v + r * 128);
+    const uint4 x = *at;
+    *at = make_uint4(finite2(x.x), finite2(x.y), finite2(x.z), finite2(x.w));
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+  return true;
+}
+
 template <int DT, bool SORTED>
 __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
     tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ PageMaps tm,
@@ -393,6 +439,7 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(live) + Cfg<KV8>::META_BYTES);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   Work* works = reinterpret_cast<Work*>(reinterpret_cast<uint8_t*>(tmem_slot) + 16);  // [WORKS]
+  volatile int* odd_v = reinterpret_cast<volatile int*>(works + WORKS);  // [WORKS] V of a mixed tile of the item is not finite
 
   // Values that steer the roles are broadcast from lane 0, by which the compiler
   // knows them to be the same in a warp: the MMA warp's operands then stay in
@@ -665,22 +712,7 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
       }
       // Key r of a tile: page and row, and whether some row of the item sees it.
       auto key = [&](const TileAt& a, int r, int& page, int& row) -> bool {
-        page = a.page;
-        row = a.row + r;
-        bool in = true;
-        if (tl.dense) {
-          if (row >= tl.ps) {
-            const int j = page_of(tl, row);
-            page += j;
-            row -= j * tl.ps;
-          }
-        } else if (tl.ps < BN) {
-          const int j = r / tl.rows;
-          page += j;
-          row = r - j * tl.rows;
-          in = j < tl.boxes;
-        }
-        return in && row < tl.ps && seen(w, page * tl.ps + row);
+        return place<BN>(tl, a, r, page, row) && seen(w, page * tl.ps + row);
       };
       auto look = [&](const TileAt& a) {
         nx_at = a;
@@ -774,6 +806,8 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
             fence_proxy_async_smem();
             __syncwarp();
           }
+          if (__builtin_expect(mixed<BN>(w, a), 0) && make_finite(ring + s * SLOT, lane) && lane == 0)
+            odd_v[(work_n - 1) % WORKS] = 1;  // (the softmax holds the item until its end)
           if (lane == 0) mbar_arrive(&full[s]);
         }
       }
@@ -873,6 +907,7 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
         ok = ok && (work_n < WORKS || warp_wait(&work_empty[k], work_n / WORKS - 1, abort_flag, ST_PAGED_WORK));
         if (ok && lane == 0) {
           works[k] = w;
+          if (!KV8) odd_v[k] = 0;
           mbar_arrive(&work_full[k]);
         }
         __syncwarp();
@@ -1063,6 +1098,33 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
       const float inv = none ? 0.f : m_run != m_run ? m_run : v_run / l_run;
       const int64_t packed = (int64_t)(w.sp.first + i) * qr.H + h;
       const float lse2 = none ? -INFINITY : m_use + log2f(l_run);
+      // What the marks took out of V, from the pages, for the keys that this row sees.
+      auto add_odd = [&](auto* to) {
+#pragma unroll 1
+        for (int j = w.t0; j < w.t1; ++j) {
+          const TileAt a = tile_at<BN>(tl, nth_tile(w, j));
+          if (!mixed<BN>(w, a)) continue;
+#pragma unroll 1
+          for (int r = 0; r < BN; ++r) {
+            int page, at;
+            if (!place<BN>(tl, a, r, page, at)) continue;
+            const int pos = page * tl.ps + at;
+            if (!((pos >= se.lo && pos < se.hi) || pos < se.sink)) continue;
+            const int id = page_id(ky, w.sp, w.b, page);
+            if (id < 0 || id >= ky.n_pages) continue;
+            const __nv_bfloat16* v =
+                static_cast<const __nv_bfloat16*>(ky.v) + id * ky.v_str[0] + w.hk * ky.v_str[1] + at * ky.v_str[2];
+#pragma unroll 1
+            for (int d = 0; d < HD; d += 2) {
+              const uint32_t x = *reinterpret_cast<const uint32_t*>(v + d), bad = x & ~finite2(x);
+              if (bad) {
+                to[d] = static_cast<float>(to[d]) + __uint_as_float(bad << 16);
+                to[d + 1] = static_cast<float>(to[d + 1]) + __uint_as_float(bad & 0xFFFF0000u);
+              }
+            }
+          }
+        }
+      };
       if (tl.splits > 1 || w.slot >= 0) {
         const int64_t at = w.slot >= 0 ? (int64_t)w.slot * (2 * BM) + u * BM + row
                                        : (int64_t)w.split * qr.rows * qr.H + packed;
@@ -1079,6 +1141,8 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
               for (int v = 0; v < 32; v += 8) store32(part_o + at * HD + c + v, r + v, tl.wide);
             }
           }
+          if constexpr (!KV8)
+            if (odd_v[(work_n - 1) % WORKS] && has_row && !none) add_odd(part_o + at * HD);
         }
       } else {
         if (has_row && qr.lse) qr.lse[packed] = lse2 * 0.6931471805599453f;
@@ -1097,6 +1161,8 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
             store32(d + c + 16, o + 8, tl.wide);
           }
         }
+        if constexpr (!KV8)
+          if (odd_v[(work_n - 1) % WORKS] && has_row && !none) add_odd(d);
       }
       // the next tile's arrival on bar_p lets PV overwrite O, which is in registers here
     }
