@@ -27,15 +27,12 @@ struct Batch {
 
 struct Seq {
   int first, n;  // packed rows
-  int len;       // total length; row i sits at position len - n + i
 };
 
-// Longest length a table of max_pages pages can hold (fits an int by the host check).
-__device__ __forceinline__ Seq seq_of(const Batch& bt, int b, int page_size) {
+__device__ __forceinline__ Seq seq_of(const Batch& bt, int b) {
   Seq s;
   s.first = min(max(__ldg(bt.cu + b), 0), bt.rows);
   s.n = min(max(__ldg(bt.cu + b + 1), s.first), bt.rows) - s.first;
-  s.len = min(max(__ldg(bt.lens + b), 0), bt.max_pages * page_size);
   return s;
 }
 

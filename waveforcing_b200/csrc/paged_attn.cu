@@ -86,7 +86,6 @@ static int64_t workspace_need(const Shape& sh) {
 
 int check_pages(const char* who, const wf_kv_pages* p);
 int check_batch(const char* who, const wf_kv_batch* b, int page_size);
-Batch make_batch(const wf_kv_batch* b);
 
 static int launch(const char* who, const Keys& ky, const Queries& qr, const Shape& sh, void* workspace,
                   int64_t workspace_bytes, void* stream) {

@@ -75,7 +75,7 @@ __device__ __forceinline__ void find_slots(Slots& sl, const Batch& bt, const Poo
     const int b = r < bt.rows ? seq_of_row(bt, r) : -1;
     if (b >= 0) {
       const int n_total = __ldg(bt.lens + b);
-      const Seq s = seq_of(bt, b, pool.page_size);
+      const Seq s = seq_of(bt, b);
       const int pos = n_total - s.n + (r - s.first);
       if (pos >= 0) {
         const int j = pos / pool.page_size;
@@ -109,7 +109,7 @@ __device__ __forceinline__ void drop_overwritten(Slots& sl, const Batch& bt, con
   while (w * 2 * bt.seqs <= THREADS) w *= 2;
   for (int b = threadIdx.x / w; b < bt.seqs; b += THREADS / w) {
     const int total = __ldg(bt.lens + b);
-    const Seq s = seq_of(bt, b, ps);
+    const Seq s = seq_of(bt, b);
     const int base = total - s.n;  // position of the sequence's first packed row
     if (s.n == 0 || total <= 0 || s.first + s.n - 1 <= r0) continue;  // none of its rows is later than the block's first
     const int j1 = min((total - 1) / ps, bt.max_pages - 1);
@@ -345,7 +345,7 @@ int check_batch(const char* who, const wf_kv_batch* b, int page_size) {
   return WF_OK;
 }
 
-Batch make_batch(const wf_kv_batch* b) {
+static Batch make_batch(const wf_kv_batch* b) {
   return Batch{b->table, b->cu, b->lens, b->table_stride, b->seqs, b->max_pages, (int)b->rows};
 }
 
