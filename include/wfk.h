@@ -248,6 +248,7 @@ int wf_paged_kv_read(const wf_kv_pages* pages, const wf_kv_batch* batch, void* k
  * no others (8-bit codes are taken as finite, as the write makes them: an e4m3
  * NaN code can reach all rows).  Over 8-bit pages weights are held in f16: below
  * 2^-21 of a row's largest they lose bits, and below 2^-32 they no longer count.
+ * Scores times log2(e) are taken to be below 2^27 in magnitude.
  * max_new and max_len are upper bounds of the sequences' packed rows and
  * lengths: they choose how the work is cut, never what is computed.
  * workspace: wf_paged_attn_workspace bytes of device memory, 16-byte aligned,

@@ -820,3 +820,32 @@ def test_values_that_are_not_finite_reach_only_rows_that_see_them(lens, new, ps,
     assert torch.equal(torch.isnan(o), torch.isnan(ref)) and torch.equal(o[torch.isinf(ref)], ref[torch.isinf(ref)])
     assert ((o - ref).abs()[fin] <= tolerance(ref, mag)[fin]).all()
     healthy()
+
+
+@pytest.mark.parametrize("dtype", [BF, E4], ids=["bf16", "e4m3"])
+@pytest.mark.parametrize("new", NEW)
+def test_maxima_that_pass_2_to_the_16(dtype, new):
+    """Scores that grow from 65526 to 65543 (times ln 2) along the keys, where the power that f16 weights
+    take for range is given up.  Products of powers of two with the keys' scales, so that no score moves by
+    rounding to f16; f32 steps there are 2^-7, and half of one is lost in the product with the scale and
+    half in the sum: d = 2^-7 ln 2."""
+    q = torch.zeros((new, 2, 128))
+    q[..., 0], q[..., 1], q[..., 2] = 32000.0, 116.0, 15.6875
+    q[1::3, :, 0] *= -1  # and falls from -65526
+    q[2::3, :, 1:] = 0  # all the same
+    keys = torch.zeros((1500, 128), dtype=torch.float64)
+    keys[:, :2] = 16.0
+    keys[:, 2] = torch.tensor([1.0, 2.0, 4.0, 8.0]).repeat_interleave(375)
+    pool = Pool(dtype, [1500], 2, 64, seed=70)
+    set_keys(pool, keys)
+    # (the scale 16 / 448 is rounded to f32, which moves all scores of a row alike, by 2^-24 of them: that is in lse's 1e-6)
+    assert torch.allclose(pool.val[0][pool.table[0][0], 0, 0, :3], torch.tensor([16.0, 16.0, 1.0]).double(), rtol=2 ** -24, atol=0)
+    cu, plan = pool.plan([new])
+    q = q.to(BF)
+    for block in (0, 1):
+        got, lse = K().paged_attention(q.to(DEV), pool.pages, *plan, block=block, return_lse=True)
+        args = (pool.table, cu, pool.lens, block, 0, 0, SCALE)
+        ref, ref_lse, _ = O.paged_attention(q, *pool.val, *args)
+        mag, _, _ = O.paged_attention(q, pool.val[0], pool.val[1].abs(), *args)
+        close(got, lse, ref, ref_lse, mag, 2 ** -7 * math.log(2))
+    healthy()
