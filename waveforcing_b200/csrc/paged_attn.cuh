@@ -261,13 +261,15 @@ __device__ __forceinline__ bool inside(const Range& r, const TileAt& a) {
 }
 __device__ __forceinline__ bool seen(const Range& r, int pos) { return (pos < r.hi && pos >= r.lo) || pos < r.sink; }
 
-// Whether some tokens see a key of the tile that others do not.  There a V row of
-// bf16 pages may hold a NaN or an infinity that its P of 0 would hand to the others:
-// such elements are taken out and given to the rows that see them.
+// Whether some tokens see keys that others do not, and whether of a tile.  There a V
+// row of bf16 pages may hold a NaN or an infinity that its P of 0 would hand to the
+// others: such elements are taken out and given to the rows that see them.
+__device__ __forceinline__ bool rows_differ(const Range& r) {
+  return r.hi != r.hi_min || r.lo != r.lo_max || r.sink != r.sink_min;
+}
 template <int BN>
 __device__ __forceinline__ bool mixed(const Range& r, const TileAt& a) {
-  return (r.hi != r.hi_min || r.lo != r.lo_max || r.sink != r.sink_min) &&
-         !(a.base + BN <= r.hi_min && (a.base >= r.lo_max || a.base + BN <= r.sink_min));
+  return rows_differ(r) && !(a.base + BN <= r.hi_min && (a.base >= r.lo_max || a.base + BN <= r.sink_min));
 }
 __device__ __forceinline__ uint32_t fma_bf16x2(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t r;

@@ -418,6 +418,7 @@ __global__ void __launch_bounds__(THREADS, 2)
       for (int e = 0; e < 4; ++e) o[k][e] = 0.f;
     float m_run[2] = {-INFINITY, -INFINITY}, m_use[2] = {0.f, 0.f}, l_run[2] = {0.f, 0.f}, v_top = 0.f;
 
+    const bool differ = !KV8 && rows_differ(it.rg);
     for (int i = p0; i < p1; ++i) {
       if (!warp_wait(&full[st], turn, abort_flag, ST_PAGED_ROWS)) break;
       uint8_t* K = ring + st * STAGE + warp * KC * 128;
@@ -519,7 +520,7 @@ __global__ void __launch_bounds__(THREADS, 2)
         }
       }
       if constexpr (!KV8) {
-        if (!whole && mixed<BN>(it.rg, tile_at<BN>(tl, mark.y))) {
+        if (!whole && differ) {
           uint32_t odd = 0;  // rows of V that are not finite: half a warp to a row
 #pragma unroll
           for (int r = lane >> 4; r < KC; r += 2) {

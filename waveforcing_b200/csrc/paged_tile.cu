@@ -382,8 +382,8 @@ __device__ __forceinline__ void store32(void* to, const uint32_t* r, bool wide) 
 }
 
 // Makes the bf16 V tile at v finite; whether it was not (a warp).  Not inlined: in the
-// marks' loop it slowed every call, mixed tiles or none (4680 x 37440 x 12 heads: 1010 us,
-// 907 so, 896 without).
+// marks' loop it slowed calls without mixed tiles too (4680 x 37440 x 12 heads: 1010 us, 907
+// so, 896 without).
 __device__ __noinline__ bool make_finite(uint8_t* v, int lane) {
   v += (lane >> 4) * 128 + ((lane >> 3) & 1) * HALF + (lane & 7) * 16;  // half a warp to a row, 16 bytes a lane
   uint32_t odd[4] = {0, 0, 0, 0};  // sums of 0 * x: 0 or NaN
@@ -405,7 +405,9 @@ __device__ __noinline__ bool make_finite(uint8_t* v, int lane) {
   return true;
 }
 
-template <int DT, bool SORTED>
+// MIXED: bf16 pages of rows that may see different keys (a mask by blocks; without one
+// and in cross attention a row sees what every other does, or nothing).
+template <int DT, bool SORTED, bool MIXED>
 __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
     tile_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ PageMaps tm,
                 const __grid_constant__ Keys ky,
@@ -806,7 +808,7 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
             fence_proxy_async_smem();
             __syncwarp();
           }
-          if (__builtin_expect(mixed<BN>(w, a), 0) && make_finite(ring + s * SLOT, lane) && lane == 0)
+          if (MIXED && __builtin_expect(mixed<BN>(w, a), 0) && make_finite(ring + s * SLOT, lane) && lane == 0)
             odd_v[(work_n - 1) % WORKS] = 1;  // (the softmax holds the item until its end)
           if (lane == 0) mbar_arrive(&full[s]);
         }
@@ -907,7 +909,7 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
         ok = ok && (work_n < WORKS || warp_wait(&work_empty[k], work_n / WORKS - 1, abort_flag, ST_PAGED_WORK));
         if (ok && lane == 0) {
           works[k] = w;
-          if (!KV8) odd_v[k] = 0;
+          if (MIXED) odd_v[k] = 0;
           mbar_arrive(&work_full[k]);
         }
         __syncwarp();
@@ -1141,7 +1143,7 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
               for (int v = 0; v < 32; v += 8) store32(part_o + at * HD + c + v, r + v, tl.wide);
             }
           }
-          if constexpr (!KV8)
+          if constexpr (MIXED)
             if (odd_v[(work_n - 1) % WORKS] && has_row && !none) add_odd(part_o + at * HD);
         }
       } else {
@@ -1161,7 +1163,7 @@ __global__ void __launch_bounds__(Cfg<DT != WF_DTYPE_BF16>::THREADS, 1)
             store32(d + c + 16, o + 8, tl.wide);
           }
         }
-        if constexpr (!KV8)
+        if constexpr (MIXED)
           if (odd_v[(work_n - 1) % WORKS] && has_row && !none) add_odd(d);
       }
       // the next tile's arrival on bar_p lets PV overwrite O, which is in registers here
@@ -1289,7 +1291,7 @@ int64_t parts(const Shape& sh) {
   return s > 1 ? (int64_t)s * sh.rows * sh.H : 0;
 }
 
-template <int DT, bool SORTED>
+template <int DT, bool SORTED, bool MIXED>
 static int start(const CUtensorMap& tq, const PageMaps& tm, const Keys& ky,
                  const Queries& qr, const Tiling& tl, unsigned grid, float* part_o, float* part_l, cudaStream_t st) {
   using C = Cfg<DT != WF_DTYPE_BF16>;
@@ -1297,10 +1299,10 @@ static int start(const CUtensorMap& tq, const PageMaps& tm, const Keys& ky,
   int dev = 0;
   WFK_CUDA_TRY(cudaGetDevice(&dev));
   if (configured != dev) {
-    WFK_CUDA_TRY(cudaFuncSetAttribute(tile_kernel<DT, SORTED>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    WFK_CUDA_TRY(cudaFuncSetAttribute(tile_kernel<DT, SORTED, MIXED>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     configured = dev;
   }
-  tile_kernel<DT, SORTED><<<grid, C::THREADS, C::SMEM, st>>>(tq, tm, ky, qr, tl, part_o, part_l);
+  tile_kernel<DT, SORTED, MIXED><<<grid, C::THREADS, C::SMEM, st>>>(tq, tm, ky, qr, tl, part_o, part_l);
   WFK_CUDA_TRY(cudaGetLastError());
   return WF_OK;
 }
@@ -1336,11 +1338,15 @@ int launch(const Keys& ky, const Queries& qr, const Shape& sh, void* workspace, 
   const int64_t n_parts = parts(sh);
   float* part_o = static_cast<float*>(workspace);
   float* part_l = part_o + n_parts * HD;
+  // (a kernel without the mixed tiles' care: six stages' cross attention 131 us for 135)
+  const bool differ = !ky.cross && qr.block > 0;
   auto pick = [&](auto x) {
     constexpr bool S = decltype(x)::value;
-    return ky.dtype == WF_DTYPE_BF16   ? start<WF_DTYPE_BF16, S>(tq, tm, ky, qr, tl, grid, part_o, part_l, st)
-           : ky.dtype == WF_DTYPE_E4M3 ? start<WF_DTYPE_E4M3, S>(tq, tm, ky, qr, tl, grid, part_o, part_l, st)
-                                       : start<WF_DTYPE_S8, S>(tq, tm, ky, qr, tl, grid, part_o, part_l, st);
+    auto run = [&](auto kernel) { return kernel(tq, tm, ky, qr, tl, grid, part_o, part_l, st); };
+    return ky.dtype == WF_DTYPE_E4M3 ? run(start<WF_DTYPE_E4M3, S, false>)
+           : ky.dtype == WF_DTYPE_S8 ? run(start<WF_DTYPE_S8, S, false>)
+           : differ                  ? run(start<WF_DTYPE_BF16, S, true>)
+                                     : run(start<WF_DTYPE_BF16, S, false>);
   };
   rc = sorted(sh) ? pick(std::true_type{}) : pick(std::false_type{});
   if (rc != WF_OK || n_parts == 0) return rc;
