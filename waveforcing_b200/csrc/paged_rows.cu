@@ -18,9 +18,9 @@
 // distributed shared memory, the ragged batch below took 94 us and the masked
 // cross attention 53.)
 //
-// Measured: 32 ragged sequences of up to 8192 tokens, 40 heads on 8, e4m3: 77 us,
-// 0.54 of the HBM copy rate; 8 x 8192 tokens, 32 heads on 8, bf16: 57 us, 4.7
-// TB/s; 32768 tokens, 12 heads, bf16: 46 us, 4.4 TB/s; 24 x 40 single rows over
+// Measured: 32 ragged sequences of up to 8192 tokens, 40 heads on 8, e4m3: 78 us,
+// 0.53 of the HBM copy rate; 8 x 8192 tokens, 32 heads on 8, bf16: 58 us, 4.6
+// TB/s; 32768 tokens, 12 heads, bf16: 47 us, 4.3 TB/s; 24 x 40 single rows over
 // 257 masked keys: 44 us.  Bound by the start (12,000 clocks to the first data:
 // lengths, page table and pages are loads that wait for each other) and, over
 // 8-bit pages, by each warp's chain of load, expansion and product: 3300 clocks a

@@ -29,15 +29,15 @@
 // 512 bytes a row and tile: 525 against 398 us without at 9472 x 16384 x 4
 // heads, where the rows' reads and the operands' share shared memory.
 //
-// Measured at that size: bf16 247 us, 1288 TFLOP/s (0.77 of the cuBLAS burst
-// rate), e4m3 341 us; 4680 x 37440 x 12 heads: bf16 904 us over 128-row pages
-// and 1000 over 1560-row ones, e4m3 1307 us; 6 x 4680 rows over 512 states and
-// 12 heads 123 us.  A tile takes about 3600 clocks
+// Measured at that size, through the torch wrapper as all figures here: bf16 247
+// us, 1288 TFLOP/s (0.77 of the cuBLAS burst rate), e4m3 315 to 346 us; 4680 x
+// 37440 x 12 heads: bf16 912 us over 128-row pages and 1049 over 1560-row ones
+// masked by blocks, e4m3 1242 to 1314 us; 6 x 4680 rows over 512 states and 12
+// heads 119 us.  A tile takes about 3600 clocks
 // where its products take 2048: a warp's chain from S to P (load, maximum,
 // exponentials, store) is as long as the other sub-tile's products cover.  8-bit
-// pages: the expansion's shared-memory traffic, and the roles' code, which
-// exceeds what the instruction caches hold (stalls for instructions 1.2 an issue
-// against 0.5).
+// pages: the expansion, with twice the instructions (197 against 104 million at
+// that size, issue slots 59 % busy against 42 %) and its shared-memory traffic.
 #include <cuda_fp16.h>
 
 #include <cmath>
@@ -1259,8 +1259,9 @@ static int64_t key_tiles(const Shape& sh) { return tiles_of_keys(sh, BN, !sh.kv8
 static bool dealt(const Shape& sh) { return sh.seqs == 1 && key_tiles(sh) >= 16; }
 
 // Splits of the keys otherwise: the count that gives the least time for the
-// slowest SM, one key tile taking about 1.4 us, an item's start and end about
-// two tiles, and the join its launch and one f32 row written and read a split.
+// slowest SM, one key tile counted as 1.4 us (whole items measure 1.9 over bf16
+// and 2.7 over 8-bit pages), an item's start and end about two tiles, and the join
+// its launch and one f32 row written and read a split.
 static int splits(const Shape& sh) {
   if (dealt(sh)) return 1;
   const int64_t items = tiles_bound(sh) * (sh.H / sh.group), nt = key_tiles(sh);

@@ -550,8 +550,8 @@ class KVPages:
     as bf16 rows, e4m3 codes (uint8) or signed 8-bit codes (int8), the 8-bit
     forms with f32 ``k_scale``, ``v_scale`` [pages, kv_heads, page_size] (a row's
     value is code * scale).  Strides are free (multiples of 16 bytes, the 128
-    elements of a row and the scales of a page contiguous), so pages stored
-    token-major are passed as a transposed view."""
+    elements of a row and the scales of a page contiguous, nothing broadcast), so
+    pages stored token-major are passed as a transposed view."""
 
     __slots__ = ("k", "v", "k_scale", "v_scale", "kv_dtype")
 
@@ -693,7 +693,9 @@ def paged_attention(q: torch.Tensor, pages: KVPages, page_table: torch.Tensor, c
     A row at position p sees keys below hi = min(len, (p // block + 1) * block)
     (block 0: the whole sequence; 1: causal; a chunk's tokens: block-causal);
     with window > 0 only the last ``window`` of those and the first ``sink``.
-    Rows that see nothing are zero.  ``max_new`` / ``max_len`` bound a
+    Rows that see nothing are zero, and what keys that a row does not see hold does
+    not matter to it, NaN included (e4m3 NaN codes, which the write never makes, do).
+    ``max_new`` / ``max_len`` bound a
     sequence's new rows and length where the caller knows them; they steer the
     split of the work only.  Rows behind cu_new[-1] are not written.  With
     ``return_lse`` also the f32 log-sum-exp [rows, H]."""
